@@ -214,6 +214,10 @@ def _positions(s):
     return s["positions"] if s["positions"] is not None else (s["offset"] + torch.arange(N, device=s["x"].device))[None]
 
 
+def _offset(s):
+    return s["offset"] if s["positions"] is None else 0
+
+
 def run(s):
     op = s["op"]
     if own:
@@ -226,9 +230,9 @@ def run(s):
         if op == "decode":
             return fb.decay_linear_decode(s["q"], s["k"], s["v"], s["log_decay"], s["state"], s["scale"]), s["state"]
         if s["grad"]:
-            y = fb.rotary(s["x"], s["freqs"], s["positions"], offset=s["offset"], interleaved=s["interleaved"], scale=s["mag"])
+            y = fb.rotary(s["x"], s["freqs"], s["positions"], offset=_offset(s), interleaved=s["interleaved"], scale=s["mag"])
             return (y.detach(), *torch.autograd.grad(y, s["x"], s["other"]))
-        return fb.rotary_pair(s["x"], s["other"], s["freqs"], s["positions"], offset=s["offset"], interleaved=s["interleaved"], scale=s["mag"])
+        return fb.rotary_pair(s["x"], s["other"], s["freqs"], s["positions"], offset=_offset(s), interleaved=s["interleaved"], scale=s["mag"])
     if op == "prefill":
         y, end = _plain(s["q"], s["k"], s["v"], s["log_decay"], s["scale"], s["state"], s["lengths"])
         return y.to(s["v"].dtype), end
