@@ -8,12 +8,15 @@ from .causal import causal_state_init, flare_causal_decode, flare_causal_mixer, 
 from .mixer import (device_status, pass_counts, flare_gather, flare_multihead_mixer, flare_scatter, mixer_backward,
                     mixer_forward, set_kernel_path)
 from .triple import causal_linear, triple_attention
+from .decay import decay_linear, decay_linear_decode, decay_linear_prefill, decay_linear_state_init
+from .rotary import Rotary, rotary, rotary_frequencies, rotary_pair
 from .modules import FLARE, FLAREBlock, FLAREModel, ResidualMLP
 from .cp_train import ContextParallel, ShardedPointCloud, cp_train_step, enable_context_parallel
 
 __all__ = [
     "flare_multihead_mixer", "flare_gather", "flare_scatter", "mixer_forward", "mixer_backward",
     "set_kernel_path", "device_status", "pass_counts", "flare_causal_prefill", "flare_causal_decode", "flare_causal_mixer", "causal_state_init", "triple_attention",
-    "causal_linear", "FLARE", "FLAREBlock", "FLAREModel", "ResidualMLP",
+    "causal_linear", "decay_linear", "decay_linear_prefill", "decay_linear_decode", "decay_linear_state_init",
+    "rotary", "rotary_pair", "rotary_frequencies", "Rotary", "FLARE", "FLAREBlock", "FLAREModel", "ResidualMLP",
     "ContextParallel", "ShardedPointCloud", "cp_train_step", "enable_context_parallel",
 ]

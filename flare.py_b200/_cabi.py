@@ -38,7 +38,13 @@ class FlarePeers(C.Structure):
                 ("flags", C.c_void_p), ("epoch", C.c_int32)]
 
 
+class FlareDecay(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("B", "H", "N", "Dk", "Dv", "dtype")] + [("scale", C.c_float)] + \
+        [(f"{n}_stride", C.c_int64 * 3) for n in ("q", "k", "v", "y", "dy", "dq", "dk", "dv")]
+
+
 _P = C.POINTER(FlareProblem)
+_D = C.POINTER(FlareDecay)
 _G = C.POINTER(FlarePeers)
 _vp, _i, _sz, _i64 = C.c_void_p, C.c_int, C.c_size_t, C.c_int64
 
@@ -76,6 +82,13 @@ SIGNATURES = {
     "flare_causal_train_bwd": (_i, [_P, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "flare_causal_linear_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "flare_causal_linear": (_i, [_i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "flare_decay_workspace_bytes": (_sz, [_D]),
+    "flare_decay_bwd_workspace_bytes": (_sz, [_D]),
+    "flare_decay_fwd": (_i, [_D, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "flare_decay_bwd": (_i, [_D, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "flare_decay_decode": (_i, [_D, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "flare_rotary": (_i, [_i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i, C.c_float,
+                          _i, _vp]),
     "flare_triple_workspace_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "flare_triple_outer": (_i, [_i, _i, _i, _i, _i, _i, _vp, _vp, _vp, C.c_float, _vp, _vp, _vp]),
     "flare_triple_contract": (_i, [_i, _i, _i, _i, _i, _i, _vp, _i64, _i64, _i64, _vp, _vp, C.c_float, _vp, _vp]),

@@ -284,6 +284,186 @@ Three scatter_bwd(const Tensor& q_, const Tensor& k_, const Tensor& z, const Ten
 }
 
 // ------------------------------------------------------------------------------------------------
+// linear attention with a decay for each head
+// ------------------------------------------------------------------------------------------------
+void same_device(const char* name, const Tensor& t, const Tensor& like) {
+  if (t.device() != like.device()) raise_py(PyExc_ValueError, std::string(name) + " must be on the device of the other operands");
+}
+// What the kernels take in place: unit stride on the last dimension, and for the 16-bit ones, whose tiles are fetched by the
+// tensor memory accelerator, rows it can address.  Where not even a copy has those (D not a multiple of 8), the rows serve.
+Tensor decay_rows(const Tensor& t) {
+  if (t.stride(-1) != 1 && t.size(-1) != 1) return t.contiguous();
+  if (t.element_size() == 2 && t.size(-1) % 8 == 0 && !addressable(t)) return t.contiguous();
+  return t;
+}
+
+// The operands of a call: checked, laid out, and the C description of them.
+struct Decay {
+  Tensor q, k, v, log_decay, lengths;
+  FlareDecay p{};
+  Decay(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& ld, double scale, const optional<Tensor>& len) {
+    for (const Tensor* t : {&q_, &k_, &v_, &ld}) need_cuda(*t);
+    for (const Tensor* t : {&q_, &k_, &v_})
+      if (t->dim() != 4) raise_py(PyExc_ValueError, "q, k, v must be [B,H,N,D]");
+    same_dtype("q, k, v must share a dtype", {&q_, &k_, &v_});
+    if (q_.sizes() != k_.sizes()) raise_py(PyExc_ValueError, "q and k must have the same shape [B,H,N,Dk]");
+    for (int i = 0; i < 3; ++i)
+      if (v_.size(i) != k_.size(i)) raise_py(PyExc_ValueError, "v must agree with q and k in batch, heads and tokens");
+    if (ld.dim() != 1 || ld.size(0) != k_.size(1) || !ld.is_floating_point()) raise_py(PyExc_ValueError, "log_decay must be a floating-point [H] tensor");
+    same_device("q", q_, k_); same_device("v", v_, k_); same_device("log_decay", ld, k_);
+    for (int i = 0; i < 4; ++i)
+      if (k_.size(i) > INT32_MAX) raise_py(PyExc_ValueError, "a dimension exceeds 32 bits");
+    q = decay_rows(q_); k = decay_rows(k_); v = decay_rows(v_);
+    log_decay = ld.to(at::kFloat).contiguous();
+    p.B = (int32_t)k.size(0); p.H = (int32_t)k.size(1); p.N = (int32_t)k.size(2); p.Dk = (int32_t)k.size(3); p.Dv = (int32_t)v.size(3);
+    p.dtype = dtype_code(k);
+    p.scale = (float)scale;
+    set_stride(p.q_stride, q); set_stride(p.k_stride, k); set_stride(p.v_stride, v);
+    if (len.has_value() && len->defined()) {
+      if (len->dim() != 1 || len->size(0) != p.B || (len->scalar_type() != at::kInt && len->scalar_type() != at::kLong))
+        raise_py(PyExc_ValueError, "lengths must be an int32 or int64 [B] tensor");
+      same_device("lengths", *len, k_);
+      // into [0, N] before the change of type, so that no 64-bit length wraps
+      lengths = (len->scalar_type() == at::kInt ? *len : len->clamp(0, p.N).to(at::kInt)).contiguous();
+    }
+  }
+  const int32_t* len() const { return lengths.defined() ? static_cast<const int32_t*>(lengths.data_ptr()) : nullptr; }
+  bool empty() const { return p.B == 0 || p.H == 0 || p.N == 0; }
+  void check_state(const Tensor& s) const {
+    need_cuda(s);
+    same_device("state", s, k);
+    if (s.scalar_type() != at::kFloat || !s.is_contiguous() || s.sizes() != at::IntArrayRef({p.B, p.H, p.Dk, p.Dv}))
+      raise_py(PyExc_ValueError, "state must be a contiguous fp32 [B,H,Dk,Dv] tensor");
+  }
+};
+
+Tensor decay_run(Decay& d, const float* state_in, float* state_out) {
+  Tensor y = like_tokens(d.v);
+  set_stride(d.p.y_stride, y);
+  const size_t bytes = flare_decay_workspace_bytes(&d.p);
+  const Tensor ws = scratch(bytes, d.k);
+  check_rc(flare_decay_fwd(&d.p, d.q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), fp(d.log_decay), d.len(), y.data_ptr(), state_in,
+                           state_out, fp(ws), bytes, stream_of(d.k)), "flare_decay_fwd");
+  return y;
+}
+
+Tensor decay_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale, const optional<Tensor>& lengths) {
+  c10::cuda::CUDAGuard guard(k.device());
+  Decay d(q, k, v, log_decay, scale, lengths);
+  if (d.empty()) return like_tokens(d.v);
+  return decay_run(d, nullptr, nullptr);
+}
+
+Three decay_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& dy_, const Tensor& log_decay, double scale,
+                const optional<Tensor>& lengths) {
+  c10::cuda::CUDAGuard guard(k.device());
+  Decay d(q, k, v, log_decay, scale, lengths);
+  if (dy_.sizes() != v.sizes() || dy_.scalar_type() != v.scalar_type() || dy_.device() != v.device())
+    raise_py(PyExc_ValueError, "dy must have the shape, dtype and device of v");
+  const Tensor dy = decay_rows(dy_);
+  Tensor dq = like_tokens(d.q), dk = like_tokens(d.k), dv = like_tokens(d.v);
+  if (d.empty()) return {dq, dk, dv};
+  set_stride(d.p.dy_stride, dy); set_stride(d.p.dq_stride, dq); set_stride(d.p.dk_stride, dk); set_stride(d.p.dv_stride, dv);
+  const size_t bytes = flare_decay_bwd_workspace_bytes(&d.p);
+  const Tensor ws = scratch(bytes, k);
+  check_rc(flare_decay_bwd(&d.p, d.q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), dy.data_ptr(), fp(d.log_decay), d.len(),
+                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), fp(ws), bytes, stream_of(k)), "flare_decay_bwd");
+  return {dq, dk, dv};
+}
+
+Two decay_prefill(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale, const optional<Tensor>& state,
+                  const optional<Tensor>& lengths) {
+  need_cuda(k);
+  c10::cuda::CUDAGuard guard(k.device());
+  Decay d(q, k, v, log_decay, scale, lengths);
+  Tensor before;
+  if (state.has_value()) {
+    need_cuda(*state);
+    before = state->contiguous();
+    d.check_state(before);
+  }
+  if (d.empty()) {
+    return {like_tokens(d.v), before.defined() ? before.clone() : at::zeros({d.p.B, d.p.H, d.p.Dk, d.p.Dv}, d.k.options().dtype(at::kFloat))};
+  }
+  Tensor after = f32({d.p.B, d.p.H, d.p.Dk, d.p.Dv}, d.k);
+  Tensor y = decay_run(d, before.defined() ? fp(before) : nullptr, fp(after));
+  return {y, after};
+}
+
+Tensor decay_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, double scale,
+                    const optional<Tensor>& lengths) {
+  need_cuda(k);
+  c10::cuda::CUDAGuard guard(k.device());
+  Decay d(q, k, v, log_decay, scale, lengths);
+  d.check_state(state);
+  Tensor y = like_tokens(d.v);
+  if (d.empty()) return y;
+  set_stride(d.p.y_stride, y);
+  check_rc(flare_decay_decode(&d.p, d.q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), fp(d.log_decay), d.len(), y.data_ptr(), fp(state),
+                              stream_of(d.k)), "flare_decay_decode");
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+  return y;
+}
+
+// ------------------------------------------------------------------------------------------------
+// rotary positions
+// ------------------------------------------------------------------------------------------------
+Two rotary_run(const Tensor& q_, const optional<Tensor>& k_, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset,
+               bool interleaved, double scale, bool back) {
+  const bool pair = k_.has_value();
+  for (const Tensor* t : {&q_, pair ? &*k_ : &q_, &freqs}) need_cuda(*t);
+  c10::cuda::CUDAGuard guard(q_.device());
+  if (q_.dim() != 4 || (pair && k_->dim() != 4)) raise_py(PyExc_ValueError, "rotary takes tensors of shape [B,H,N,D]");
+  if (pair) {
+    same_dtype("q and k must share a dtype", {&q_, &*k_});
+    same_device("k", *k_, q_);
+    if (k_->size(0) != q_.size(0) || k_->size(2) != q_.size(2) || k_->size(3) != q_.size(3))
+      raise_py(PyExc_ValueError, "q and k must agree in batch, tokens and features");
+  }
+  const int64_t B = q_.size(0), N = q_.size(2), D = q_.size(3);
+  same_device("freqs", freqs, q_);
+  if (freqs.scalar_type() != at::kDouble || freqs.dim() != 1 || !freqs.is_contiguous()) raise_py(PyExc_ValueError, "freqs must be a contiguous fp64 [R/2] tensor");
+  if (freqs.size(0) < 1 || 2 * freqs.size(0) > D) raise_py(PyExc_ValueError, "freqs rotate " + std::to_string(2 * freqs.size(0)) + " of " + std::to_string(D) + " features");
+  for (int64_t n : {B, N, D, q_.size(1), pair ? k_->size(1) : 0})
+    if (n > INT32_MAX) raise_py(PyExc_ValueError, "a dimension exceeds 32 bits");
+  Tensor pos;
+  int64_t ps[2] = {0, 0};
+  if (positions.has_value() && positions->defined()) {
+    pos = *positions;
+    same_device("positions", pos, q_);
+    if (pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) raise_py(PyExc_ValueError, "positions must be int32 or int64");
+    if (pos.dim() == 1) pos = pos.unsqueeze(0);
+    if (pos.dim() != 2 || (pos.size(0) != B && pos.size(0) != 1) || pos.size(1) != N) raise_py(PyExc_ValueError, "positions must be [N], [1,N] or [B,N]");
+    ps[0] = pos.size(0) == 1 ? 0 : pos.stride(0);
+    ps[1] = pos.stride(1);
+  }
+  auto rows = [](const Tensor& t) { return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); };
+  const Tensor q = rows(q_), k = pair ? rows(*k_) : Tensor();
+  const int dtype = dtype_code(q);
+  Tensor qo = like_tokens(q), ko = pair ? like_tokens(k) : Tensor();
+  // no rows in one of the two: the other is turned alone
+  const bool has_q = q.numel() > 0, has_k = pair && k.numel() > 0;
+  if (!has_q && !has_k) return {qo, ko};
+  const Tensor &first = has_q ? q : k, &first_out = has_q ? qo : ko;
+  const bool both = has_q && has_k;
+  int64_t xs[3], os[3], ks[3], kos[3];
+  set_stride(xs, first); set_stride(os, first_out);
+  if (both) { set_stride(ks, k); set_stride(kos, ko); }
+  check_rc(flare_rotary((int)B, (int)first.size(1), both ? (int)k.size(1) : 0, (int)N, (int)D, (int)(2 * freqs.size(0)), dtype,
+                        first.data_ptr(), xs, first_out.data_ptr(), os, both ? k.data_ptr() : nullptr, ks, both ? ko.data_ptr() : nullptr, kos,
+                        static_cast<const double*>(freqs.data_ptr()), pos.defined() ? pos.data_ptr() : nullptr,
+                        pos.defined() && pos.scalar_type() == at::kInt, ps, offset, interleaved, (float)scale, back, stream_of(q)), "flare_rotary");
+  return {qo, ko};
+}
+Tensor rotary(const Tensor& x, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset, bool interleaved, double scale, bool back) {
+  return std::get<0>(rotary_run(x, std::nullopt, freqs, positions, offset, interleaved, scale, back));
+}
+Two rotary_pair(const Tensor& q, const Tensor& k, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset, bool interleaved,
+                double scale, bool back) {
+  return rotary_run(q, k, freqs, positions, offset, interleaved, scale, back);
+}
+
+// ------------------------------------------------------------------------------------------------
 // operators and autograd
 // ------------------------------------------------------------------------------------------------
 #define FLARE_OP(name)                                                                                        \
@@ -300,6 +480,10 @@ FLARE_OP(gather_fwd)
 FLARE_OP(gather_bwd)
 FLARE_OP(scatter_fwd)
 FLARE_OP(scatter_bwd)
+FLARE_OP(decay_fwd)
+FLARE_OP(decay_bwd)
+FLARE_OP(rotary)
+FLARE_OP(rotary_pair)
 
 // In torch.autocast the latents stay the module's fp32 parameter and meet 16-bit projections here: rounding them
 // inside the operator keeps the cast and its backward out of the autograd graph, and dq is returned in q's own dtype
@@ -444,6 +628,124 @@ Two scatter_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& z, doub
   Tensor lse_n;
   const Tensor y = ScatterFn::apply(q, k, z, scale, key_mask, &lse_n);
   return {y, lse_n};
+}
+
+// ------------------------------------------------------------------------------------------------
+// autograd of the decayed linear attention and of the rotation
+// ------------------------------------------------------------------------------------------------
+void no_gradient_of(const char* what, const Tensor& t) {
+  if (torch::autograd::compute_requires_grad(t)) raise_py(PyExc_NotImplementedError, std::string(what) + " is not differentiated; pass it detached");
+}
+
+class DecayFn : public torch::autograd::Function<DecayFn> {
+ public:
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale,
+                        const optional<Tensor>& lengths) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    Tensor y = Op_decay_fwd::get().call(q, k, v, log_decay, scale, lengths);
+    ctx->save_for_backward({q, k, v, log_decay, lengths.value_or(Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined()) return variable_list(6);
+    const auto s = ctx->get_saved_variables();
+    auto [dq, dk, dv] = Op_decay_bwd::get().call(s[0], s[1], s[2], g[0], s[3], ctx->saved_data["scale"].toDouble(), maybe(s[4]));
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor()};
+  }
+};
+Tensor decay_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale, const optional<Tensor>& lengths) {
+  no_gradient_of("log_decay", log_decay);
+  if (!torch::autograd::compute_requires_grad(q, k, v)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return Op_decay_fwd::get().call(q, k, v, log_decay, scale, lengths);
+  }
+  return DecayFn::apply(q, k, v, log_decay, scale, lengths);
+}
+Three decay_bwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& dy, const Tensor& log_decay, double scale,
+                         const optional<Tensor>& lengths) {
+  Three r;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    r = Op_decay_bwd::get().call(q, k, v, dy, log_decay, scale, lengths);
+  }
+  return no_second_derivative("flare_b200::decay_bwd", std::move(r), q, k, v, dy);
+}
+
+// The gradient of a rotation is the rotation back, so that every derivative is one of these two operators again.
+class RotaryFn : public torch::autograd::Function<RotaryFn> {
+ public:
+  static constexpr bool is_traceable = true;
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset,
+                        bool interleaved, double scale, bool back) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({freqs, positions.value_or(Tensor())});
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["back"] = back;
+    ctx->set_materialize_grads(false);
+    return Op_rotary::get().call(x, freqs, positions, offset, interleaved, scale, back);
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    if (!g[0].defined()) return variable_list(7);
+    const auto s = ctx->get_saved_variables();
+    return {Op_rotary::get().call(g[0], s[0], maybe(s[1]), ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(),
+                                  ctx->saved_data["scale"].toDouble(), !ctx->saved_data["back"].toBool()),
+            Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+class RotaryPairFn : public torch::autograd::Function<RotaryPairFn> {
+ public:
+  static constexpr bool is_traceable = true;
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& freqs, const optional<Tensor>& positions,
+                               int64_t offset, bool interleaved, double scale, bool back) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({freqs, positions.value_or(Tensor())});
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["back"] = back;
+    ctx->set_materialize_grads(false);
+    auto [a, b] = Op_rotary_pair::get().call(q, k, freqs, positions, offset, interleaved, scale, back);
+    return {a, b};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+    variable_list out(8);
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    const int64_t offset = ctx->saved_data["offset"].toInt();
+    const bool interleaved = ctx->saved_data["interleaved"].toBool(), back = !ctx->saved_data["back"].toBool();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    if (g[0].defined() && g[1].defined()) {
+      std::tie(out[0], out[1]) = Op_rotary_pair::get().call(g[0], g[1], s[0], maybe(s[1]), offset, interleaved, scale, back);
+    } else {
+      const int i = g[0].defined() ? 0 : 1;
+      out[i] = Op_rotary::get().call(g[i], s[0], maybe(s[1]), offset, interleaved, scale, back);
+    }
+    return out;
+  }
+};
+Tensor rotary_autograd(const Tensor& x, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset, bool interleaved, double scale,
+                       bool back) {
+  no_gradient_of("freqs", freqs);
+  if (!torch::autograd::compute_requires_grad(x)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return Op_rotary::get().call(x, freqs, positions, offset, interleaved, scale, back);
+  }
+  return RotaryFn::apply(x, freqs, positions, offset, interleaved, scale, back);
+}
+Two rotary_pair_autograd(const Tensor& q, const Tensor& k, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset,
+                         bool interleaved, double scale, bool back) {
+  no_gradient_of("freqs", freqs);
+  if (!torch::autograd::compute_requires_grad(q, k)) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return Op_rotary_pair::get().call(q, k, freqs, positions, offset, interleaved, scale, back);
+  }
+  const variable_list r = RotaryPairFn::apply(q, k, freqs, positions, offset, interleaved, scale, back);
+  return {r[0], r[1]};
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -734,6 +1036,54 @@ FLARE_PY(causal_linear, 3, {
   return THPVariable_Wrap(std::move(y));
 })
 
+FLARE_PY(decay, 6, {
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &ld = tensor_arg(a[3]);
+  const double scale = double_arg(a[4]);
+  const optional<Tensor> lengths = optional_arg(a[5]);
+  for (const Tensor* t : {&q, &k, &v, &ld}) need_cuda(*t);
+  Tensor y;
+  { pybind11::gil_scoped_release nogil; y = Op_decay_fwd::get().call(q, k, v, ld, scale, lengths); }
+  return THPVariable_Wrap(std::move(y));
+})
+FLARE_PY(decay_prefill, 7, {
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &ld = tensor_arg(a[3]);
+  const double scale = double_arg(a[4]);
+  const optional<Tensor> state = optional_arg(a[5]), lengths = optional_arg(a[6]);
+  Two r;
+  { pybind11::gil_scoped_release nogil; at::AutoDispatchBelowADInplaceOrView below; r = decay_prefill(q, k, v, ld, scale, state, lengths); }
+  return pair(std::get<0>(r), std::get<1>(r));
+})
+FLARE_PY(decay_decode, 7, {
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &v = tensor_arg(a[2]), &ld = tensor_arg(a[3]), &state = tensor_arg(a[4]);
+  const double scale = double_arg(a[5]);
+  const optional<Tensor> lengths = optional_arg(a[6]);
+  Tensor y;
+  { pybind11::gil_scoped_release nogil; at::AutoDispatchBelowADInplaceOrView below; y = decay_decode(q, k, v, ld, state, scale, lengths); }
+  return THPVariable_Wrap(std::move(y));
+})
+FLARE_PY(rotary, 6, {
+  const Tensor &x = tensor_arg(a[0]), &freqs = tensor_arg(a[1]);
+  const optional<Tensor> positions = optional_arg(a[2]);
+  const int64_t offset = int_arg(a[3]);
+  const bool interleaved = int_arg(a[4]) != 0;
+  const double scale = double_arg(a[5]);
+  need_cuda(x); need_cuda(freqs);
+  Tensor y;
+  { pybind11::gil_scoped_release nogil; y = Op_rotary::get().call(x, freqs, positions, offset, interleaved, scale, false); }
+  return THPVariable_Wrap(std::move(y));
+})
+FLARE_PY(rotary_pair, 7, {
+  const Tensor &q = tensor_arg(a[0]), &k = tensor_arg(a[1]), &freqs = tensor_arg(a[2]);
+  const optional<Tensor> positions = optional_arg(a[3]);
+  const int64_t offset = int_arg(a[4]);
+  const bool interleaved = int_arg(a[5]) != 0;
+  const double scale = double_arg(a[6]);
+  need_cuda(q); need_cuda(k); need_cuda(freqs);
+  Two r;
+  { pybind11::gil_scoped_release nogil; r = Op_rotary_pair::get().call(q, k, freqs, positions, offset, interleaved, scale, false); }
+  return pair(std::get<0>(r), std::get<1>(r));
+})
+
 PyObject* py_set_error_type(PyObject*, PyObject* type) {
   Py_XINCREF(type);
   Py_XDECREF(g_flare_error);
@@ -743,7 +1093,8 @@ PyObject* py_set_error_type(PyObject*, PyObject* type) {
 
 #define FLARE_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(&py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {FLARE_METHOD(mixer), FLARE_METHOD(causal_prefill), FLARE_METHOD(causal_decode), FLARE_METHOD(causal_mixer),
-                           FLARE_METHOD(triple), FLARE_METHOD(causal_linear), {"set_error_type", py_set_error_type, METH_O, nullptr},
+                           FLARE_METHOD(triple), FLARE_METHOD(causal_linear), FLARE_METHOD(decay), FLARE_METHOD(decay_prefill),
+                           FLARE_METHOD(decay_decode), FLARE_METHOD(rotary), FLARE_METHOD(rotary_pair), {"set_error_type", py_set_error_type, METH_O, nullptr},
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_flare_torch", "flare_b200 operators", -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -756,6 +1107,10 @@ TORCH_LIBRARY(flare_b200, m) {
   m.def("gather_bwd(Tensor q, Tensor k, Tensor v, Tensor dz, Tensor z32, Tensor lse_m, float scale, Tensor? key_mask) -> (Tensor, Tensor, Tensor)");
   m.def("scatter_fwd(Tensor q, Tensor k, Tensor z, float scale, Tensor? key_mask) -> (Tensor, Tensor)");
   m.def("scatter_bwd(Tensor q, Tensor k, Tensor z, Tensor dy, Tensor y, Tensor lse_n, float scale, Tensor? key_mask) -> (Tensor, Tensor, Tensor)");
+  m.def("decay_fwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, float scale, Tensor? lengths) -> Tensor");
+  m.def("decay_bwd(Tensor q, Tensor k, Tensor v, Tensor dy, Tensor log_decay, float scale, Tensor? lengths) -> (Tensor, Tensor, Tensor)");
+  m.def("rotary(Tensor x, Tensor freqs, Tensor? positions, int offset, bool interleaved, float scale, bool back) -> Tensor");
+  m.def("rotary_pair(Tensor q, Tensor k, Tensor freqs, Tensor? positions, int offset, bool interleaved, float scale, bool back) -> (Tensor, Tensor)");
 }
 TORCH_LIBRARY_IMPL(flare_b200, CUDA, m) {
   m.impl("mixer_fwd", &mixer_fwd);
@@ -764,6 +1119,10 @@ TORCH_LIBRARY_IMPL(flare_b200, CUDA, m) {
   m.impl("gather_bwd", &gather_bwd);
   m.impl("scatter_fwd", &scatter_fwd);
   m.impl("scatter_bwd", &scatter_bwd);
+  m.impl("decay_fwd", &decay_fwd);
+  m.impl("decay_bwd", &decay_bwd);
+  m.impl("rotary", &rotary);
+  m.impl("rotary_pair", &rotary_pair);
 }
 TORCH_LIBRARY_IMPL(flare_b200, Autograd, m) {
   m.impl("scatter_bwd", &scatter_bwd_autograd);
@@ -772,6 +1131,10 @@ TORCH_LIBRARY_IMPL(flare_b200, Autograd, m) {
   m.impl("mixer_fwd", &mixer_fwd_autograd);
   m.impl("gather_fwd", &gather_fwd_autograd);
   m.impl("scatter_fwd", &scatter_fwd_autograd);
+  m.impl("decay_fwd", &decay_fwd_autograd);
+  m.impl("decay_bwd", &decay_bwd_autograd);
+  m.impl("rotary", &rotary_autograd);
+  m.impl("rotary_pair", &rotary_pair_autograd);
 }
 
 PyMODINIT_FUNC PyInit__flare_torch(void) { return PyModule_Create(&g_module); }

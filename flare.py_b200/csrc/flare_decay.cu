@@ -1,0 +1,602 @@
+// Linear attention with a decay for each head:  S_t = lambda_h S_{t-1} + k_t v_t^T,  y_t = scale * q_t^T S_t.
+//
+// This file: the C entries, the fp32-arithmetic kernels (fp32 inputs and every shape and alignment the tensor-core ones of
+// flare_decay_tc.cu do not take), the scan over segments, and the single-token form.
+//
+// The token axis is cut into segments, a CTA each.  With one segment a CTA walks its whole sequence; with several, pass 1
+// adds up every segment (sum of lambda^(end-1-n) b_n c_n^T), k_decay_prefix turns the sums into the states before the
+// segments, and pass 2 walks all segments side by side.  A walk takes 64 tokens at a time:
+//     out = (lambda^(i-j) (a_i . b_j))_{j <= i} C  +  lambda^(i+1) A S,      S <- lambda^64 S + (lambda^(63-j) B)^T C
+// The mirror image (n >= t) of the gradients is the same walk over rows taken from the end.
+#include <cstdarg>
+#include <cstdio>
+#include "decay.h"
+#include "launch.h"
+
+namespace flare { void set_last_error(const char* msg); }
+
+namespace flare {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kSub = 64;
+constexpr int kPitchA = kSub + 4;
+
+int refuse(int code, const char* fmt, ...) {
+  char msg[400];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(msg, sizeof(msg), fmt, ap);
+  va_end(ap);
+  set_last_error(msg);
+  return code;
+}
+
+// rows r < 64 of one operand into shared memory as fp32, zeros behind row cnt and column D.  Row r is token tok0 + r * step.
+template <typename T>
+__device__ __forceinline__ void load_rows(float* dst, int pitch, const T* src, long long row_stride, int tok0, int step, int cnt,
+                                          int col0, int cols, int D, bool vec) {
+  const int quads = cols / 4;
+  for (int e = threadIdx.x; e < kSub * quads; e += kThreads) {
+    const int r = e / quads, c = 4 * (e % quads), col = col0 + c;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < cnt && col < D) {
+      const T* p = src + (long long)(tok0 + r * step) * row_stride + col;
+      if (vec) {                                   // D and every stride a multiple of four elements, bases aligned alike
+        if constexpr (sizeof(T) == 4) {
+          x = *reinterpret_cast<const float4*>(p);
+        } else {
+          const uint2 t = *reinterpret_cast<const uint2*>(p);
+          const T* h = reinterpret_cast<const T*>(&t);
+          x = make_float4(to_f32(h[0]), to_f32(h[1]), to_f32(h[2]), to_f32(h[3]));
+        }
+      } else {
+        x.x = to_f32(p[0]);
+        if (col + 1 < D) x.y = to_f32(p[1]);
+        if (col + 2 < D) x.z = to_f32(p[2]);
+        if (col + 3 < D) x.w = to_f32(p[3]);
+      }
+    }
+    *reinterpret_cast<float4*>(dst + r * pitch + c) = x;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ bool quads_aligned(const void* p, const long long (&s)[3], int D) {
+  return reinterpret_cast<uintptr_t>(p) % (4 * sizeof(T)) == 0 && s[0] % 4 == 0 && s[1] % 4 == 0 && s[2] % 4 == 0 && D % 4 == 0;
+}
+
+__device__ __forceinline__ float at4(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// CV columns of a thread: a column block is 16 * CV wide.
+template <int CV>
+__device__ __forceinline__ void load_cv(const float* p, float (&x)[CV]) {
+  if constexpr (CV == 4) {
+    const float4 t = *reinterpret_cast<const float4*>(p);
+    x[0] = t.x; x[1] = t.y; x[2] = t.z; x[3] = t.w;
+  } else {
+    const float2 t = *reinterpret_cast<const float2*>(p);
+    x[0] = t.x; x[1] = t.y;
+  }
+}
+
+// WALK: the outputs (and state_out) of a segment from the state before it.  Otherwise its sum alone.
+// What bounds it: fp32 FMA issue.  Tiles of 4 x 4 results per thread take 8 16-byte loads for 64 multiply-adds; blocks of
+// the masked product above the diagonal are left out.
+template <typename T, int CV, bool WALK>
+__global__ void __launch_bounds__(kThreads, CV == 4 ? 2 : 1) k_decay_simt(const __grid_constant__ DecayArgs a) {
+  grid_dep_sync();
+  constexpr int DVB = 16 * CV;
+  extern __shared__ __align__(16) float sm[];
+  const DecayUnit& u = a.u[blockIdx.z];
+  const int n_cb = (u.Dc + DVB - 1) / DVB;
+  const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = blockIdx.y;
+  if (cb >= n_cb) return;
+  const int b = bh / a.H, h = bh % a.H;
+  const int Da = u.Da, Dap = (Da + 3) & ~3, pitch = Dap + 4, c0 = cb * DVB;
+  float* sS = sm;                                  // [Dap][DVB]
+  float* sB = sS + Dap * DVB;                      // [64][pitch]
+  float* sC = sB + kSub * pitch;                   // [64][DVB]
+  float* sW = sC + kSub * DVB;                     // lambda^0 ... lambda^64
+  float* sQ = sW + 72;                             // [64][pitch]
+  float* sA = sQ + kSub * pitch;                   // [64][kPitchA]
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const float ld = a.log_decay[h];
+  if (tid <= kSub) {
+    const double g = ld < -140.f ? -140.0 : (double)ld;     // NaN stays NaN
+    sW[tid] = (float)exp(g * tid);
+  }
+  const int live = decay_live(a, b);
+  const int n0 = seg * a.seg_len, n1 = min(live, n0 + a.seg_len), n_end = min(a.N, n0 + a.seg_len);
+  const T* pa = static_cast<const T*>(u.a) + b * u.as[0] + h * u.as[1];
+  const T* pb = static_cast<const T*>(u.b) + b * u.bs[0] + h * u.bs[1];
+  const T* pc = static_cast<const T*>(u.c) + b * u.cs[0] + h * u.cs[1];
+  const bool va = WALK && quads_aligned<T>(u.a, u.as, Da), vb = quads_aligned<T>(u.b, u.bs, Da), vc = quads_aligned<T>(u.c, u.cs, u.Dc);
+  const long long st_off = (long long)bh * Da * u.Dc;
+  const float* before = nullptr;                   // the state before the segment
+  if constexpr (WALK) {
+    if (a.n_seg > 1) before = u.seg + ((long long)bh * a.n_seg + seg) * Da * u.Dc;
+    else if (u.state_in) before = u.state_in + st_off;
+  }
+  for (int e = tid; e < Dap * DVB; e += kThreads) {
+    const int d = e / DVB, c = c0 + e % DVB;
+    sS[e] = before && d < Da && c < u.Dc ? before[(long long)d * u.Dc + c] : 0.f;
+  }
+  const DecayStep full(ld, kSub);
+  T* po = nullptr;
+  bool vo = false;
+  if constexpr (WALK) {
+    po = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1];
+    vo = quads_aligned<T>(u.out, u.os, u.Dc);
+  }
+
+  for (int s = 0; n0 + s * kSub < n1; ++s) {
+    const int cnt = min(kSub, n1 - n0 - s * kSub);
+    const int tok0 = u.rev ? n1 - 1 - s * kSub : n0 + s * kSub, step = u.rev ? -1 : 1;
+    __syncthreads();
+    load_rows(sB, pitch, pb, u.bs[2], tok0, step, cnt, 0, Dap, Da, vb);
+    load_rows(sC, DVB, pc, u.cs[2], tok0, step, cnt, c0, DVB, u.Dc, vc);
+    if constexpr (WALK) load_rows(sQ, pitch, pa, u.as[2], tok0, step, cnt, 0, Dap, Da, va);
+    __syncthreads();
+    if constexpr (WALK) {
+      // (a_i . b_j) for j <= i: thread rows i = ty + 16 p, columns j = tx + 16 r; r > p is above the diagonal
+      float acc[4][4] = {};
+      for (int k = 0; k < Dap; k += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const float4*>(sQ + (ty + 16 * p) * pitch + k);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = *reinterpret_cast<const float4*>(sB + (tx + 16 * r) * pitch + k);
+#pragma unroll
+        for (int p = 0; p < 4; ++p)
+#pragma unroll
+          for (int r = 0; r <= p; ++r)
+            acc[p][r] = fmaf(x[p].x, y[r].x, fmaf(x[p].y, y[r].y, fmaf(x[p].z, y[r].z, fmaf(x[p].w, y[r].w, acc[p][r]))));
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int r = 0; r <= p; ++r) {
+          const int i = ty + 16 * p, j = tx + 16 * r;
+          sA[i * kPitchA + j] = j <= i ? acc[p][r] * sW[i - j] : 0.f;
+        }
+      // lambda^(i+1) (A S) first, then the masked product on top
+      float out[4][CV] = {};
+      for (int k = 0; k < Dap; k += 4) {
+        float4 x[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const float4*>(sQ + (ty + 16 * p) * pitch + k);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          float y[CV];
+          load_cv<CV>(sS + (k + kk) * DVB + CV * tx, y);
+#pragma unroll
+          for (int p = 0; p < 4; ++p)
+#pragma unroll
+            for (int c = 0; c < CV; ++c) out[p][c] = fmaf(at4(x[p], kk), y[c], out[p][c]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const float w = sW[ty + 16 * p + 1];
+#pragma unroll
+        for (int c = 0; c < CV; ++c) out[p][c] *= w;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int jb = 0; jb < 4; ++jb)
+        for (int j = 16 * jb; j < 16 * jb + 16; j += 4) {
+          float4 x[4];
+#pragma unroll
+          for (int p = jb; p < 4; ++p) x[p] = *reinterpret_cast<const float4*>(sA + (ty + 16 * p) * kPitchA + j);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            float y[CV];
+            load_cv<CV>(sC + (j + kk) * DVB + CV * tx, y);
+#pragma unroll
+            for (int p = jb; p < 4; ++p)
+#pragma unroll
+              for (int c = 0; c < CV; ++c) out[p][c] = fmaf(at4(x[p], kk), y[c], out[p][c]);
+          }
+        }
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int i = ty + 16 * p, col = c0 + CV * tx;
+        if (i >= cnt || col >= u.Dc) continue;
+        T* o = po + (long long)(tok0 + i * step) * u.os[2] + col;
+        T t[CV];
+#pragma unroll
+        for (int c = 0; c < CV; ++c) t[c] = from_f32<T>(out[p][c] * a.scale);
+        if (vo) {
+          struct alignas(CV * sizeof(T)) Pack { T x[CV]; };
+          *reinterpret_cast<Pack*>(o) = *reinterpret_cast<const Pack*>(t);
+        } else {
+#pragma unroll
+          for (int c = 0; c < CV; ++c)
+            if (col + c < u.Dc) o[c] = t[c];
+        }
+      }
+      __syncthreads();                             // the products with S are done
+    }
+    const DecayStep decay = cnt == kSub ? full : DecayStep(ld, cnt);
+    for (int k0 = 4 * ty; k0 < Dap; k0 += 64) {
+      float acc[4][CV] = {};
+      for (int i = 0; i < cnt; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(sB + i * pitch + k0);
+        const float w = sW[cnt - 1 - i];
+        float y[CV];
+        load_cv<CV>(sC + i * DVB + CV * tx, y);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          const float xw = at4(x, p) * w;
+#pragma unroll
+          for (int c = 0; c < CV; ++c) acc[p][c] = fmaf(xw, y[c], acc[p][c]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int c = 0; c < CV; ++c) {
+          float* e = sS + (k0 + p) * DVB + CV * tx + c;
+          *e = decay(*e) + acc[p][c];
+        }
+    }
+  }
+  __syncthreads();
+  float* end = nullptr;
+  if constexpr (WALK) {
+    if (u.state_out && seg == a.n_seg - 1) end = u.state_out + st_off;
+    const int z0 = max(n0, live);                  // rows behind the sequence: zeros
+    for (int e = tid; e < (n_end - z0) * DVB; e += kThreads) {
+      const int c = c0 + e % DVB;
+      if (c < u.Dc) po[(long long)(z0 + e / DVB) * u.os[2] + c] = from_f32<T>(0.f);
+    }
+  } else {
+    end = u.seg + ((long long)bh * a.n_seg + seg) * Da * u.Dc;
+  }
+  if (end)
+    for (int e = tid; e < Da * DVB; e += kThreads) {
+      const int d = e / DVB, c = c0 + e % DVB;
+      if (c < u.Dc) end[(long long)d * u.Dc + c] = sS[e];
+    }
+}
+
+// sums of the segments -> states before them, in place.  A thread owns one element of one (unit, b, h).
+__global__ void __launch_bounds__(256) k_decay_prefix(const __grid_constant__ DecayArgs a) {
+  grid_dep_sync();
+  const DecayUnit& u = a.u[blockIdx.y];
+  const long long per = (long long)u.Da * u.Dc;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)a.B * a.H * per) return;
+  const int bh = (int)(i / per), b = bh / a.H, h = bh % a.H;
+  float* s = u.seg + (long long)bh * a.n_seg * per + i % per;
+  float run = u.state_in ? u.state_in[i] : 0.f;
+  const float ld = a.log_decay[h];
+  const int live = decay_live(a, b);
+  const DecayStep full(ld, a.seg_len);
+  auto add = [&](int seg, float sum) {
+    const int cnt = min(a.seg_len, live - seg * a.seg_len);
+    if (cnt == a.seg_len) run = full(run) + sum;
+    else if (cnt > 0) run = DecayStep(ld, cnt)(run) + sum;
+  };
+  constexpr int kAhead = 8;                        // loads in flight: a segment's addition waits for the one before it
+  for (int s0 = 0; s0 < a.n_seg; s0 += kAhead) {
+    float x[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int seg = u.rev ? a.n_seg - 1 - s0 - j : s0 + j;
+      x[j] = s0 + j < a.n_seg ? s[(long long)seg * per] : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (s0 + j >= a.n_seg) break;
+      const int seg = u.rev ? a.n_seg - 1 - s0 - j : s0 + j;
+      s[(long long)seg * per] = run;
+      add(seg, x[j]);
+    }
+  }
+}
+
+// ---- single tokens ---------------------------------------------------------------------------------------------------
+// One CTA per (b, h, block of columns); the state stays in registers over the T tokens, so a call reads and writes it once.
+// A thread holds kRows quads of four columns: all its loads are in flight before the first is used (the time is the state's
+// way through HBM, 8 bytes an element).
+constexpr int kDecThreads = 256;
+
+struct DecodeArgs {
+  int B, H, T, Dk, Dv;
+  int lanes;                                       // threads beside one another on a row (a power of two): 4 * lanes columns
+  float scale;
+  const float* log_decay;
+  const int* lengths;
+  const void *q, *k, *v;
+  void* y;
+  long long qs[3], ks[3], vs[3], ys[3];
+  float* state;
+};
+
+template <typename T, int ROWS, bool VEC>
+__global__ void __launch_bounds__(kDecThreads) k_decay_decode(const __grid_constant__ DecodeArgs a) {
+  grid_dep_sync();
+  __shared__ float sQ[256], sK[256];
+  __shared__ float4 sY[kDecThreads];
+  const int bh = blockIdx.x, b = bh / a.H, h = bh % a.H, tid = threadIdx.x;
+  const int lane = tid & (a.lanes - 1), row0 = tid / a.lanes, per_row = kDecThreads / a.lanes;
+  const int col = 4 * (blockIdx.y * a.lanes + lane);
+  const int live = a.lengths ? max(0, min(a.T, a.lengths[b])) : a.T;
+  const T* pq = static_cast<const T*>(a.q) + b * a.qs[0] + h * a.qs[1];
+  const T* pk = static_cast<const T*>(a.k) + b * a.ks[0] + h * a.ks[1];
+  const T* pv = static_cast<const T*>(a.v) + b * a.vs[0] + h * a.vs[1];
+  T* py = static_cast<T*>(a.y) + b * a.ys[0] + h * a.ys[1];
+  float* st = a.state + (long long)bh * a.Dk * a.Dv;
+  float4 S[ROWS];
+  if (live > 0) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int d = row0 + r * per_row;
+      S[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (d >= a.Dk) continue;
+      const float* p = st + (long long)d * a.Dv + col;
+      if constexpr (VEC) {
+        if (col < a.Dv) S[r] = *reinterpret_cast<const float4*>(p);
+      } else {
+        if (col < a.Dv) S[r].x = p[0];
+        if (col + 1 < a.Dv) S[r].y = p[1];
+        if (col + 2 < a.Dv) S[r].z = p[2];
+        if (col + 3 < a.Dv) S[r].w = p[3];
+      }
+    }
+  }
+  const DecayStep decay(a.log_decay[h], 1);
+  for (int t = 0; t < a.T; ++t) {
+    T* o = py + (long long)t * a.ys[2];
+    if (t >= live) {                               // tokens behind the sequence: zeros, the state as it is
+      if (row0 == 0)
+        for (int c = 0; c < 4; ++c)
+          if (col + c < a.Dv) o[col + c] = from_f32<T>(0.f);
+      continue;
+    }
+    for (int d = tid; d < a.Dk; d += kDecThreads) {
+      sQ[d] = to_f32(pq[(long long)t * a.qs[2] + d]);
+      sK[d] = to_f32(pk[(long long)t * a.ks[2] + d]);
+    }
+    float v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = col + c < a.Dv ? to_f32(pv[(long long)t * a.vs[2] + col + c]) : 0.f;
+    __syncthreads();
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int d = row0 + r * per_row;
+      if (d >= a.Dk) continue;
+      const float k = sK[d], q = sQ[d];
+      S[r].x = fmaf(k, v[0], decay(S[r].x)); S[r].y = fmaf(k, v[1], decay(S[r].y));
+      S[r].z = fmaf(k, v[2], decay(S[r].z)); S[r].w = fmaf(k, v[3], decay(S[r].w));
+      y.x = fmaf(q, S[r].x, y.x); y.y = fmaf(q, S[r].y, y.y); y.z = fmaf(q, S[r].z, y.z); y.w = fmaf(q, S[r].w, y.w);
+    }
+    sY[tid] = y;
+    __syncthreads();
+    for (int half = per_row / 2; half > 0; half /= 2) {      // the rows' shares, in a fixed order
+      if (row0 < half) {
+        const float4 x = sY[tid + half * a.lanes];
+        y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w;
+        sY[tid] = y;
+      }
+      __syncthreads();
+    }
+    if (row0 == 0) {
+      const float r[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (col + c < a.Dv) o[col + c] = from_f32<T>(r[c] * a.scale);
+    }
+  }
+  if (live > 0) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const int d = row0 + r * per_row;
+      if (d >= a.Dk) continue;
+      float* p = st + (long long)d * a.Dv + col;
+      if constexpr (VEC) {
+        if (col < a.Dv) *reinterpret_cast<float4*>(p) = S[r];
+      } else {
+        if (col < a.Dv) p[0] = S[r].x;
+        if (col + 1 < a.Dv) p[1] = S[r].y;
+        if (col + 2 < a.Dv) p[2] = S[r].z;
+        if (col + 3 < a.Dv) p[3] = S[r].w;
+      }
+    }
+  }
+}
+
+template <typename T>
+int run_decode(const DecodeArgs& a0, cudaStream_t st) {
+  DecodeArgs a = a0;
+  // columns of a CTA: as many as its threads can hold at 16 quads each
+  auto rows_of = [&](int lanes) { return (a.Dk + kDecThreads / lanes - 1) / (kDecThreads / lanes); };
+  int lanes = 1;
+  while (4 * lanes < a.Dv && rows_of(2 * lanes) <= 16) lanes *= 2;
+  a.lanes = lanes;
+  const int rows = rows_of(lanes);
+  const dim3 grid((unsigned)(a.B * a.H), (unsigned)((a.Dv + 4 * lanes - 1) / (4 * lanes)));
+  const bool vec = a.Dv % 4 == 0 && reinterpret_cast<uintptr_t>(a.state) % 16 == 0;
+  auto go = [&](auto kernel) { launch_dep(kernel, grid, dim3(kDecThreads), 0, st, a); };
+  if (rows <= 4) vec ? go(k_decay_decode<T, 4, true>) : go(k_decay_decode<T, 4, false>);
+  else vec ? go(k_decay_decode<T, 16, true>) : go(k_decay_decode<T, 16, false>);
+  return FLARE_OK;
+}
+
+// ---- host side -------------------------------------------------------------------------------------------------------
+int pick_segments(int B, int H, int N, int Dc, int n_units) {
+  const int cb = (Dc + 63) / 64;
+  const long long ctas = (long long)B * H * cb * n_units;
+  long long s = (2LL * num_sms() + ctas - 1) / ctas;         // two CTAs' worth of work per SM
+  const long long max_s = ((long long)N + 2 * kSub - 1) / (2 * kSub);
+  if (s > max_s) s = max_s;
+  if (s > 256) s = 256;
+  return s < 1 ? 1 : (int)s;
+}
+
+size_t simt_smem(int Da, int CV, bool walk) {
+  const int Dap = (Da + 3) & ~3, DVB = 16 * CV;
+  const size_t f = (size_t)Dap * DVB + kSub * (Dap + 4) + kSub * DVB + 72 + (walk ? kSub * (Dap + 4) + kSub * kPitchA : 0);
+  return f * sizeof(float);
+}
+
+template <typename T, int CV>
+int run_simt_cv(const DecayArgs& a, int Da, int Dc, cudaStream_t st) {
+  const int cb = (Dc + 16 * CV - 1) / (16 * CV);
+  const dim3 grid((unsigned)(a.B * a.H * cb), (unsigned)a.n_seg, (unsigned)a.n_units);
+  const size_t sm_w = simt_smem(Da, CV, true), sm_s = simt_smem(Da, CV, false);
+  if (tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_simt<T, CV, true>), 227 * 1024) != FLARE_OK ||
+      tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_simt<T, CV, false>), 227 * 1024) != FLARE_OK)
+    return refuse(FLARE_ECUDA, "decay: cudaFuncSetAttribute failed");
+  if (a.n_seg > 1) {
+    launch_dep(k_decay_simt<T, CV, false>, grid, dim3(kThreads), sm_s, st, a);
+    launch_decay_prefix(a, st);
+  }
+  launch_dep(k_decay_simt<T, CV, true>, grid, dim3(kThreads), sm_w, st, a);
+  return FLARE_OK;
+}
+
+// column blocks of 64 where the tiles of Da <= 128 features leave room for two CTAs per SM or one, else of 32
+template <typename T>
+int run_simt(const DecayArgs& a, int Da, int Dc, cudaStream_t st) {
+  return Dc > 32 && Da <= 128 ? run_simt_cv<T, 4>(a, Da, Dc, st) : run_simt_cv<T, 2>(a, Da, Dc, st);
+}
+
+int check_problem(const char* what, const FlareDecay* p) {
+  if (!p) return refuse(FLARE_EINVAL, "%s: null problem", what);
+  if (p->B < 1 || p->H < 1 || p->N < 1) return refuse(FLARE_EINVAL, "%s: bad sizes B=%d H=%d N=%d", what, p->B, p->H, p->N);
+  if (p->Dk < 1 || p->Dv < 1 || p->Dk > 256 || p->Dv > 256)
+    return refuse(FLARE_EUNSUPPORTED, "%s: Dk=%d Dv=%d, both must be 1 to 256", what, p->Dk, p->Dv);
+  if (p->dtype != FLARE_F32 && p->dtype != FLARE_F16 && p->dtype != FLARE_BF16) return refuse(FLARE_EINVAL, "%s: bad dtype %d", what, p->dtype);
+  if ((long long)p->B * p->H > (1 << 24)) return refuse(FLARE_EUNSUPPORTED, "%s: B*H > 2^24", what);
+  if (p->N > (1 << 30)) return refuse(FLARE_EUNSUPPORTED, "%s: N > 2^30", what);
+  return FLARE_OK;
+}
+
+DecayArgs base_args(const FlareDecay* p, const float* log_decay, const int* lengths) {
+  DecayArgs a = {};
+  a.B = p->B; a.H = p->H; a.N = p->N;
+  a.scale = p->scale;
+  a.log_decay = log_decay;
+  a.lengths = lengths;
+  return a;
+}
+
+void set(long long (&dst)[3], const int64_t* s) { for (int i = 0; i < 3; ++i) dst[i] = s[i]; }
+
+DecayUnit unit(const void* x, const int64_t* xs, const void* y, const int64_t* ys, const void* z, const int64_t* zs, void* out,
+               const int64_t* os, int Da, int Dc, int rev) {
+  DecayUnit u = {};
+  u.a = x; u.b = y; u.c = z; u.out = out;
+  set(u.as, xs); set(u.bs, ys); set(u.cs, zs); set(u.os, os);
+  u.Da = Da; u.Dc = Dc; u.rev = rev;
+  return u;
+}
+
+// Segments and workspace follow from the sizes alone, for either family, so that the size asked for fits both.
+int seg_max(const FlareDecay* p, int units) {
+  const int D = p->Dk > p->Dv ? p->Dk : p->Dv;
+  int s = pick_segments(p->B, p->H, p->N, units == 1 ? p->Dv : D, units);
+  const int t = decay_tc_segments(p->B, p->H, p->N, units == 1 ? p->Dk : D, units == 1 ? p->Dv : D, units);
+  return s > t ? s : t;
+}
+size_t ws_bytes(const FlareDecay* p, int units) {
+  const int s = seg_max(p, units);
+  return s > 1 ? (size_t)units * p->B * p->H * s * p->Dk * p->Dv * sizeof(float) : 0;
+}
+
+int run(DecayArgs& a, const FlareDecay* p, float* ws, cudaStream_t st, const char* what) {
+  int Da = 0, Dc = 0;
+  for (int i = 0; i < a.n_units; ++i) {
+    Da = a.u[i].Da > Da ? a.u[i].Da : Da;
+    Dc = a.u[i].Dc > Dc ? a.u[i].Dc : Dc;
+  }
+  const bool tc = decay_tc_supported(a, p->dtype);
+  int n = tc ? decay_tc_segments(p->B, p->H, p->N, Da, Dc, a.n_units) : pick_segments(p->B, p->H, p->N, Dc, a.n_units);
+  const int block = tc ? 128 : kSub;
+  a.seg_len = (int)((((long long)p->N + n - 1) / n + block - 1) / block) * block;
+  a.n_seg = (p->N + a.seg_len - 1) / a.seg_len;
+  for (int i = 0; i < a.n_units; ++i) a.u[i].seg = ws + (size_t)i * p->B * p->H * a.n_seg * p->Dk * p->Dv;
+  int rc;
+  if (tc) rc = decay_tc(a, p->dtype, st);
+  else if (p->dtype == FLARE_F32) rc = run_simt<float>(a, Da, Dc, st);
+  else if (p->dtype == FLARE_F16) rc = run_simt<__half>(a, Da, Dc, st);
+  else rc = run_simt<__nv_bfloat16>(a, Da, Dc, st);
+  if (rc != FLARE_OK) return refuse(rc, "%s: the kernels could not be launched", what);
+  const cudaError_t e = cudaPeekAtLastError();
+  if (e != cudaSuccess) return refuse(FLARE_ECUDA, "%s: %s", what, cudaGetErrorString(e));
+  return FLARE_OK;
+}
+
+}  // namespace
+
+void launch_decay_prefix(const DecayArgs& a, cudaStream_t st) {
+  const long long n = (long long)a.B * a.H * a.u[0].Da * a.u[0].Dc;        // Da * Dc is Dk * Dv for every unit
+  launch_dep(k_decay_prefix, dim3((unsigned)((n + 255) / 256), (unsigned)a.n_units), dim3(256), 0, st, a);
+}
+
+}  // namespace flare
+
+using namespace flare;
+
+extern "C" {
+
+size_t flare_decay_workspace_bytes(const FlareDecay* p) { return check_problem("decay", p) == FLARE_OK ? ws_bytes(p, 1) : 0; }
+size_t flare_decay_bwd_workspace_bytes(const FlareDecay* p) { return check_problem("decay_bwd", p) == FLARE_OK ? ws_bytes(p, 3) : 0; }
+
+int flare_decay_fwd(const FlareDecay* p, const void* q, const void* k, const void* v, const float* log_decay,
+                    const int32_t* lengths, void* y, const float* state_in, float* state_out, float* workspace,
+                    size_t workspace_bytes, flare_stream_t stream) {
+  if (int rc = check_problem("decay", p)) return rc;
+  if (!q || !k || !v || !y || !log_decay) return refuse(FLARE_EINVAL, "decay: null pointer");
+  const size_t need = ws_bytes(p, 1);
+  if (need && (!workspace || workspace_bytes < need)) return refuse(FLARE_EWORKSPACE, "decay: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return refuse(FLARE_EALIGN, "decay: workspace must be 16-byte aligned");
+  DecayArgs a = base_args(p, log_decay, lengths);
+  a.n_units = 1;
+  a.u[0] = unit(q, p->q_stride, k, p->k_stride, v, p->v_stride, y, p->y_stride, p->Dk, p->Dv, 0);
+  a.u[0].state_in = state_in;
+  a.u[0].state_out = state_out;
+  return run(a, p, workspace, static_cast<cudaStream_t>(stream), "decay");
+}
+
+int flare_decay_bwd(const FlareDecay* p, const void* q, const void* k, const void* v, const void* dy, const float* log_decay,
+                    const int32_t* lengths, void* dq, void* dk, void* dv, float* workspace, size_t workspace_bytes,
+                    flare_stream_t stream) {
+  if (int rc = check_problem("decay_bwd", p)) return rc;
+  if (!q || !k || !v || !dy || !dq || !dk || !dv || !log_decay) return refuse(FLARE_EINVAL, "decay_bwd: null pointer");
+  const size_t need = ws_bytes(p, 3);
+  if (need && (!workspace || workspace_bytes < need)) return refuse(FLARE_EWORKSPACE, "decay_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return refuse(FLARE_EALIGN, "decay_bwd: workspace must be 16-byte aligned");
+  DecayArgs a = base_args(p, log_decay, lengths);
+  a.n_units = 3;
+  a.u[0] = unit(dy, p->dy_stride, v, p->v_stride, k, p->k_stride, dq, p->dq_stride, p->Dv, p->Dk, 0);
+  a.u[1] = unit(v, p->v_stride, dy, p->dy_stride, q, p->q_stride, dk, p->dk_stride, p->Dv, p->Dk, 1);
+  a.u[2] = unit(k, p->k_stride, q, p->q_stride, dy, p->dy_stride, dv, p->dv_stride, p->Dk, p->Dv, 1);
+  return run(a, p, workspace, static_cast<cudaStream_t>(stream), "decay_bwd");
+}
+
+int flare_decay_decode(const FlareDecay* p, const void* q, const void* k, const void* v, const float* log_decay,
+                       const int32_t* lengths, void* y, float* state, flare_stream_t stream) {
+  if (int rc = check_problem("decay_decode", p)) return rc;
+  if (!q || !k || !v || !y || !log_decay || !state) return refuse(FLARE_EINVAL, "decay_decode: null pointer");
+  DecodeArgs a = {};
+  a.B = p->B; a.H = p->H; a.T = p->N; a.Dk = p->Dk; a.Dv = p->Dv;
+  a.scale = p->scale;
+  a.log_decay = log_decay; a.lengths = lengths;
+  a.q = q; a.k = k; a.v = v; a.y = y;
+  set(a.qs, p->q_stride); set(a.ks, p->k_stride); set(a.vs, p->v_stride); set(a.ys, p->y_stride);
+  a.state = state;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p->dtype == FLARE_F32) run_decode<float>(a, st);
+  else if (p->dtype == FLARE_F16) run_decode<__half>(a, st);
+  else run_decode<__nv_bfloat16>(a, st);
+  const cudaError_t e = cudaPeekAtLastError();
+  if (e != cudaSuccess) return refuse(FLARE_ECUDA, "decay_decode: %s", cudaGetErrorString(e));
+  return FLARE_OK;
+}
+
+}  // extern "C"

@@ -290,6 +290,53 @@ int flare_causal_linear(int B, int H, int N, int Dk, int Dv, int dtype, const vo
                         const void* k, const int64_t* k_stride, const void* v, const int64_t* v_stride,
                         void* y, const int64_t* y_stride, float* workspace, flare_stream_t stream);
 
+/* Linear attention with a decay for each head, lambda_h = exp(log_decay[h]):
+ *   S_t = lambda S_{t-1} + k_t v_t^T,   y_t = scale * q_t^T S_t        (S_{-1} = state_in, zero if NULL)
+ * i.e. y_t = scale * sum_{n<=t} lambda^(t-n) (q_t . k_n) v_n.  The reference has the form without a decay only
+ * (lra/models/triton/causal_linear.py:23-145).  q, k: [B,H,N,Dk], v, y: [B,H,N,Dv], unit stride on the last dimension,
+ * any element strides for b, h, n; Dk and Dv up to 256; states are contiguous fp32 [B,H,Dk,Dv].  log_decay: fp32 [H],
+ * usually <= 0 (0 = no decay, -inf = the token itself alone).  lengths: int32 [B] or NULL; tokens at or behind
+ * lengths[b] (taken into [0, N]) leave the state alone, have outputs and gradients of zero and may hold anything,
+ * NaN included.
+ *   flare_decay_fwd:    all N tokens.  state_in may be NULL (empty), state_out may be NULL; they may be the same buffer.
+ *   flare_decay_bwd:    dq, dk, dv of an empty prefix from dy: the same sum with the roles exchanged,
+ *     dq_t = scale sum_{n<=t} lambda^(t-n) (dy_t . v_n) k_n,  dk_n = scale sum_{t>=n} lambda^(t-n) (v_n . dy_t) q_t,
+ *     dv_n = scale sum_{t>=n} lambda^(t-n) (k_n . q_t) dy_t.
+ *   flare_decay_decode: the N tokens (usually N = 1) one after the other on `state`, updated in place.
+ * 16-bit inputs with Dk, Dv (and in the backward both) up to 128 and 16-byte aligned rows run on the tensor cores, the
+ * rest on fp32 kernels.  fp16 products q.k must stay within fp16's range.  Workspaces: the two functions' bytes, 0 when a
+ * problem needs none. */
+typedef struct FlareDecay {
+  int32_t B, H, N, Dk, Dv;
+  int32_t dtype;                 /* of q, k, v, y, dy, dq, dk, dv */
+  float   scale;
+  int64_t q_stride[3], k_stride[3], v_stride[3], y_stride[3];     /* b, h, n (elements) */
+  int64_t dy_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} FlareDecay;
+size_t flare_decay_workspace_bytes(const FlareDecay* p);
+size_t flare_decay_bwd_workspace_bytes(const FlareDecay* p);
+int flare_decay_fwd(const FlareDecay* p, const void* q, const void* k, const void* v, const float* log_decay,
+                    const int32_t* lengths, void* y, const float* state_in, float* state_out, float* workspace,
+                    size_t workspace_bytes, flare_stream_t stream);
+int flare_decay_bwd(const FlareDecay* p, const void* q, const void* k, const void* v, const void* dy, const float* log_decay,
+                    const int32_t* lengths, void* dq, void* dk, void* dv, float* workspace, size_t workspace_bytes,
+                    flare_stream_t stream);
+int flare_decay_decode(const FlareDecay* p, const void* q, const void* k, const void* v, const float* log_decay,
+                       const int32_t* lengths, void* y, float* state, flare_stream_t stream);
+
+/* Rotary positions (the reference applies them to k, lra/models/embeddings.py and backends.py:599-600): for i < R/2 the
+ * pair (x0, x1) = (x[i], x[i + R/2]), or (x[2i], x[2i + 1]) when `interleaved`, becomes
+ * mag * (x0 cos t - x1 sin t, x0 sin t + x1 cos t) with t = position * freqs[i]; features R ... D-1 are copied.  `back`
+ * turns the other way (the gradient).  q [B,Hq,N,D] and, unless NULL, k [B,Hk,N,D] in one launch; unit stride on D, any
+ * strides for b, h, n; an output may be its input.  freqs: DEVICE fp64 [R/2], radians per position (angles are formed in 64
+ * bits).  Token n of batch entry b stands at positions[b * position_stride[0] + n * position_stride[1]] + offset (int64, or
+ * int32), or at n + offset where positions is NULL. */
+int flare_rotary(int B, int Hq, int Hk, int N, int D, int R, int dtype, const void* q, const int64_t* q_stride, void* q_out,
+                 const int64_t* q_out_stride, const void* k, const int64_t* k_stride, void* k_out,
+                 const int64_t* k_out_stride, const double* freqs, const void* positions, int positions_are_int32,
+                 const int64_t* position_stride, int64_t offset, int interleaved, float mag, int back,
+                 flare_stream_t stream);
+
 /* Triple attention (lra/models/triton/triple.py:27-290; einsum references :846-860, :887-931) as the two
  * shapes of work its forward and backward are made of.  Inputs are [BH, N, D] contiguous in `dtype`,
  * as the reference makes them (triple.py:51-55); tensors of rank 3 are fp32.

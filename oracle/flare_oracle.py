@@ -461,3 +461,51 @@ def make_inputs(B, H, N, M, D, dtype=torch.float32, seed=0, std_pow=-0.25, q4d=F
     v = torch.randn(B, H, N, D, generator=g) * sd
     dy = torch.randn(B, H, N, D, generator=g)
     return tuple(t.to(dtype) for t in (q, k, v, dy))
+
+
+# ---------------------------------------------------------------------------------------------------
+# linear attention with a decay for each head, and rotary positions
+# ---------------------------------------------------------------------------------------------------
+def decay_linear_recurrent(q, k, v, log_decay, scale=1.0, state=None, lengths=None):
+    """Token by token in fp64: S <- lambda S + k v^T, y = scale q^T S.  Returns (y, state)."""
+    q, k, v, lam = q.double(), k.double(), v.double(), torch.exp(log_decay.double())
+    B, H, N, Dk = q.shape
+    S = torch.zeros(B, H, Dk, v.shape[-1], dtype=torch.float64, device=q.device) if state is None else state.double().clone()
+    y = torch.zeros(B, H, N, v.shape[-1], dtype=torch.float64, device=q.device)
+    for t in range(N):
+        S1 = lam[:, None, None] * S + k[:, :, t, :, None] * v[:, :, t, None, :]
+        y1 = scale * (q[:, :, t, None, :] @ S1)[:, :, 0]
+        if lengths is None:
+            S, y[:, :, t] = S1, y1
+        else:
+            live = (t < lengths)[:, None, None]
+            S = torch.where(live[..., None], S1, S)
+            y[:, :, t] = torch.where(live, y1, torch.zeros_like(y1))
+    return y, S
+
+
+def decay_linear_dense(q, k, v, log_decay, scale=1.0, lengths=None):
+    """y = scale * (lambda^(t-n) q_t.k_n)_{n<=t} V as one masked product; differentiable, in the inputs' own dtype."""
+    N = q.shape[2]
+    t = torch.arange(N, device=q.device)
+    d = t[:, None] - t[None, :]
+    ld = log_decay.to(q.dtype)[:, None, None]
+    w = torch.where(d == 0, torch.ones_like(ld * d), torch.exp(ld * d.clamp(min=1)))
+    A = torch.where(d >= 0, (q @ k.transpose(-1, -2)) * w, torch.zeros((), dtype=q.dtype, device=q.device))
+    if lengths is not None:
+        live = t[None, :] < lengths[:, None]
+        A = torch.where((live[:, :, None] & live[:, None, :])[:, None], A, torch.zeros((), dtype=q.dtype, device=q.device))
+    return scale * (A @ v)
+
+
+def rotary_complex(x, freqs, positions, interleaved=False, scale=1.0, back=False):
+    """The rotation as a complex product in fp64; positions [N] or [B,N]."""
+    half = freqs.numel()
+    pos = positions.double()
+    angle = (pos[None] if pos.dim() == 1 else pos)[:, None, :, None] * freqs.double()
+    turn = scale * torch.polar(torch.ones_like(angle), -angle if back else angle)
+    r, rest = x.double()[..., :2 * half], x.double()[..., 2 * half:]
+    z = torch.complex(r[..., 0::2], r[..., 1::2]) if interleaved else torch.complex(r[..., :half], r[..., half:])
+    z = z * turn
+    r = torch.stack((z.real, z.imag), -1).flatten(-2) if interleaved else torch.cat((z.real, z.imag), -1)
+    return torch.cat((r, rest), -1)
