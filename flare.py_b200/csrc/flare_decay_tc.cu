@@ -1,18 +1,23 @@
 // Decayed linear attention on the tensor cores: 16-bit operands, up to 128 features in a and b, any number in c (in blocks of
-// 64 columns).  One CTA walks a segment of one (unit, b, h, column block) in chunks of 128 tokens:
+// 64 columns).  A sequence (one unit, b, h, column block) is taken in chunks of 128 tokens:
 //
 //   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 256 threads weigh, mask and pack it there
 //   out = scale * (P C + lambda^(i+1) A X)          X: the state before the chunk, in two 16-bit terms; two accumulators
-//   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms; X itself in fp32 registers
+//   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms; X itself in fp32
 //
 // The mirror image in time (n >= t) walks the chunks from the last and mirrors the weights.
 //
-// Warps: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 loads and products.  A chunk's product S is
-// issued before the chunk before it is finished, and B^T C does not wait for the state: what is serial from chunk to chunk is
-// the state's multiply-add, its packing and A X.
+// The CTAs of a cluster take the chunks of one sequence in turn.  Everything but X <- ... is theirs alone; X travels from
+// CTA to CTA through distributed shared memory (a bulk copy per warp onto the receiver's mbarrier), so what is serial from chunk
+// to chunk is one multiply-add of the state and its way to the next SM.  Where even clusters of eight leave SMs idle, the token axis is
+// cut into segments as well: k_decay_tc_sums adds up each, k_decay_prefix makes the states before them.
 //
-// Everything that the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are
-// cleared in shared memory before a product reads them, so that padding may hold NaN.
+// Warps of the walk: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 loads and products.  Everything that
+// the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are cleared in shared memory
+// before a product reads them, so that padding may hold NaN.
+//
+// The roles' loops are kept short on purpose: four roles share a scheduler, and unrolled to straight lines they waited for
+// instructions more than for data.
 #include "decay.h"
 #include "launch.h"
 #include "tc_common.cuh"
@@ -28,30 +33,45 @@ constexpr int kL = 128;                            // tokens of a chunk
 constexpr int kBlk = 128 * 128;                    // bytes of a [128 rows][64] tile
 
 struct DecayMaps {
-  CUtensorMap m[4];                                // boxes of [128 tokens][64 features]
+  CUtensorMap in[4], out[kDecayUnits];             // boxes of [128 tokens][64 features]
   int ia[kDecayUnits], ib[kDecayUnits], ic[kDecayUnits];
-};
-
-template <int DK, bool WALK> struct Plan {
-  static constexpr int kCB = DK / 64;              // column blocks of a and b
-  static constexpr int kStages = WALK && DK == 64 ? 3 : 2;
-  static constexpr int kXBuf = DK == 64 ? 2 : 1;   // buffers of the packed state
-  static constexpr int kXTile = DK * 128;          // one term of it: [DK][64]
-  static constexpr int oA = 0;
-  static constexpr int oB = oA + (WALK ? kStages * kCB * kBlk : 0);
-  static constexpr int oC = oB + kStages * kCB * kBlk;
-  static constexpr int oW = oC + kStages * kBlk;   // weighted C: two terms
-  static constexpr int oX = oW + 2 * kBlk;
-  static constexpr int oBars = oX + (WALK ? kXBuf * 2 * kXTile : 0);
-  static constexpr int kBytes = oBars + 512 + 1024;
-  static constexpr int kWarpC = WALK ? 8 : 0, kWarpX = kWarpC + 4, kWarpI = kWarpX + 4;
-  static constexpr int kThreads = 32 * (kWarpI + 1);
-  static constexpr int kTmem = WALK ? 512 : 64;
-  static constexpr int cY = 256, cYx = 320, cKv = WALK ? 384 : 0;      // S of even and odd chunks at 0 and 128
 };
 
 __device__ __forceinline__ void arrive_on(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+// bytes of this CTA's shared memory into another's, counted on a barrier over there
+__device__ __forceinline__ void copy_to_cta(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "r"(src), "r"(bytes), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void* src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];"
+               ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  return r;
 }
 // the hi and lo terms of a pair: lo is what rounding to 16 bits left of each
 template <typename T>
@@ -61,150 +81,129 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   lo = Op16<T>::pack(x - r.x, y - r.y);
 }
 
-template <typename T, int DK, bool WALK>
-__global__ void __launch_bounds__(Plan<DK, WALK>::kThreads, 1)
-k_decay_tc(const __grid_constant__ DecayMaps maps, const __grid_constant__ DecayArgs a, int* status) {
+// What a chunk is to the CTA that takes it.
+struct Span {
+  int n0, n1, nch;                                 // live tokens of the segment, its chunks
+  bool rev;
+  __device__ __forceinline__ Span(const DecayArgs& a, int live, int seg, bool reverse) : rev(reverse) {
+    n0 = seg * a.seg_len;
+    n1 = min(live, n0 + a.seg_len);
+    nch = n1 > n0 ? (n1 - n0 + kL - 1) / kL : 0;
+  }
+  __device__ __forceinline__ int first(int c) const { return n0 + kL * (rev ? nch - 1 - c : c); }   // of the c-th chunk walked
+  __device__ __forceinline__ int live(int c) const { return min(kL, n1 - first(c)); }
+};
+
+// C weighted by the decay to the chunk's end, in two terms; one thread a row.  Rows behind the length are cleared, here and in
+// the tiles of b and c themselves.
+template <typename T, int CB>
+__device__ __forceinline__ void weigh_c(int r, int cnt, float w, uint8_t* src, uint8_t* hi_t, uint8_t* b_t) {
+  if (r < cnt) {
+#pragma unroll 2
+    for (int ch = 0; ch < 8; ++ch) {
+      const uint32_t at = swz_off<128>(r, ch);
+      const uint4 x = *reinterpret_cast<const uint4*>(src + at);
+      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+      uint32_t hs[4], ls[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = mul2(Op16<T>::unpack(xs[i]), make_float2(w, w));
+        split2<T>(f.x, f.y, hs[i], ls[i]);
+      }
+      *reinterpret_cast<uint4*>(hi_t + at) = make_uint4(hs[0], hs[1], hs[2], hs[3]);
+      *reinterpret_cast<uint4*>(hi_t + kBlk + at) = make_uint4(ls[0], ls[1], ls[2], ls[3]);
+    }
+  } else {
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+    for (int ch = 0; ch < 8; ++ch) {
+      const uint32_t at = 128 * r + 16 * ch;
+      *reinterpret_cast<uint4*>(src + at) = z;
+      *reinterpret_cast<uint4*>(hi_t + at) = z;
+      *reinterpret_cast<uint4*>(hi_t + kBlk + at) = z;
+#pragma unroll
+      for (int i = 0; i < CB; ++i) *reinterpret_cast<uint4*>(b_t + i * kBlk + at) = z;
+    }
+  }
+  fence_proxy_async();
+}
+
+// B^T (hi | lo): 128 x 128, the lo terms in the upper columns.  For 64 features the 128 rows are the features twice (the second
+// block of the operand starts where the first does), so that each of the state's 128 threads has half a row to update.
+template <int DK, int F>
+__device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t w_tile) {
+  const uint32_t id = idesc_f16(128, 128, F, F, 1, 1);
+  const uint64_t dB = smem_desc_mn128(b_tile, DK == 128 ? kBlk : 0, 1024), dW = smem_desc_mn128(w_tile, kBlk, 1024);
+#pragma unroll
+  for (int kk = 0; kk < 8; ++kk) mma_ss(d, dB + 128 * kk, dW + 128 * kk, id, kk > 0);
+}
+
+// ---- the sums of the segments ----------------------------------------------------------------------------------------------
+// Warps 0-3 weighted C, 4-7 the sum (in registers), 8 loads and products.
+template <int DK> struct SumPlan {
+  static constexpr int kCB = DK / 64, kStages = 2;
+  static constexpr int oB = 0, oC = kStages * kCB * kBlk, oW = oC + kStages * kBlk, oBars = oW + 2 * kBlk, kBytes = oBars + 256 + 1024;
+  static constexpr int kThreads = 288;
+};
+
+template <typename T, int DK>
+__global__ void __launch_bounds__(SumPlan<DK>::kThreads, 1)
+k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ DecayArgs a, int* status) {
   grid_dep_sync();
-  using L = Plan<DK, WALK>;
+  using L = SumPlan<DK>;
   constexpr int F = Op16<T>::kFmt, NST = L::kStages, CB = L::kCB;
-  constexpr bool kHalfRange = F == 0;              // fp16: the packed state is scaled by a power of two
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
-  uint64_t *bFullAB = bars, *bFullC = bars + 3, *bS = bars + 6, *bP = bars + 8, *bX = bars + 10, *bYx = bars + 12, *bW = bars + 14,
-           *bKv = bars + 15, *bKvFree = bars + 16, *bY = bars + 17, *bYFree = bars + 18;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
-  int* abort_flag = reinterpret_cast<int*>(bars + 21);
-  float* sExp = reinterpret_cast<float*>(bars + 22);         // 2^e of the packed state, by chunk modulo 4
-  uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 24);   // [2][4]
-
+  uint64_t *bFull = bars, *bW = bars + 2, *bKv = bars + 3, *bKvFree = bars + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 5);
+  int* abort_flag = reinterpret_cast<int*>(bars + 6);
   const DecayUnit& u = a.u[blockIdx.z];
   const int n_cb = (u.Dc + 63) / 64;
-  const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = blockIdx.y;
+  const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = u.rev ? blockIdx.y + 1 : blockIdx.y;
   if (cb >= n_cb) return;
-  const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int live = decay_live(a, b);
-  const int n0 = seg * a.seg_len, n1 = min(live, n0 + a.seg_len);
-  const int nch = n1 > n0 ? (n1 - n0 + kL - 1) / kL : 0;
-  const bool rev = u.rev != 0;
-  const float ld = a.log_decay[h], g2 = decay_log2(ld);
-  auto first_of = [&](int c) { return n0 + kL * (rev ? nch - 1 - c : c); };      // first token of the c-th chunk in walking order
-  auto live_of = [&](int c) { return min(kL, n1 - first_of(c)); };
-  const CUtensorMap *mA = &maps.m[maps.ia[blockIdx.z]], *mB = &maps.m[maps.ib[blockIdx.z]], *mC = &maps.m[maps.ic[blockIdx.z]];
-
-  auto load_ab = [&](int c) {
-    const int st = c % NST, t0 = first_of(c);
-    mbar_expect_tx(bFullAB + st, (WALK ? 2 : 1) * CB * kBlk);
+  const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb, tid = threadIdx.x, warp = tid >> 5;
+  const float ld = a.log_decay[h];
+  const Span sp(a, decay_live(a, b), seg, u.rev != 0);
+  auto load = [&](int c) {
+    const int st = c % NST, t0 = sp.first(c);
+    mbar_expect_tx(bFull + st, (CB + 1) * kBlk);
 #pragma unroll
-    for (int i = 0; i < CB; ++i) {
-      if constexpr (WALK) tma_load_4d(smem + L::oA + (st * CB + i) * kBlk, mA, bFullAB + st, 64 * i, t0, h, b);
-      tma_load_4d(smem + L::oB + (st * CB + i) * kBlk, mB, bFullAB + st, 64 * i, t0, h, b);
-    }
-  };
-  auto load_c = [&](int c) {
-    const int st = c % NST;
-    mbar_expect_tx(bFullC + st, kBlk);
-    tma_load_4d(smem + L::oC + st * kBlk, mC, bFullC + st, c0, first_of(c), h, b);
+    for (int i = 0; i < CB; ++i) tma_load_4d(smem + L::oB + (st * CB + i) * kBlk, &maps.in[maps.ib[blockIdx.z]], bFull + st, 64 * i, t0, h, b);
+    tma_load_4d(smem + L::oC + st * kBlk, &maps.in[maps.ic[blockIdx.z]], bFull + st, c0, t0, h, b);
   };
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) { mbar_init(bFullAB + i, 1); mbar_init(bFullC + i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bYx + i, 1); }
-    mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128); mbar_init(bY, 1); mbar_init(bYFree, 256);
+    for (int i = 0; i < NST; ++i) mbar_init(bFull + i, 1);
+    mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128);
     *abort_flag = 0;
     fence_barrier_init();
-    for (int c = 0; c < NST && c < nch; ++c) { load_ab(c); load_c(c); }
+    for (int c = 0; c < NST && c < sp.nch; ++c) load(c);
   }
-  if (warp == 1) tmem_alloc<L::kTmem>(tmem_slot);
+  if (warp == 1) tmem_alloc<128>(tmem_slot);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // a wait that runs out marks the launch as failed and every later wait returns at once, so that the CTA ends
   auto gave_up = [&] { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
-  auto wait = [&](uint64_t* bar, int parity) { if (!gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag); };
-
-  if (warp == L::kWarpI) {
-    // ---- loads and products ------------------------------------------------------------------------------------------
-    const uint32_t id_s = idesc_f16(128, 128, F, F, 0, 0), id_y = idesc_f16(128, 64, F, F, 0, 1), id_kv = idesc_f16(128, 64, F, F, 1, 1);
-    const uint32_t base = smem_u32(smem);
-    auto product_s = [&](int c) {
-      wait(bFullAB + c % NST, c / NST);
-      if (live_of(c) < kL) wait(bW, c);            // rows behind the length are cleared first
-      tc_fence_after();
-      if (elect_one()) {
-        const int st = c % NST;
-#pragma unroll
-        for (int kk = 0; kk < DK / 16; ++kk) {
-          const uint32_t off = (st * CB + kk / 4) * kBlk;
-          mma_ss(tmem + 128 * (c & 1), smem_desc<128>(base + L::oA + off) + 2 * (kk & 3), smem_desc<128>(base + L::oB + off) + 2 * (kk & 3), id_s, kk > 0);
-        }
-        mma_commit(bS + (c & 1));
-      }
-      __syncwarp();
-    };
-    if (WALK && nch > 0) product_s(0);
+  auto wait = [&](uint64_t* bar, int parity) {
+    if (!mbar_try_wait(bar, parity & 1) && !gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag);
+  };
+  if (warp == 8) {
+    const int nch = __reduce_max_sync(0xffffffffu, sp.nch);
+    const uint32_t d = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
     for (int c = 0; c < nch && !gave_up(); ++c) {
       const int st = c % NST;
-      // B^T (weighted C).  For DK = 64 the 128 rows are the 64 features twice (the second block starts where the first does),
-      // so that every thread of the state's four warps has half a row to update.
-      wait(bFullAB + st, c / NST);
       wait(bW, c);
       if (c > 0) wait(bKvFree, c - 1);
       tc_fence_after();
       if (elect_one()) {
-        const uint64_t dB = smem_desc_mn128(base + L::oB + st * CB * kBlk, DK == 128 ? kBlk : 0, 1024);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const uint64_t dW = smem_desc<128>(base + L::oW + t * kBlk);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) mma_ss(tmem + L::cKv, dB + 128 * kk, dW + 128 * kk, id_kv, t + kk > 0);
-        }
+        product_kv<DK, F>(d, base + L::oB + st * CB * kBlk, base + L::oW);
         mma_commit(bKv);
       }
       __syncwarp();
-      if constexpr (WALK) {
-        // c of the chunk before is used up (its product ran ahead of the one just issued).  Before the next S, which may have
-        // to wait for that chunk's C.
-        if (c > 0 && c - 1 + NST < nch) {
-          wait(bY, c - 1);
-          if (elect_one()) load_c(c - 1 + NST);
-          __syncwarp();
-        }
-        if (c + 1 < nch) product_s(c + 1);
-        wait(bX + (c & 1), c >> 1);
-        if (c > 0) wait(bYFree, c - 1);
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t x = base + L::oX + (c % L::kXBuf) * 2 * L::kXTile;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const uint64_t dX = smem_desc<128>(x + t * L::kXTile);
-#pragma unroll
-            for (int kk = 0; kk < DK / 16; ++kk)
-              mma_ss(tmem + L::cYx, smem_desc<128>(base + L::oA + (st * CB + kk / 4) * kBlk) + 2 * (kk & 3), dX + 128 * kk, id_y, t + kk > 0);
-          }
-          mma_commit(bYx + (c & 1));
-        }
-        __syncwarp();
-        if (c + NST < nch) {                       // a and b of this chunk are used up
-          wait(bYx + (c & 1), c >> 1);
-          if (elect_one()) load_ab(c + NST);
-          __syncwarp();
-        }
-        wait(bP + (c & 1), c >> 1);
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t dC = smem_desc<128>(base + L::oC + st * kBlk);
-          const uint32_t p = tmem + 128 * (c & 1);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) mma_ts(tmem + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
-          mma_commit(bY);
-        }
-        __syncwarp();
-      } else if (c + NST < nch) {
+      if (c + NST < nch) {
         wait(bKv, c);
-        if (elect_one()) { load_ab(c + NST); load_c(c + NST); }
+        if (elect_one()) load(c + NST);
         __syncwarp();
       }
     }
@@ -212,231 +211,467 @@ k_decay_tc(const __grid_constant__ DecayMaps maps, const __grid_constant__ Decay
       const long long t0 = clock64();
       while (clock64() - t0 < (1LL << 22)) {}
     }
-  } else if (warp >= L::kWarpX) {
-    // ---- the state -----------------------------------------------------------------------------------------------------
+  } else if (warp >= 4) {
     constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
-    const int r = tid - 32 * L::kWarpX, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
-    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const long long st_off = (long long)bh * u.Da * u.Dc, seg_off = ((long long)bh * a.n_seg + seg) * u.Da * u.Dc;
-    const float* before = nullptr;
-    if constexpr (WALK) before = a.n_seg > 1 ? u.seg + seg_off : u.state_in ? u.state_in + st_off : nullptr;
+    const int r = tid - 128, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col;
     float X[NC];
 #pragma unroll
-    for (int j = 0; j < NC; j += 4) {
-      float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (before && d < u.Da && c0 + col + j < u.Dc) t = *reinterpret_cast<const float4*>(before + (long long)d * u.Dc + c0 + col + j);
-      X[j] = t.x; X[j + 1] = t.y; X[j + 2] = t.z; X[j + 3] = t.w;
-    }
+    for (int j = 0; j < NC; ++j) X[j] = 0.f;
     const DecayStep full(ld, kL);
-    for (int c = 0; c < nch && !gave_up(); ++c) {
-      if constexpr (WALK) {
-        float down = 1.f;
-        if constexpr (kHalfRange) {
-          // the largest magnitude of the tile to 2^13 ... 2^14: X may lie outside fp16's range
-          uint32_t top = 0;
-#pragma unroll
-          for (int j = 0; j < NC; ++j) top = max(top, __float_as_uint(X[j]) & 0x7fffffffu);
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (lane == 0) sMax[4 * (c & 1) + (warp & 3)] = top;
-          asm volatile("bar.sync 1, 128;" ::: "memory");
-          const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (c & 1));
-          top = max(max(all.x, all.y), max(all.z, all.w));
-          const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
-          down = __uint_as_float((uint32_t)(127 - e) << 23);
-          if (r == 0) sExp[c & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
-        }
-        if (c >= L::kXBuf) wait(bYx + ((c - L::kXBuf) & 1), (c - L::kXBuf) >> 1);
-        uint8_t* x = smem + L::oX + (c % L::kXBuf) * 2 * L::kXTile;
-#pragma unroll
-        for (int j = 0; j < NC; j += 8) {
-          uint32_t hi[4], lo[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) split2<T>(X[j + 2 * i] * down, X[j + 2 * i + 1] * down, hi[i], lo[i]);
-          const uint32_t at = swz_off<128>(d, (col + j) / 8);
-          *reinterpret_cast<uint4*>(x + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(x + L::kXTile + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        fence_proxy_async();
-        arrive_on(bX + (c & 1));
-      }
+    for (int c = 0; c < sp.nch && !gave_up(); ++c) {
+      const int cnt = sp.live(c);
+      const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
       wait(bKv, c);
       tc_fence_after();
-      const int cnt = live_of(c);
-      const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
 #pragma unroll
       for (int j = 0; j < NC; j += 16) {
-        uint32_t v[16];
-        tmem_ld16(lane_base + L::cKv + col + j, v);
+        uint32_t v[16], lo[16];
+        tmem_ld16(lane_base + j, v);
+        tmem_ld16(lane_base + 64 + j, lo);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) X[j + i] = decay(X[j + i]) + __uint_as_float(v[i]);
+        for (int i = 0; i < 16; ++i) X[j + i] = decay(X[j + i]) + (__uint_as_float(v[i]) + __uint_as_float(lo[i]));
       }
       tc_fence_before();
       arrive_on(bKvFree);
     }
-    float* end = nullptr;
-    if constexpr (WALK) end = u.state_out && seg == a.n_seg - 1 ? u.state_out + st_off : nullptr;
-    else end = u.seg + seg_off;
-    if (end && d < u.Da)
+    float* end = u.seg + ((long long)bh * a.n_seg + seg) * u.Da * u.Dc + (long long)d * u.Dc + c0 + col;
+    if (d < u.Da)
 #pragma unroll
       for (int j = 0; j < NC; j += 4)
-        if (c0 + col + j < u.Dc) *reinterpret_cast<float4*>(end + (long long)d * u.Dc + c0 + col + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
-  } else if (warp >= L::kWarpC) {
-    // ---- C weighted by the decay to the chunk's end, in two terms ----------------------------------------------------------
-    const int r = tid - 32 * L::kWarpC;
-    for (int c = 0; c < nch && !gave_up(); ++c) {
-      const int st = c % NST, cnt = live_of(c);
-      const float w = exp2f(g2 * (float)(rev ? r : max(0, cnt - 1 - r)));
-      wait(bFullC + st, c / NST);
-      if (cnt < kL) wait(bFullAB + st, c / NST);
+        if (c0 + col + j < u.Dc) *reinterpret_cast<float4*>(end + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
+  } else {
+    const float g2 = decay_log2(ld);
+    for (int c = 0; c < sp.nch && !gave_up(); ++c) {
+      const int st = c % NST, cnt = sp.live(c);
+      const float w = exp2f(g2 * (float)(sp.rev ? tid : max(0, cnt - 1 - tid)));
+      wait(bFull + st, c / NST);
       if (c > 0) wait(bKv, c - 1);                 // the products with the weighted C of the chunk before are done
-      uint8_t *src = smem + L::oC + st * kBlk, *hi_t = smem + L::oW, *lo_t = hi_t + kBlk;
-      if (r < cnt) {
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-          const uint32_t at = swz_off<128>(r, ch);
-          const uint4 x = *reinterpret_cast<const uint4*>(src + at);
-          uint4 hi, lo;
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-          uint32_t hs[4], ls[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = Op16<T>::unpack(xs[i]);
-            split2<T>(f.x * w, f.y * w, hs[i], ls[i]);
-          }
-          hi = make_uint4(hs[0], hs[1], hs[2], hs[3]);
-          lo = make_uint4(ls[0], ls[1], ls[2], ls[3]);
-          *reinterpret_cast<uint4*>(hi_t + at) = hi;
-          *reinterpret_cast<uint4*>(lo_t + at) = lo;
-        }
-      } else {                                     // behind the length: whatever stands there takes part in no product
-        const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int ch = 0; ch < 8; ++ch) {
-          const uint32_t at = 128 * r + 16 * ch;
-          *reinterpret_cast<uint4*>(src + at) = z;
-          *reinterpret_cast<uint4*>(hi_t + at) = z;
-          *reinterpret_cast<uint4*>(lo_t + at) = z;
-#pragma unroll
-          for (int i = 0; i < CB; ++i) *reinterpret_cast<uint4*>(smem + L::oB + (st * CB + i) * kBlk + at) = z;
-        }
-      }
-      fence_proxy_async();
+      weigh_c<T, CB>(tid, cnt, w, smem + L::oC + st * kBlk, smem + L::oW, smem + L::oB + st * CB * kBlk);
       arrive_on(bW);
-    }
-  } else if constexpr (WALK) {
-    // ---- weights of P, outputs -----------------------------------------------------------------------------------------
-    const int r0 = 32 * (warp & 3), r = r0 + lane, hb = warp >> 2;    // token r, half of the columns
-    const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
-    // The weights depend on i - j alone, so a thread keeps those of its row for all chunks.
-    float w[64];
-#pragma unroll
-    for (int j = 0; j < 64; ++j) {
-      const int dist = rev ? 64 * hb + j - r : r - 64 * hb - j;
-      w[j] = dist >= 0 ? exp2f(g2 * (float)dist) : 0.f;
-    }
-    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
-    T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0 + 32 * hb;
-    const int cols = u.Dc - c0 - 32 * hb;          // of this thread's 32 columns, those that exist
-
-    auto weigh = [&](int c) {
-      wait(bS + (c & 1), c >> 1);
-      tc_fence_after();
-      const int cnt = live_of(c);
-      const uint32_t s = lane_base + 128 * (c & 1) + 64 * hb;
-      uint32_t v[2][16];
-      tmem_ld16(s, v[0]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j0 = 64 * hb + 16 * i;           // the block's first column; the warp's rows are r0 ... r0 + 31
-        const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = (rev ? j0 >= r0 + 31 : j0 + 15 <= r0) && cnt == kL;
-        tmem_wait_ld();
-        if (i + 1 < 4) tmem_ld16(s + 16 * (i + 1), v[(i + 1) & 1]);
-        uint32_t p[8];
-        if (none) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) p[k] = 0u;
-        } else if (all) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k)
-            p[k] = Op16<T>::pack(__uint_as_float(v[i & 1][2 * k]) * w[16 * i + 2 * k], __uint_as_float(v[i & 1][2 * k + 1]) * w[16 * i + 2 * k + 1]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float w0 = w[16 * i + 2 * k], w1 = w[16 * i + 2 * k + 1];
-            const float x0 = w0 != 0.f && j0 + 2 * k < cnt ? __uint_as_float(v[i & 1][2 * k]) * w0 : 0.f;
-            const float x1 = w1 != 0.f && j0 + 2 * k + 1 < cnt ? __uint_as_float(v[i & 1][2 * k + 1]) * w1 : 0.f;
-            p[k] = Op16<T>::pack(x0, x1);
-          }
-        }
-        tmem_st8(s + 8 * i, p);                    // over columns of this thread that are read already
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      arrive_on(bP + (c & 1));
-    };
-    auto store_row = [&](int tok, const uint4 (&o)[4]) {
-      T* p = out + (long long)tok * u.os[2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (8 * i < cols) *reinterpret_cast<uint4*>(p + 8 * i) = o[i];
-    };
-
-    if (nch > 0) weigh(0);
-    for (int c = 0; c < nch && !gave_up(); ++c) {
-      if (c + 1 < nch) weigh(c + 1);
-      wait(bY, c);
-      tc_fence_after();
-      float fx = wx;
-      if constexpr (kHalfRange) fx *= sExp[c & 3];
-      uint4 o[4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        uint32_t y[16], x[16];
-        tmem_ld16(lane_base + L::cY + 32 * hb + 16 * i, y);
-        tmem_ld16(lane_base + L::cYx + 32 * hb + 16 * i, x);
-        tmem_wait_ld();
-        uint32_t q[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          q[k] = Op16<T>::pack(fmaf(fx, __uint_as_float(x[2 * k]), a.scale * __uint_as_float(y[2 * k])),
-                               fmaf(fx, __uint_as_float(x[2 * k + 1]), a.scale * __uint_as_float(y[2 * k + 1])));
-        o[2 * i] = make_uint4(q[0], q[1], q[2], q[3]);
-        o[2 * i + 1] = make_uint4(q[4], q[5], q[6], q[7]);
-      }
-      tc_fence_before();
-      arrive_on(bYFree);
-      const int tok = first_of(c) + r;
-      if (tok < n1) store_row(tok, o);
-    }
-    const uint4 z[4] = {};
-    for (int tok = max(n0, live) + (tid & 127); tok < min(a.N, n0 + a.seg_len); tok += 128) {
-      T* p = out + (long long)tok * u.os[2];       // rows behind the sequence: zeros
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (8 * i < cols) *reinterpret_cast<uint4*>(p + 8 * i) = z[i];
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc<L::kTmem>(tmem);
+  if (warp == 1) tmem_dealloc<128>(tmem);
+}
+
+// ---- the walk --------------------------------------------------------------------------------------------------------------
+template <int DK> struct WalkPlan {
+  static constexpr int kCB = DK / 64;
+  // Tiles in flight.  Shared memory holds three chunks of 64 features; of 128 features two tiles of a and of c, and one of b,
+  // which is free as soon as S and B^T C have been formed.
+  static constexpr int kA = DK == 64 ? 3 : 2, kB = DK == 64 ? 3 : 1, kC = DK == 64 ? 3 : 2;
+  static constexpr bool kStage = DK == 64;         // outputs leave through shared memory and the TMA
+  static constexpr int kXTile = DK * 128;          // one term of the packed state: [DK][64]
+  static constexpr int kXBytes = DK * 64 * 4;      // the state in fp32 as it arrives
+  static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + 2 * kBlk,
+                       oIn = oX + 2 * kXTile, oOut = oIn + kXBytes, oBars = oOut + (kStage ? kBlk : 0);
+  static constexpr int kBytes = oBars + 512 + 1024;
+  static constexpr int kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 1);
+  static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
+};
+
+template <typename T, int DK>
+__global__ void __launch_bounds__(WalkPlan<DK>::kThreads, 1)
+k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ DecayArgs a, int* status) {
+  grid_dep_sync();
+  using L = WalkPlan<DK>;
+  constexpr int F = Op16<T>::kFmt, CB = L::kCB;
+  constexpr bool kHalfRange = F == 0;              // fp16: the packed state is scaled by a power of two
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
+  uint64_t *bFullA = bars, *bFullB = bars + 3, *bFullC = bars + 6, *bS = bars + 9, *bP = bars + 11, *bX = bars + 13, *bYx = bars + 15, *bW = bars + 16,
+           *bKv = bars + 17, *bKvFree = bars + 18, *bY = bars + 19, *bYFree = bars + 20, *bIn = bars + 21;    // bIn: one a warp of the state
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
+  int* abort_flag = reinterpret_cast<int*>(bars + 26);
+  float* sExp = reinterpret_cast<float*>(bars + 28);         // 2^e of the packed state, by chunk modulo 4
+  uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 30);   // [2][4]
+
+  const DecayUnit& u = a.u[blockIdx.z];
+  const int n_cb = (u.Dc + 63) / 64, size = cluster_size(), rank = cluster_rank();
+  const int sequence = blockIdx.x / size, bh = sequence % (a.B * a.H), cb = sequence / (a.B * a.H), seg = blockIdx.y;
+  if (cb >= n_cb) return;                          // the whole cluster alike
+  const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int live = decay_live(a, b);
+  const bool rev = u.rev != 0;
+  const Span sp(a, live, seg, rev);
+  const int mine = (sp.nch - rank + size - 1) / size;        // chunks rank, rank + size, ... are this CTA's: 0, 1, ... below
+  const float ld = a.log_decay[h], g2 = decay_log2(ld);
+  auto chunk = [&](int i) { return rank + size * i; };
+
+  auto load = [&](uint8_t* tiles, uint64_t* full, const CUtensorMap* map, int st, int blocks, int col, int i) {
+    mbar_expect_tx(full + st, blocks * kBlk);
+    for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + (st * blocks + k) * kBlk, map, full + st, col + 64 * k, sp.first(chunk(i)), h, b);
+  };
+  auto load_a = [&](int i) { load(smem + L::oA, bFullA, &maps.in[maps.ia[blockIdx.z]], i % L::kA, CB, 0, i); };
+  auto load_b = [&](int i) { load(smem + L::oB, bFullB, &maps.in[maps.ib[blockIdx.z]], i % L::kB, CB, 0, i); };
+  auto load_c = [&](int i) { load(smem + L::oC, bFullC, &maps.in[maps.ic[blockIdx.z]], i % L::kC, 1, c0, i); };
+  if (tid == 0) {
+    for (int i = 0; i < 3; ++i) { mbar_init(bFullA + i, 1); mbar_init(bFullB + i, 1); mbar_init(bFullC + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); }
+    mbar_init(bYx, 1); mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128); mbar_init(bY, 1); mbar_init(bYFree, 256);
+    for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    for (int i = 0; i < mine; ++i) {
+      if (i < L::kB) load_b(i);
+      if (i < L::kA) load_a(i);
+      if (i < L::kC) load_c(i);
+      if (i >= 2) break;
+    }
+    if (size > 1 && mine > (rank == 0 ? 1 : 0))                           // the first state that comes from another CTA
+      for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, L::kXBytes / 4);
+  }
+  if (warp == 1) tmem_alloc<512>(tmem_slot);
+  tc_fence_before();
+  cluster_sync();                                  // every CTA's barriers stand before a state is sent
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // A wait that runs out marks the launch as failed and every later wait returns at once, so that the CTA ends.  Warps that
+  // meet at a named barrier go through all their chunks all the same.
+  auto gave_up = [&] { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
+  auto wait = [&](uint64_t* bar, int parity) {
+    if (!mbar_try_wait(bar, parity & 1) && !gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag);
+  };
+
+  if (warp == L::kWarpI) {
+    // ---- loads and products ------------------------------------------------------------------------------------------
+    // counts and addresses through a warp reduction: the compiler then keeps them, and the descriptors, in uniform registers
+    const int n = __reduce_max_sync(0xffffffffu, mine);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
+    constexpr uint32_t id_s = idesc_f16(128, 128, F, F, 0, 0), id_y = idesc_f16(128, 64, F, F, 0, 1);
+    auto product_s = [&](int i) {
+      wait(bFullA + i % L::kA, i / L::kA);
+      wait(bFullB + i % L::kB, i / L::kB);
+      if (sp.live(chunk(i)) < kL) wait(bW, i);     // rows behind the length are cleared first
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dA = smem_desc<128>(base + L::oA + (i % L::kA) * CB * kBlk), dB = smem_desc<128>(base + L::oB + (i % L::kB) * CB * kBlk);
+        const uint32_t d = tm + 128 * (i & 1);
+#pragma unroll
+        for (int kk = 0; kk < DK / 16; ++kk) {
+          const uint32_t off = (kk / 4) * (kBlk >> 4) + 2 * (kk & 3);
+          mma_ss(d, dA + off, dB + off, id_s, kk > 0);
+        }
+        mma_commit(bS + (i & 1));
+      }
+      __syncwarp();
+    };
+    if (n > 0) product_s(0);
+    for (int i = 0; i < n && !gave_up(); ++i) {
+      wait(bFullB + i % L::kB, i / L::kB);
+      wait(bW, i);
+      if (i > 0) wait(bKvFree, i - 1);
+      tc_fence_after();
+      if (elect_one()) {
+        product_kv<DK, F>(tm + L::cKv, base + L::oB + (i % L::kB) * CB * kBlk, base + L::oW);
+        mma_commit(bKv);
+      }
+      __syncwarp();
+      // c of the chunk before is used up (its product ran ahead of the one just issued).  Before the next S, which may have
+      // to wait for that chunk's C.
+      if (i > 0 && i - 1 + L::kC < n) {
+        wait(bY, i - 1);
+        if (elect_one()) load_c(i - 1 + L::kC);
+        __syncwarp();
+      }
+      if (L::kB > 1 && i + 1 < n) product_s(i + 1);
+      wait(bX + (i & 1), i >> 1);
+      if (i > 0) wait(bYFree, i - 1);
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dA = smem_desc<128>(base + L::oA + (i % L::kA) * CB * kBlk), dX = smem_desc<128>(base + L::oX);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int kk = 0; kk < DK / 16; ++kk)
+            mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
+        mma_commit(bYx);
+      }
+      __syncwarp();
+      if (i + L::kB < n) {                         // b of this chunk is used up
+        wait(bKv, i);
+        if (elect_one()) load_b(i + L::kB);
+        __syncwarp();
+      }
+      wait(bP + (i & 1), i >> 1);
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t dC = smem_desc<128>(base + L::oC + (i % L::kC) * kBlk);
+        const uint32_t p = tm + 128 * (i & 1);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
+        mma_commit(bY);
+      }
+      __syncwarp();
+      if (i + L::kA < n) {                         // so is a
+        wait(bYx, i);
+        if (elect_one()) load_a(i + L::kA);
+        __syncwarp();
+      }
+      if (L::kB == 1 && i + 1 < n) product_s(i + 1);
+    }
+    if (gave_up()) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
+      const long long t0 = clock64();
+      while (clock64() - t0 < (1LL << 22)) {}
+    }
+  } else if (warp >= L::kWarpX) {
+    // ---- the state -----------------------------------------------------------------------------------------------------
+    // It lives in sIn: a thread's quads of columns q = 0, 1, ... stand at 512 q + 16 lane of its warp's quarter.  They are read,
+    // packed for this chunk's product, and replaced by the state behind the chunk, which is then copied to the CTA that takes
+    // the next one.  That CTA's copy further on cannot arrive here before this one has been read: each waits for the one before.
+    constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
+    const int r = tid - 32 * L::kWarpX, w = warp & 3, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
+    const uint32_t kv = tmem + ((uint32_t)(w * 32) << 16) + L::cKv + col;
+    uint8_t* in = smem + L::oIn + w * (L::kXBytes / 4) + 16 * lane;
+    const long long own = (long long)d * u.Dc + c0 + col;
+    const int cols = d < u.Da ? u.Dc - c0 - col : 0;         // of this thread's columns, those that exist
+    if (rank == 0) {
+      const float* before = a.n_seg > 1 ? u.seg + ((long long)bh * a.n_seg + seg) * u.Da * u.Dc : u.state_in ? u.state_in + (long long)bh * u.Da * u.Dc : nullptr;
+#pragma unroll 2
+      for (int j = 0; j < NC; j += 4)
+        *reinterpret_cast<float4*>(in + 128 * j) = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const DecayStep full(ld, kL);
+    for (int i = 0; i < mine; ++i) {
+      const int c = chunk(i), cnt = sp.live(c);
+      const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
+      wait(bKv, i);
+      if (i > 0) wait(bYx, i - 1);                 // the product with the packed state of the chunk before is done
+      if (size > 1 && c > 0) {
+        wait(bIn + w, rank == 0 ? i - 1 : i);
+        if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
+      }
+      tc_fence_after();
+      float down = 1.f;
+      if constexpr (kHalfRange) {
+        // the largest magnitude of the tile to 2^13 ... 2^14: X may lie outside fp16's range
+        uint32_t top = 0;
+#pragma unroll 2
+        for (int j = 0; j < NC; j += 4) {
+          const uint4 t = *reinterpret_cast<const uint4*>(in + 128 * j);
+          top = max(max(max(top, t.x & 0x7fffffffu), t.y & 0x7fffffffu), max(t.z & 0x7fffffffu, t.w & 0x7fffffffu));
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) sMax[4 * (i & 1) + w] = top;
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
+        top = max(max(all.x, all.y), max(all.z, all.w));
+        const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
+        down = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
+      }
+#pragma unroll 2
+      for (int j = 0; j < NC; j += 8) {
+        uint32_t v[8], lo[8];
+        tmem_ld8(kv + j, v);
+        tmem_ld8(kv + 64 + j, lo);
+        float4 x[2] = {*reinterpret_cast<const float4*>(in + 128 * j), *reinterpret_cast<const float4*>(in + 128 * j + 512)};
+        const float* X = reinterpret_cast<const float*>(x);
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) split2<T>(X[2 * k] * down, X[2 * k + 1] * down, h[k], l[k]);
+        const uint32_t at = L::oX + swz_off<128>(d, (col + j) / 8);
+        *reinterpret_cast<uint4*>(smem + at) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(smem + L::kXTile + at) = make_uint4(l[0], l[1], l[2], l[3]);
+        tmem_wait_ld();
+        float y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = decay(X[k]) + (__uint_as_float(v[k]) + __uint_as_float(lo[k]));
+        *reinterpret_cast<float4*>(in + 128 * j) = make_float4(y[0], y[1], y[2], y[3]);
+        *reinterpret_cast<float4*>(in + 128 * j + 512) = make_float4(y[4], y[5], y[6], y[7]);
+      }
+      fence_proxy_async();
+      if (size > 1 && c + 1 < sp.nch) {
+        __syncwarp();
+        if (lane == 0) {
+          const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
+          copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
+        }
+      }
+      tc_fence_before();
+      arrive_on(bKvFree);
+      arrive_on(bX + (i & 1));
+    }
+    // behind the last chunk (or, without one, behind none: rank 0 then)
+    const int last = sp.nch > 0 ? (sp.nch - 1) % size : 0;
+    if (u.state_out && seg == a.n_seg - 1 && rank == last)
+#pragma unroll 2
+      for (int j = 0; j < NC; j += 4)
+        if (j < cols) *reinterpret_cast<float4*>(u.state_out + (long long)bh * u.Da * u.Dc + own + j) = *reinterpret_cast<const float4*>(in + 128 * j);
+  } else if (warp >= L::kWarpC) {
+    // ---- weighted C ----------------------------------------------------------------------------------------------------
+    const int r = tid - 32 * L::kWarpC;
+    for (int i = 0; i < mine && !gave_up(); ++i) {
+      const int cnt = sp.live(chunk(i));
+      const float w = exp2f(g2 * (float)(rev ? r : max(0, cnt - 1 - r)));
+      wait(bFullC + i % L::kC, i / L::kC);
+      if (cnt < kL) wait(bFullB + i % L::kB, i / L::kB);
+      if (i > 0) wait(bKv, i - 1);                 // the products with the weighted C of the chunk before are done
+      weigh_c<T, CB>(r, cnt, w, smem + L::oC + (i % L::kC) * kBlk, smem + L::oW, smem + L::oB + (i % L::kB) * CB * kBlk);
+      arrive_on(bW);
+    }
+  } else {
+    // ---- weights of P, outputs -----------------------------------------------------------------------------------------
+    const int r0 = 32 * (warp & 3), r = r0 + lane, hb = warp >> 2;    // token r, half of the columns
+    const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
+    // A weight lambda^(i-j) of a block of 16 columns below the diagonal is a factor of the column times one of the (row, block);
+    // the two blocks that the diagonal crosses in a warp's rows take an exponential each.
+    float2 wcol[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      wcol[k] = make_float2(exp2f(g2 * (float)(rev ? 2 * k : 15 - 2 * k)), exp2f(g2 * (float)(rev ? 2 * k + 1 : 14 - 2 * k)));
+    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
+    T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0 + 32 * hb;
+    const int cols = u.Dc - c0 - 32 * hb;          // of this thread's 32 columns, those that exist
+
+    auto weigh = [&](int i) {
+      const int cnt = sp.live(chunk(i));
+      const uint32_t s = lane_base + 128 * (i & 1) + 64 * hb;
+      wait(bS + (i & 1), i >> 1);
+      tc_fence_after();
+#pragma unroll 1
+      for (int k = 0; k < 4; ++k) {
+        const int j0 = 64 * hb + 16 * k;           // the block's first column; the warp's rows are r0 ... r0 + 31
+        const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = (rev ? j0 >= r0 + 31 : j0 + 15 <= r0) && cnt == kL;
+        uint32_t p[8];
+        if (none) {
+#pragma unroll
+          for (int m = 0; m < 8; ++m) p[m] = 0u;
+        } else {
+          uint32_t v[16];
+          tmem_ld16(s + 16 * k, v);
+          const float row = exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15));
+          tmem_wait_ld();
+          if (all) {
+            const float2 f = make_float2(row, row);
+#pragma unroll
+            for (int m = 0; m < 8; ++m) {
+              const float2 x = mul2(mul2(make_float2(__uint_as_float(v[2 * m]), __uint_as_float(v[2 * m + 1])), wcol[m]), f);
+              p[m] = Op16<T>::pack(x.x, x.y);
+            }
+          } else {
+            const int d = rev ? j0 - r : r - j0, sign = rev ? 1 : -1;
+#pragma unroll
+            for (int m = 0; m < 16; m += 2) {
+              const int d0 = d + sign * m, d1 = d0 + sign;
+              const float x0 = d0 >= 0 && j0 + m < cnt ? __uint_as_float(v[m]) * exp2f(g2 * (float)d0) : 0.f;
+              const float x1 = d1 >= 0 && j0 + m + 1 < cnt ? __uint_as_float(v[m + 1]) * exp2f(g2 * (float)d1) : 0.f;
+              p[m / 2] = Op16<T>::pack(x0, x1);
+            }
+          }
+        }
+        tmem_st8(s + 8 * k, p);                    // over columns of this thread that are read already
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      arrive_on(bP + (i & 1));
+    };
+    auto finish = [&](int i) {
+      const int c = chunk(i), cnt = sp.live(c), tok0 = sp.first(c);
+      if constexpr (L::kStage) {                   // the tile of the chunk before has left shared memory
+        if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+      }
+      wait(bY, i);
+      tc_fence_after();
+      float fx = wx;
+      if constexpr (kHalfRange) fx *= sExp[i & 3];
+#pragma unroll 2
+      for (int k = 0; k < 4; ++k) {
+        uint32_t y[8], x[8];
+        tmem_ld8(lane_base + L::cY + 32 * hb + 8 * k, y);
+        tmem_ld8(lane_base + L::cYx + 32 * hb + 8 * k, x);
+        tmem_wait_ld();
+        uint32_t q[4];
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const uint32_t t = Op16<T>::pack(fmaf(fx, __uint_as_float(x[2 * m]), a.scale * __uint_as_float(y[2 * m])),
+                                           fmaf(fx, __uint_as_float(x[2 * m + 1]), a.scale * __uint_as_float(y[2 * m + 1])));
+          q[m] = r < cnt ? t : 0u;                 // rows behind the sequence: zeros
+        }
+        const uint4 o = make_uint4(q[0], q[1], q[2], q[3]);
+        if constexpr (L::kStage) *reinterpret_cast<uint4*>(smem + L::oOut + swz_off<128>(r, 4 * hb + k)) = o;
+        else if (tok0 + r < a.N && 8 * k < cols) *reinterpret_cast<uint4*>(out + (long long)(tok0 + r) * u.os[2] + 8 * k) = o;
+      }
+      tc_fence_before();
+      arrive_on(bYFree);
+      if constexpr (L::kStage) {
+        fence_proxy_async();
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        if (tid == 0) tma_store_4d(&maps.out[blockIdx.z], smem + L::oOut, c0, tok0, h, b);      // clipped at N and at the last column
+      }
+    };
+    // With two chunks of a and b in flight the next weights come before this chunk's outputs, else behind them.
+    constexpr int kAhead = L::kB > 1 ? 1 : 0;
+    for (int i = 0; i < mine + kAhead; ++i) {
+      if (i < mine) weigh(i);
+      if (i >= kAhead) finish(i - kAhead);
+    }
+    // chunks of the segment that no live token is in: zeros
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    for (int tok = sp.n0 + kL * (sp.nch + rank) + (tid & 127); tok < min(a.N, sp.n0 + a.seg_len);
+         tok = sp.n0 + (tok - sp.n0) / kL * kL + kL * size + (tid & 127)) {
+      T* p = out + (long long)tok * u.os[2];
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (8 * k < cols) *reinterpret_cast<uint4*>(p + 8 * k) = z;
+    }
+    if constexpr (L::kStage)
+      if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  tc_fence_before();
+  cluster_sync();                                  // no CTA leaves while another may still write into it
+  if (warp == 1) tmem_dealloc<512>(tmem);
+}
+
+int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, const DecayMaps& maps, const DecayArgs& a, int* status) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  void* args[] = {const_cast<DecayMaps*>(&maps), const_cast<DecayArgs*>(&a), &status};
+  return cudaLaunchKernelExC(&cfg, kernel, args) == cudaSuccess ? FLARE_OK : FLARE_ECUDA;
+}
+
+// How a call is spread: CTAs of a sequence (a cluster) and segments of the token axis.
+struct Spread { int cluster, segments; };
+Spread pick_spread(int B, int H, int N, int Dc, int n_units) {
+  const long long seqs = (long long)B * H * ((Dc + 63) / 64) * n_units;
+  const int chunks = (int)(((long long)N + kL - 1) / kL), sms = num_sms();
+  Spread s = {1, 1};
+  while (s.cluster < 8 && seqs * s.cluster * 2 <= sms + sms / 8 && s.cluster * 2 <= chunks) s.cluster *= 2;
+  if (s.cluster == 8) {
+    long long n = sms / (seqs * 8);
+    if (n > chunks / 16) n = chunks / 16;
+    s.segments = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  }
+  return s;
 }
 
 template <typename T, int DK>
-int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, cudaStream_t st) {
-  using W = Plan<DK, true>;
-  using S = Plan<DK, false>;
+int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, int cluster, cudaStream_t st) {
+  using W = WalkPlan<DK>;
+  using S = SumPlan<DK>;
   int* status = tc_status_ptr();
-  if (tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_tc<T, DK, true>), W::kBytes) != FLARE_OK ||
-      tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_tc<T, DK, false>), S::kBytes) != FLARE_OK)
+  const void* walk = reinterpret_cast<const void*>(&k_decay_tc_walk<T, DK>);
+  if (tc_set_dyn_smem(walk, W::kBytes) != FLARE_OK ||
+      tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_tc_sums<T, DK>), S::kBytes) != FLARE_OK)
     return FLARE_ECUDA;
-  const dim3 grid((unsigned)(a.B * a.H * ((Dc + 63) / 64)), (unsigned)a.n_seg, (unsigned)a.n_units);
-  if (a.n_seg > 1) {
-    launch_dep(k_decay_tc<T, DK, false>, grid, dim3(S::kThreads), S::kBytes, st, maps, a, status);
+  const unsigned seqs = (unsigned)(a.B * a.H * ((Dc + 63) / 64));
+  if (a.n_seg > 1) {                               // the last segment walked needs no sum
+    launch_dep(k_decay_tc_sums<T, DK>, dim3(seqs, (unsigned)a.n_seg - 1, (unsigned)a.n_units), dim3(S::kThreads), S::kBytes, st, maps, a, status);
     launch_decay_prefix(a, st);
   }
-  launch_dep(k_decay_tc<T, DK, true>, grid, dim3(W::kThreads), W::kBytes, st, maps, a, status);
-  return FLARE_OK;
+  return launch_walk(walk, dim3(seqs * cluster, (unsigned)a.n_seg, (unsigned)a.n_units), W::kThreads, W::kBytes, cluster, st, maps, a, status);
 }
 
 }  // namespace
@@ -458,45 +693,46 @@ bool decay_tc_supported(const DecayArgs& a, int dtype) {
   return true;
 }
 
-// Segments of the token axis: with as many as there are SMs to fill, but a segment of four chunks at least, since every CTA
-// has a start-up and the sums of the segments are a pass of their own over b and c.
 int decay_tc_segments(int B, int H, int N, int Da, int Dc, int n_units) {
   (void)Da;
-  const long long ctas = (long long)B * H * ((Dc + 63) / 64) * n_units;
-  long long s = num_sms() / ctas;
-  const long long most = ((long long)N + 4 * kL - 1) / (4 * kL);
-  if (s > most) s = most;
-  if (s > 256) s = 256;
-  return s < 1 ? 1 : (int)s;
+  return pick_spread(B, H, N, Dc, n_units).segments;
 }
 
 int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
   DecayMaps maps;
   const void* seen[4] = {};
   int n = 0, Da = 0, Dc = 0;
-  auto map_of = [&](const void* p, const long long (&s)[3], int D) {
-    for (int i = 0; i < n; ++i)
-      if (seen[i] == p) return i;
-    if (n == 4) return -1;
+  auto make = [&](CUtensorMap* m, const void* p, const long long (&s)[3], int D) {
     // a dimension of one entry has no stride of its own: any valid one
     const uint64_t row = a.N > 1 ? s[2] : D, head = a.H > 1 ? s[1] : row * (uint64_t)a.N, batch = a.B > 1 ? s[0] : head * (uint64_t)a.H;
-    if (!make_tile_map_cols(&maps.m[n], p, dtype == FLARE_BF16 ? 1 : 0, D, 64, (uint64_t)a.N, (uint64_t)a.H, (uint64_t)a.B, 2 * row, 2 * head,
-                            2 * batch, 128))
-      return -1;
+    return make_tile_map_cols(m, p, dtype == FLARE_BF16 ? 1 : 0, D, 64, (uint64_t)a.N, (uint64_t)a.H, (uint64_t)a.B, 2 * row, 2 * head, 2 * batch, 128);
+  };
+  auto map_of = [&](const void* p, const long long (&s)[3], int D, int like) {
+    // one tensor is an operand of several units; the same address with another shape is another tensor
+    for (int i = 0; i < n; ++i)
+      if (i == like && seen[i] == p) return i;
+    if (n == 4 || !make(&maps.in[n], p, s, D)) return -1;
     seen[n] = p;
     return n++;
   };
   for (int i = 0; i < a.n_units; ++i) {
     const DecayUnit& u = a.u[i];
-    maps.ia[i] = map_of(u.a, u.as, u.Da);
-    maps.ib[i] = map_of(u.b, u.bs, u.Da);
-    maps.ic[i] = map_of(u.c, u.cs, u.Dc);
-    if (maps.ia[i] < 0 || maps.ib[i] < 0 || maps.ic[i] < 0) return FLARE_EUNSUPPORTED;
     Da = u.Da > Da ? u.Da : Da;
     Dc = u.Dc > Dc ? u.Dc : Dc;
+    if (!make(&maps.out[i], u.out, u.os, u.Dc)) return FLARE_EUNSUPPORTED;
   }
-  if (dtype == FLARE_BF16) return Da <= 64 ? launch_all<__nv_bfloat16, 64>(maps, a, Dc, st) : launch_all<__nv_bfloat16, 128>(maps, a, Dc, st);
-  return Da <= 64 ? launch_all<__half, 64>(maps, a, Dc, st) : launch_all<__half, 128>(maps, a, Dc, st);
+  // the operands in the order dy v k | (v dy) q | (k q dy): each tensor's map is made once
+  const int order[3][3] = {{0, 1, 2}, {1, 0, 3}, {2, 3, 0}};
+  for (int i = 0; i < a.n_units; ++i) {
+    const DecayUnit& u = a.u[i];
+    maps.ia[i] = map_of(u.a, u.as, u.Da, order[i][0]);
+    maps.ib[i] = map_of(u.b, u.bs, u.Da, order[i][1]);
+    maps.ic[i] = map_of(u.c, u.cs, u.Dc, order[i][2]);
+    if (maps.ia[i] < 0 || maps.ib[i] < 0 || maps.ic[i] < 0) return FLARE_EUNSUPPORTED;
+  }
+  const int cluster = pick_spread(a.B, a.H, a.N, Dc, a.n_units).cluster;
+  if (dtype == FLARE_BF16) return Da <= 64 ? launch_all<__nv_bfloat16, 64>(maps, a, Dc, cluster, st) : launch_all<__nv_bfloat16, 128>(maps, a, Dc, cluster, st);
+  return Da <= 64 ? launch_all<__half, 64>(maps, a, Dc, cluster, st) : launch_all<__half, 128>(maps, a, Dc, cluster, st);
 }
 
 }  // namespace flare
