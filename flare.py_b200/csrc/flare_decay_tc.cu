@@ -12,7 +12,7 @@
 // to chunk is one multiply-add of the state and its way to the next SM.  Where even clusters of eight leave SMs idle, the token axis is
 // cut into segments as well: k_decay_tc_sums adds up each, k_decay_prefix makes the states before them.
 //
-// Warps of the walk: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 loads and products.  Everything that
+// Warps of the walk: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 products, 17 loads.  Everything that
 // the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are cleared in shared memory
 // before a product reads them, so that padding may hold NaN.
 //
@@ -269,7 +269,7 @@ template <int DK> struct WalkPlan {
   static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + 2 * kBlk,
                        oIn = oX + 2 * kXTile, oOut = oIn + kXBytes, oBars = oOut + (kStage ? kBlk : 0);
   static constexpr int kBytes = oBars + 512 + 1024;
-  static constexpr int kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 1);
+  static constexpr int kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 2);
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
 };
 
@@ -283,12 +283,13 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
-  uint64_t *bFullA = bars, *bFullB = bars + 3, *bFullC = bars + 6, *bS = bars + 9, *bP = bars + 11, *bX = bars + 13, *bYx = bars + 15, *bW = bars + 16,
+  uint64_t *bFull = bars, *bFullC = bars + 3, *bS = bars + 9, *bP = bars + 11, *bX = bars + 13, *bYx = bars + 15, *bW = bars + 16,
            *bKv = bars + 17, *bKvFree = bars + 18, *bY = bars + 19, *bYFree = bars + 20, *bIn = bars + 21;    // bIn: one a warp of the state
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
   int* abort_flag = reinterpret_cast<int*>(bars + 26);
   float* sExp = reinterpret_cast<float*>(bars + 28);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 30);   // [2][4]
+  uint64_t *bFreeA = bars + 34, *bFreeB = bars + 37, *bFreeC = bars + 40;     // by tile
 
   const DecayUnit& u = a.u[blockIdx.z];
   const int n_cb = (u.Dc + 63) / 64, size = cluster_size(), rank = cluster_rank();
@@ -303,15 +304,21 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const float ld = a.log_decay[h], g2 = decay_log2(ld);
   auto chunk = [&](int i) { return rank + size * i; };
 
-  auto load = [&](uint8_t* tiles, uint64_t* full, const CUtensorMap* map, int st, int blocks, int col, int i) {
-    mbar_expect_tx(full + st, blocks * kBlk);
-    for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + (st * blocks + k) * kBlk, map, full + st, col + 64 * k, sp.first(chunk(i)), h, b);
+  // a and b of a chunk land on one barrier (chunk modulo 3), c on its own
+  auto load = [&](uint8_t* tiles, uint64_t* full, int which, int st, int blocks, int col, int i) {
+    for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + (st * blocks + k) * kBlk, &maps.in[which], full, col + 64 * k, sp.first(chunk(i)), h, b);
   };
-  auto load_a = [&](int i) { load(smem + L::oA, bFullA, &maps.in[maps.ia[blockIdx.z]], i % L::kA, CB, 0, i); };
-  auto load_b = [&](int i) { load(smem + L::oB, bFullB, &maps.in[maps.ib[blockIdx.z]], i % L::kB, CB, 0, i); };
-  auto load_c = [&](int i) { load(smem + L::oC, bFullC, &maps.in[maps.ic[blockIdx.z]], i % L::kC, 1, c0, i); };
+  auto load_a = [&](int i) { load(smem + L::oA, bFull + i % 3, maps.ia[blockIdx.z], i % L::kA, CB, 0, i); };
+  auto load_b = [&](int i) {
+    mbar_expect_tx(bFull + i % 3, 2 * CB * kBlk);
+    load(smem + L::oB, bFull + i % 3, maps.ib[blockIdx.z], i % L::kB, CB, 0, i);
+  };
+  auto load_c = [&](int i) {
+    mbar_expect_tx(bFullC + i % L::kC, kBlk);
+    load(smem + L::oC, bFullC + i % L::kC, maps.ic[blockIdx.z], i % L::kC, 1, c0, i);
+  };
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) { mbar_init(bFullA + i, 1); mbar_init(bFullB + i, 1); mbar_init(bFullC + i, 1); }
+    for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFreeA + i, 1); mbar_init(bFreeB + i, 1); mbar_init(bFreeC + i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); }
     mbar_init(bYx, 1); mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128); mbar_init(bY, 1); mbar_init(bYFree, 256);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
@@ -338,15 +345,38 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     if (!mbar_try_wait(bar, parity & 1) && !gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag);
   };
 
-  if (warp == L::kWarpI) {
-    // ---- loads and products ------------------------------------------------------------------------------------------
+  if (warp == L::kWarpI + 1) {
+    // ---- loads: a tile is refilled when the products that read it have completed ------------------------------------------
+    const int n = __reduce_max_sync(0xffffffffu, mine);
+    for (int i = 0; i < n && !gave_up(); ++i) {
+      if (i + L::kB < n) {                         // b: S and B^T C
+        wait(bFreeB + i % L::kB, i / L::kB);
+        if (elect_one()) load_b(i + L::kB);
+        __syncwarp();
+      }
+      if (i + L::kA < n) {                         // a: S and A X
+        wait(bFreeA + i % L::kA, i / L::kA);
+        if (elect_one()) load_a(i + L::kA);
+        __syncwarp();
+      }
+      if (i + L::kC < n) {                         // c: its weighting, and P C
+        wait(bFreeC + i % L::kC, i / L::kC);
+        if (elect_one()) load_c(i + L::kC);
+        __syncwarp();
+      }
+    }
+    if (gave_up()) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
+      const long long t0 = clock64();
+      while (clock64() - t0 < (1LL << 22)) {}
+    }
+  } else if (warp == L::kWarpI) {
+    // ---- products ------------------------------------------------------------------------------------------------------
     // counts and addresses through a warp reduction: the compiler then keeps them, and the descriptors, in uniform registers
     const int n = __reduce_max_sync(0xffffffffu, mine);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
     constexpr uint32_t id_s = idesc_f16(128, 128, F, F, 0, 0), id_y = idesc_f16(128, 64, F, F, 0, 1);
     auto product_s = [&](int i) {
-      wait(bFullA + i % L::kA, i / L::kA);
-      wait(bFullB + i % L::kB, i / L::kB);
+      wait(bFull + i % 3, i / 3);
       if (sp.live(chunk(i)) < kL) wait(bW, i);     // rows behind the length are cleared first
       tc_fence_after();
       if (elect_one()) {
@@ -363,22 +393,15 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     };
     if (n > 0) product_s(0);
     for (int i = 0; i < n && !gave_up(); ++i) {
-      wait(bFullB + i % L::kB, i / L::kB);
       wait(bW, i);
       if (i > 0) wait(bKvFree, i - 1);
       tc_fence_after();
       if (elect_one()) {
         product_kv<DK, F>(tm + L::cKv, base + L::oB + (i % L::kB) * CB * kBlk, base + L::oW);
         mma_commit(bKv);
+        mma_commit(bFreeB + i % L::kB);
       }
       __syncwarp();
-      // c of the chunk before is used up (its product ran ahead of the one just issued).  Before the next S, which may have
-      // to wait for that chunk's C.
-      if (i > 0 && i - 1 + L::kC < n) {
-        wait(bY, i - 1);
-        if (elect_one()) load_c(i - 1 + L::kC);
-        __syncwarp();
-      }
       if (L::kB > 1 && i + 1 < n) product_s(i + 1);
       wait(bX + (i & 1), i >> 1);
       if (i > 0) wait(bYFree, i - 1);
@@ -391,13 +414,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           for (int kk = 0; kk < DK / 16; ++kk)
             mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
         mma_commit(bYx);
+        mma_commit(bFreeA + i % L::kA);
       }
       __syncwarp();
-      if (i + L::kB < n) {                         // b of this chunk is used up
-        wait(bKv, i);
-        if (elect_one()) load_b(i + L::kB);
-        __syncwarp();
-      }
       wait(bP + (i & 1), i >> 1);
       tc_fence_after();
       if (elect_one()) {
@@ -406,18 +425,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
         mma_commit(bY);
+        mma_commit(bFreeC + i % L::kC);
       }
       __syncwarp();
-      if (i + L::kA < n) {                         // so is a
-        wait(bYx, i);
-        if (elect_one()) load_a(i + L::kA);
-        __syncwarp();
-      }
       if (L::kB == 1 && i + 1 < n) product_s(i + 1);
-    }
-    if (gave_up()) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
-      const long long t0 = clock64();
-      while (clock64() - t0 < (1LL << 22)) {}
     }
   } else if (warp >= L::kWarpX) {
     // ---- the state -----------------------------------------------------------------------------------------------------
@@ -437,16 +448,36 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         *reinterpret_cast<float4*>(in + 128 * j) = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const DecayStep full(ld, kL);
+    // x: eight columns of the state before the chunk, packed for the product
+    auto pack = [&](const float4 (&x)[2], float down, int j) {
+      const float* X = reinterpret_cast<const float*>(x);
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) split2<T>(X[2 * k] * down, X[2 * k + 1] * down, h[k], l[k]);
+      const uint32_t at = L::oX + swz_off<128>(d, (col + j) / 8);
+      *reinterpret_cast<uint4*>(smem + at) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(smem + L::kXTile + at) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+    auto update = [&](const float4 (&x)[2], const DecayStep& decay, const uint32_t (&v)[8], const uint32_t (&lo)[8], int j) {
+      const float* X = reinterpret_cast<const float*>(x);
+      float y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = decay(X[k]) + (__uint_as_float(v[k]) + __uint_as_float(lo[k]));
+      *reinterpret_cast<float4*>(in + 128 * j) = make_float4(y[0], y[1], y[2], y[3]);
+      *reinterpret_cast<float4*>(in + 128 * j + 512) = make_float4(y[4], y[5], y[6], y[7]);
+    };
     for (int i = 0; i < mine; ++i) {
       const int c = chunk(i), cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
-      wait(bKv, i);
+      // In a long chain B^T C is there before the state is, and what is behind the chunk goes out first; in a short one the
+      // state is there first, and A X waits for it.
+      const bool chained = size > 2;
+      if (chained) wait(bKv, i);
       if (i > 0) wait(bYx, i - 1);                 // the product with the packed state of the chunk before is done
       if (size > 1 && c > 0) {
         wait(bIn + w, rank == 0 ? i - 1 : i);
         if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
       }
-      tc_fence_after();
       float down = 1.f;
       if constexpr (kHalfRange) {
         // the largest magnitude of the tile to 2^13 ... 2^14: X may lie outside fp16's range
@@ -465,37 +496,41 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         down = __uint_as_float((uint32_t)(127 - e) << 23);
         if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
       }
+      if (!chained) {
+#pragma unroll 2
+        for (int j = 0; j < NC; j += 8) {
+          const float4 x[2] = {*reinterpret_cast<const float4*>(in + 128 * j), *reinterpret_cast<const float4*>(in + 128 * j + 512)};
+          pack(x, down, j);
+        }
+        fence_proxy_async();
+        arrive_on(bX + (i & 1));
+        wait(bKv, i);
+      }
+      tc_fence_after();
 #pragma unroll 2
       for (int j = 0; j < NC; j += 8) {
         uint32_t v[8], lo[8];
         tmem_ld8(kv + j, v);
         tmem_ld8(kv + 64 + j, lo);
-        float4 x[2] = {*reinterpret_cast<const float4*>(in + 128 * j), *reinterpret_cast<const float4*>(in + 128 * j + 512)};
-        const float* X = reinterpret_cast<const float*>(x);
-        uint32_t h[4], l[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) split2<T>(X[2 * k] * down, X[2 * k + 1] * down, h[k], l[k]);
-        const uint32_t at = L::oX + swz_off<128>(d, (col + j) / 8);
-        *reinterpret_cast<uint4*>(smem + at) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(smem + L::kXTile + at) = make_uint4(l[0], l[1], l[2], l[3]);
+        const float4 x[2] = {*reinterpret_cast<const float4*>(in + 128 * j), *reinterpret_cast<const float4*>(in + 128 * j + 512)};
+        if (chained) pack(x, down, j);
         tmem_wait_ld();
-        float y[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) y[k] = decay(X[k]) + (__uint_as_float(v[k]) + __uint_as_float(lo[k]));
-        *reinterpret_cast<float4*>(in + 128 * j) = make_float4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<float4*>(in + 128 * j + 512) = make_float4(y[4], y[5], y[6], y[7]);
+        update(x, decay, v, lo, j);
       }
-      fence_proxy_async();
+      tc_fence_before();
+      arrive_on(bKvFree);
       if (size > 1 && c + 1 < sp.nch) {
+        fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
           const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
           copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
         }
       }
-      tc_fence_before();
-      arrive_on(bKvFree);
-      arrive_on(bX + (i & 1));
+      if (chained) {
+        fence_proxy_async();
+        arrive_on(bX + (i & 1));
+      }
     }
     // behind the last chunk (or, without one, behind none: rank 0 then)
     const int last = sp.nch > 0 ? (sp.nch - 1) % size : 0;
@@ -510,7 +545,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       const int cnt = sp.live(chunk(i));
       const float w = exp2f(g2 * (float)(rev ? r : max(0, cnt - 1 - r)));
       wait(bFullC + i % L::kC, i / L::kC);
-      if (cnt < kL) wait(bFullB + i % L::kB, i / L::kB);
+      if (cnt < kL) wait(bFull + i % 3, i / 3);
       if (i > 0) wait(bKv, i - 1);                 // the products with the weighted C of the chunk before are done
       weigh_c<T, CB>(r, cnt, w, smem + L::oC + (i % L::kC) * kBlk, smem + L::oW, smem + L::oB + (i % L::kB) * CB * kBlk);
       arrive_on(bW);
