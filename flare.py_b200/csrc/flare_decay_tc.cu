@@ -3,7 +3,8 @@
 //
 //   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 256 threads weigh, mask and pack it there
 //   out = scale * (P C + lambda^(i+1) A X)          X: the state before the chunk, in two 16-bit terms; two accumulators
-//   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms; X itself in fp32
+//   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms where the state is a result, in one
+//                                                   where only outputs are, which round as much themselves; X itself in fp32
 //
 // The mirror image in time (n >= t) walks the chunks from the last and mirrors the weights.
 //
@@ -12,8 +13,8 @@
 // to chunk is one multiply-add of the state and its way to the next SM.  Where even clusters of eight leave SMs idle, the token axis is
 // cut into segments as well: k_decay_tc_sums adds up each, k_decay_prefix makes the states before them.
 //
-// Warps of the walk: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 products, 17 loads.  Everything that
-// the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are cleared in shared memory
+// Warps of the walk: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 and 17 products, 18 loads.  Everything
+// that the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are cleared in shared memory
 // before a product reads them, so that padding may hold NaN.
 //
 // The roles' loops are kept short on purpose: four roles share a scheduler, and unrolled to straight lines they waited for
@@ -68,17 +69,31 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+// two values an instruction
+__device__ __forceinline__ uint64_t& as_u64(float2& x) { return reinterpret_cast<uint64_t&>(x); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(reinterpret_cast<uint64_t&>(r)) : "l"(reinterpret_cast<uint64_t&>(a)), "l"(reinterpret_cast<uint64_t&>(b)));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(as_u64(r)) : "l"(as_u64(a)), "l"(as_u64(b)));
   return r;
 }
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(as_u64(r)) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(as_u64(r)) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return r;
+}
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 floats(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
 // the hi and lo terms of a pair: lo is what rounding to 16 bits left of each
 template <typename T>
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  hi = Op16<T>::pack(x, y);
-  const float2 r = Op16<T>::unpack(hi);
-  lo = Op16<T>::pack(x - r.x, y - r.y);
+__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
+  hi = Op16<T>::pack(x.x, x.y);
+  const float2 r = fma2(Op16<T>::unpack(hi), both(-1.f), x);
+  lo = Op16<T>::pack(r.x, r.y);
 }
 
 // What a chunk is to the CTA that takes it.
@@ -94,46 +109,56 @@ struct Span {
   __device__ __forceinline__ int live(int c) const { return min(kL, n1 - first(c)); }
 };
 
-// C weighted by the decay to the chunk's end, in two terms; one thread a row.  Rows behind the length are cleared, here and in
-// the tiles of b and c themselves.
+// C weighted by the decay to the chunk's end, in two terms or one; one thread a row.  Rows behind the length are cleared, here
+// and in the tiles of b and c themselves.
 template <typename T, int CB>
-__device__ __forceinline__ void weigh_c(int r, int cnt, float w, uint8_t* src, uint8_t* hi_t, uint8_t* b_t) {
-  if (r < cnt) {
-#pragma unroll 2
-    for (int ch = 0; ch < 8; ++ch) {
-      const uint32_t at = swz_off<128>(r, ch);
-      const uint4 x = *reinterpret_cast<const uint4*>(src + at);
-      const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-      uint32_t hs[4], ls[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = mul2(Op16<T>::unpack(xs[i]), make_float2(w, w));
-        split2<T>(f.x, f.y, hs[i], ls[i]);
-      }
-      *reinterpret_cast<uint4*>(hi_t + at) = make_uint4(hs[0], hs[1], hs[2], hs[3]);
-      *reinterpret_cast<uint4*>(hi_t + kBlk + at) = make_uint4(ls[0], ls[1], ls[2], ls[3]);
-    }
-  } else {
+__device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8_t* src, uint8_t* hi_t, uint8_t* lo_t, uint8_t* b_t) {
+  if (r >= cnt) {
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
     for (int ch = 0; ch < 8; ++ch) {
       const uint32_t at = 128 * r + 16 * ch;
       *reinterpret_cast<uint4*>(src + at) = z;
       *reinterpret_cast<uint4*>(hi_t + at) = z;
-      *reinterpret_cast<uint4*>(hi_t + kBlk + at) = z;
+      if (two) *reinterpret_cast<uint4*>(lo_t + at) = z;
 #pragma unroll
       for (int i = 0; i < CB; ++i) *reinterpret_cast<uint4*>(b_t + i * kBlk + at) = z;
+    }
+  } else if (two) {
+#pragma unroll 2
+    for (int ch = 0; ch < 8; ++ch) {
+      const uint32_t at = swz_off<128>(r, ch);
+      const uint4 x = *reinterpret_cast<const uint4*>(src + at);
+      uint4 hi, lo;
+      split2<T>(mul2(Op16<T>::unpack(x.x), both(w)), hi.x, lo.x);
+      split2<T>(mul2(Op16<T>::unpack(x.y), both(w)), hi.y, lo.y);
+      split2<T>(mul2(Op16<T>::unpack(x.z), both(w)), hi.z, lo.z);
+      split2<T>(mul2(Op16<T>::unpack(x.w), both(w)), hi.w, lo.w);
+      *reinterpret_cast<uint4*>(hi_t + at) = hi;
+      *reinterpret_cast<uint4*>(lo_t + at) = lo;
+    }
+  } else {
+    auto weighed = [&](uint32_t x) {
+      const float2 f = mul2(Op16<T>::unpack(x), both(w));
+      return Op16<T>::pack(f.x, f.y);
+    };
+#pragma unroll 4
+    for (int ch = 0; ch < 8; ++ch) {
+      const uint32_t at = swz_off<128>(r, ch);
+      const uint4 x = *reinterpret_cast<const uint4*>(src + at);
+      *reinterpret_cast<uint4*>(hi_t + at) = make_uint4(weighed(x.x), weighed(x.y), weighed(x.z), weighed(x.w));
     }
   }
   fence_proxy_async();
 }
 
-// B^T (hi | lo): 128 x 128, the lo terms in the upper columns.  For 64 features the 128 rows are the features twice (the second
-// block of the operand starts where the first does), so that each of the state's 128 threads has half a row to update.
+// B^T (hi | lo): 128 x 128 with the lo terms in the upper columns, or B^T hi alone.  For 64 features the 128 rows are the
+// features twice (the second block of the operand starts where the first does), so that each of the state's 128 threads has
+// half a row to update.
 template <int DK, int F>
-__device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t w_tile) {
-  const uint32_t id = idesc_f16(128, 128, F, F, 1, 1);
+__device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t w_tile, bool two) {
   const uint64_t dB = smem_desc_mn128(b_tile, DK == 128 ? kBlk : 0, 1024), dW = smem_desc_mn128(w_tile, kBlk, 1024);
+  const uint32_t id = two ? idesc_f16(128, 128, F, F, 1, 1) : idesc_f16(128, 64, F, F, 1, 1);
 #pragma unroll
   for (int kk = 0; kk < 8; ++kk) mma_ss(d, dB + 128 * kk, dW + 128 * kk, id, kk > 0);
 }
@@ -197,7 +222,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if (c > 0) wait(bKvFree, c - 1);
       tc_fence_after();
       if (elect_one()) {
-        product_kv<DK, F>(d, base + L::oB + st * CB * kBlk, base + L::oW);
+        product_kv<DK, F>(d, base + L::oB + st * CB * kBlk, base + L::oW, true);
         mma_commit(bKv);
       }
       __syncwarp();
@@ -248,7 +273,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       const float w = exp2f(g2 * (float)(sp.rev ? tid : max(0, cnt - 1 - tid)));
       wait(bFull + st, c / NST);
       if (c > 0) wait(bKv, c - 1);                 // the products with the weighted C of the chunk before are done
-      weigh_c<T, CB>(tid, cnt, w, smem + L::oC + st * kBlk, smem + L::oW, smem + L::oB + st * CB * kBlk);
+      weigh_c<T, CB>(tid, cnt, w, true, smem + L::oC + st * kBlk, smem + L::oW, smem + L::oW + kBlk, smem + L::oB + st * CB * kBlk);
       arrive_on(bW);
     }
   }
@@ -260,16 +285,17 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 // ---- the walk --------------------------------------------------------------------------------------------------------------
 template <int DK> struct WalkPlan {
   static constexpr int kCB = DK / 64;
-  // Tiles in flight.  Shared memory holds three chunks of 64 features; of 128 features two tiles of a and of c, and one of b,
-  // which is free as soon as S and B^T C have been formed.
+  // Tiles in flight: three chunks of 64 features; of 128 features two, and one of b, which is free as soon as S and B^T C have
+  // been formed.
   static constexpr int kA = DK == 64 ? 3 : 2, kB = DK == 64 ? 3 : 1, kC = DK == 64 ? 3 : 2;
+  static constexpr int kW = 2;                     // tiles for the weighted C: two terms, or two buffers of one
   static constexpr bool kStage = DK == 64;         // outputs leave through shared memory and the TMA
   static constexpr int kXTile = DK * 128;          // one term of the packed state: [DK][64]
   static constexpr int kXBytes = DK * 64 * 4;      // the state in fp32 as it arrives
-  static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + 2 * kBlk,
+  static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + kW * kBlk,
                        oIn = oX + 2 * kXTile, oOut = oIn + kXBytes, oBars = oOut + (kStage ? kBlk : 0);
   static constexpr int kBytes = oBars + 512 + 1024;
-  static constexpr int kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 2);
+  static constexpr int kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 3);
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
 };
 
@@ -283,13 +309,13 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
-  uint64_t *bFull = bars, *bFullC = bars + 3, *bS = bars + 9, *bP = bars + 11, *bX = bars + 13, *bYx = bars + 15, *bW = bars + 16,
-           *bKv = bars + 17, *bKvFree = bars + 18, *bY = bars + 19, *bYFree = bars + 20, *bIn = bars + 21;    // bIn: one a warp of the state
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 25);
-  int* abort_flag = reinterpret_cast<int*>(bars + 26);
-  float* sExp = reinterpret_cast<float*>(bars + 28);         // 2^e of the packed state, by chunk modulo 4
-  uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 30);   // [2][4]
-  uint64_t *bFreeA = bars + 34, *bFreeB = bars + 37, *bFreeC = bars + 40;     // by tile
+  uint64_t *bFull = bars, *bFullC = bars + 3, *bFreeA = bars + 6, *bFreeB = bars + 9, *bFreeC = bars + 12, *bS = bars + 15, *bP = bars + 17,
+           *bX = bars + 19, *bW = bars + 21, *bKv = bars + 23, *bYx = bars + 25, *bKvFree = bars + 26, *bY = bars + 27, *bYFree = bars + 28,
+           *bIn = bars + 29;                                 // bIn: one a warp of the state
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
+  int* abort_flag = reinterpret_cast<int*>(bars + 34);
+  float* sExp = reinterpret_cast<float*>(bars + 36);         // 2^e of the packed state, by chunk modulo 4
+  uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 38);   // [2][4]
 
   const DecayUnit& u = a.u[blockIdx.z];
   const int n_cb = (u.Dc + 63) / 64, size = cluster_size(), rank = cluster_rank();
@@ -303,24 +329,32 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const int mine = (sp.nch - rank + size - 1) / size;        // chunks rank, rank + size, ... are this CTA's: 0, 1, ... below
   const float ld = a.log_decay[h], g2 = decay_log2(ld);
   auto chunk = [&](int i) { return rank + size * i; };
+  const bool two = u.state_out != nullptr;
+  const int n_w = two ? 1 : 2;                     // buffers of the weighted C
+  auto w_tile = [&](int i) { return L::oW + (two ? 0 : (i & 1) * kBlk); };
 
-  // a and b of a chunk land on one barrier (chunk modulo 3), c on its own
+  // a and b of a chunk land on one barrier, c on its own
   auto load = [&](uint8_t* tiles, uint64_t* full, int which, int st, int blocks, int col, int i) {
     for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + (st * blocks + k) * kBlk, &maps.in[which], full, col + 64 * k, sp.first(chunk(i)), h, b);
   };
-  auto load_a = [&](int i) { load(smem + L::oA, bFull + i % 3, maps.ia[blockIdx.z], i % L::kA, CB, 0, i); };
+  auto load_a = [&](int i) { load(smem + L::oA, bFull + i % L::kA, maps.ia[blockIdx.z], i % L::kA, CB, 0, i); };
   auto load_b = [&](int i) {
-    mbar_expect_tx(bFull + i % 3, 2 * CB * kBlk);
-    load(smem + L::oB, bFull + i % 3, maps.ib[blockIdx.z], i % L::kB, CB, 0, i);
+    mbar_expect_tx(bFull + i % L::kA, 2 * CB * kBlk);
+    load(smem + L::oB, bFull + i % L::kA, maps.ib[blockIdx.z], i % L::kB, CB, 0, i);
   };
   auto load_c = [&](int i) {
     mbar_expect_tx(bFullC + i % L::kC, kBlk);
     load(smem + L::oC, bFullC + i % L::kC, maps.ic[blockIdx.z], i % L::kC, 1, c0, i);
   };
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFreeA + i, 1); mbar_init(bFreeB + i, 1); mbar_init(bFreeC + i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); }
-    mbar_init(bYx, 1); mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128); mbar_init(bY, 1); mbar_init(bYFree, 256);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1);
+      mbar_init(bFreeA + i, 2); mbar_init(bFreeB + i, 2); mbar_init(bFreeC + i, 2);       // two products each
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1);
+    }
+    mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bY, 2); mbar_init(bYFree, 256);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -345,90 +379,106 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     if (!mbar_try_wait(bar, parity & 1) && !gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag);
   };
 
-  if (warp == L::kWarpI + 1) {
-    // ---- loads: a tile is refilled when the products that read it have completed ------------------------------------------
-    const int n = __reduce_max_sync(0xffffffffu, mine);
-    for (int i = 0; i < n && !gave_up(); ++i) {
-      if (i + L::kB < n) {                         // b: S and B^T C
-        wait(bFreeB + i % L::kB, i / L::kB);
-        if (elect_one()) load_b(i + L::kB);
-        __syncwarp();
-      }
-      if (i + L::kA < n) {                         // a: S and A X
-        wait(bFreeA + i % L::kA, i / L::kA);
-        if (elect_one()) load_a(i + L::kA);
-        __syncwarp();
-      }
-      if (i + L::kC < n) {                         // c: its weighting, and P C
-        wait(bFreeC + i % L::kC, i / L::kC);
-        if (elect_one()) load_c(i + L::kC);
-        __syncwarp();
-      }
-    }
-    if (gave_up()) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
-      const long long t0 = clock64();
-      while (clock64() - t0 < (1LL << 22)) {}
-    }
-  } else if (warp == L::kWarpI) {
-    // ---- products ------------------------------------------------------------------------------------------------------
+  if (warp >= L::kWarpI) {
     // counts and addresses through a warp reduction: the compiler then keeps them, and the descriptors, in uniform registers
     const int n = __reduce_max_sync(0xffffffffu, mine);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
     constexpr uint32_t id_s = idesc_f16(128, 128, F, F, 0, 0), id_y = idesc_f16(128, 64, F, F, 0, 1);
-    auto product_s = [&](int i) {
-      wait(bFull + i % 3, i / 3);
-      if (sp.live(chunk(i)) < kL) wait(bW, i);     // rows behind the length are cleared first
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t dA = smem_desc<128>(base + L::oA + (i % L::kA) * CB * kBlk), dB = smem_desc<128>(base + L::oB + (i % L::kB) * CB * kBlk);
-        const uint32_t d = tm + 128 * (i & 1);
+    auto tile_a = [&](int i) { return smem_desc<128>(base + L::oA + i % L::kA * (CB * kBlk)); };
+    if (warp == L::kWarpI) {
+      // ---- S = A B^T and P C -------------------------------------------------------------------------------------------
+      auto product_s = [&](int i) {
+        wait(bFull + i % L::kA, i / L::kA);
+        if (sp.live(chunk(i)) < kL) wait(bW + (i & 1), i >> 1);        // rows behind the length are cleared first
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dA = tile_a(i), dB = smem_desc<128>(base + L::oB + i % L::kB * (CB * kBlk));
+          const uint32_t d = tm + 128 * (i & 1);
 #pragma unroll
-        for (int kk = 0; kk < DK / 16; ++kk) {
-          const uint32_t off = (kk / 4) * (kBlk >> 4) + 2 * (kk & 3);
-          mma_ss(d, dA + off, dB + off, id_s, kk > 0);
+          for (int kk = 0; kk < DK / 16; ++kk) {
+            const uint32_t off = (kk / 4) * (kBlk >> 4) + 2 * (kk & 3);
+            mma_ss(d, dA + off, dB + off, id_s, kk > 0);
+          }
+          mma_commit(bS + (i & 1));
+          mma_commit(bFreeA + i % L::kA);
+          mma_commit(bFreeB + i % L::kB);
         }
-        mma_commit(bS + (i & 1));
-      }
-      __syncwarp();
-    };
-    if (n > 0) product_s(0);
-    for (int i = 0; i < n && !gave_up(); ++i) {
-      wait(bW, i);
-      if (i > 0) wait(bKvFree, i - 1);
-      tc_fence_after();
-      if (elect_one()) {
-        product_kv<DK, F>(tm + L::cKv, base + L::oB + (i % L::kB) * CB * kBlk, base + L::oW);
-        mma_commit(bKv);
-        mma_commit(bFreeB + i % L::kB);
-      }
-      __syncwarp();
-      if (L::kB > 1 && i + 1 < n) product_s(i + 1);
-      wait(bX + (i & 1), i >> 1);
-      if (i > 0) wait(bYFree, i - 1);
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t dA = smem_desc<128>(base + L::oA + (i % L::kA) * CB * kBlk), dX = smem_desc<128>(base + L::oX);
+        __syncwarp();
+      };
+      if (n > 0) product_s(0);
+      for (int i = 0; i < n && !gave_up(); ++i) {
+        if (L::kB > 1 && i + 1 < n) product_s(i + 1);
+        wait(bP + (i & 1), i >> 1);
+        if (i > 0) wait(bYFree, i - 1);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dC = smem_desc<128>(base + L::oC + i % L::kC * kBlk);
+          const uint32_t p = tm + 128 * (i & 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int kk = 0; kk < DK / 16; ++kk)
-            mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
-        mma_commit(bYx);
-        mma_commit(bFreeA + i % L::kA);
+          for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
+          mma_commit(bY);
+          mma_commit(bFreeC + i % L::kC);
+        }
+        __syncwarp();
+        if (L::kB == 1 && i + 1 < n) product_s(i + 1);
       }
-      __syncwarp();
-      wait(bP + (i & 1), i >> 1);
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t dC = smem_desc<128>(base + L::oC + (i % L::kC) * kBlk);
-        const uint32_t p = tm + 128 * (i & 1);
+    } else if (warp == L::kWarpI + 1) {
+      // ---- B^T C, a chunk ahead, and A X ---------------------------------------------------------------------------------
+      auto product_bc = [&](int i) {
+        wait(bFull + i % L::kA, i / L::kA);
+        wait(bW + (i & 1), i >> 1);
+        if (i > 0) wait(bKvFree, i - 1);
+        tc_fence_after();
+        if (elect_one()) {
+          product_kv<DK, F>(tm + L::cKv, base + L::oB + i % L::kB * (CB * kBlk), base + w_tile(i), two);
+          mma_commit(bKv + (i & 1));
+          mma_commit(bFreeB + i % L::kB);
+          mma_commit(bFreeC + i % L::kC);          // c has been weighed
+        }
+        __syncwarp();
+      };
+      if (n > 0) product_bc(0);
+      for (int i = 0; i < n && !gave_up(); ++i) {
+        if (i + 1 < n) product_bc(i + 1);
+        wait(bX + (i & 1), i >> 1);
+        if (i > 0) wait(bYFree, i - 1);
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t dA = tile_a(i), dX = smem_desc<128>(base + L::oX);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
-        mma_commit(bY);
-        mma_commit(bFreeC + i % L::kC);
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int kk = 0; kk < DK / 16; ++kk)
+              mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
+          mma_commit(bYx);
+          mma_commit(bFreeA + i % L::kA);
+          mma_commit(bY);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (L::kB == 1 && i + 1 < n) product_s(i + 1);
+    } else {
+      // ---- loads: a tile is refilled when the two products that read it have completed -----------------------------------
+      for (int i = 0; i < n && !gave_up(); ++i) {
+        if (i + L::kB < n) {
+          wait(bFreeB + i % L::kB, i / L::kB);
+          if (elect_one()) load_b(i + L::kB);
+          __syncwarp();
+        }
+        if (i + L::kA < n) {
+          wait(bFreeA + i % L::kA, i / L::kA);
+          if (elect_one()) load_a(i + L::kA);
+          __syncwarp();
+        }
+        if (i + L::kC < n) {
+          wait(bFreeC + i % L::kC, i / L::kC);
+          if (elect_one()) load_c(i + L::kC);
+          __syncwarp();
+        }
+      }
+      if (gave_up()) {                             // copies in flight end (within microseconds) before the CTA's memory is given back
+        const long long t0 = clock64();
+        while (clock64() - t0 < (1LL << 22)) {}
+      }
     }
   } else if (warp >= L::kWarpX) {
     // ---- the state -----------------------------------------------------------------------------------------------------
@@ -448,89 +498,127 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         *reinterpret_cast<float4*>(in + 128 * j) = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
     const DecayStep full(ld, kL);
-    // x: eight columns of the state before the chunk, packed for the product
-    auto pack = [&](const float4 (&x)[2], float down, int j) {
-      const float* X = reinterpret_cast<const float*>(x);
-      uint32_t h[4], l[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) split2<T>(X[2 * k] * down, X[2 * k + 1] * down, h[k], l[k]);
+    // eight columns of the state before the chunk, packed for the product
+    auto pack = [&](const float4& x0, const float4& x1, float down, int j) {
+      uint4 h, l;
+      split2<T>(mul2(make_float2(x0.x, x0.y), both(down)), h.x, l.x);
+      split2<T>(mul2(make_float2(x0.z, x0.w), both(down)), h.y, l.y);
+      split2<T>(mul2(make_float2(x1.x, x1.y), both(down)), h.z, l.z);
+      split2<T>(mul2(make_float2(x1.z, x1.w), both(down)), h.w, l.w);
       const uint32_t at = L::oX + swz_off<128>(d, (col + j) / 8);
-      *reinterpret_cast<uint4*>(smem + at) = make_uint4(h[0], h[1], h[2], h[3]);
-      *reinterpret_cast<uint4*>(smem + L::kXTile + at) = make_uint4(l[0], l[1], l[2], l[3]);
+      *reinterpret_cast<uint4*>(smem + at) = h;
+      *reinterpret_cast<uint4*>(smem + L::kXTile + at) = l;
     };
-    auto update = [&](const float4 (&x)[2], const DecayStep& decay, const uint32_t (&v)[8], const uint32_t (&lo)[8], int j) {
-      const float* X = reinterpret_cast<const float*>(x);
-      float y[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) y[k] = decay(X[k]) + (__uint_as_float(v[k]) + __uint_as_float(lo[k]));
-      *reinterpret_cast<float4*>(in + 128 * j) = make_float4(y[0], y[1], y[2], y[3]);
-      *reinterpret_cast<float4*>(in + 128 * j + 512) = make_float4(y[4], y[5], y[6], y[7]);
+    auto stepped = [&](const float4& x, const DecayStep& decay, const float2& v0, const float2& v1) {
+      const float2 m = both(decay.mul), k = both(decay.keep), a0 = make_float2(x.x, x.y), a1 = make_float2(x.z, x.w);
+      const float2 y0 = add2(fma2(m, a0, mul2(k, a0)), v0), y1 = add2(fma2(m, a1, mul2(k, a1)), v1);
+      return make_float4(y0.x, y0.y, y1.x, y1.y);
+    };
+    // the largest magnitude of an fp16 tile to 2^13 ... 2^14: X may lie outside fp16's range
+    auto scale_down = [&](uint32_t top, int i) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) sMax[4 * (i & 1) + w] = top;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
+      top = max(max(all.x, all.y), max(all.z, all.w));
+      const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
+      if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
+      return __uint_as_float((uint32_t)(127 - e) << 23);
+    };
+    auto magnitude = [](const float4& x) {
+      return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+    };
+    auto send = [&](int c) {                       // what this warp has written, to the CTA of the next chunk
+      if (size == 1 || c + 1 == sp.nch) return;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
+        copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
+      }
+    };
+    auto receive = [&](int i, int c) {
+      if (size == 1 || c == 0) return;
+      wait(bIn + w, rank == 0 ? i - 1 : i);
+      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
     };
     for (int i = 0; i < mine; ++i) {
       const int c = chunk(i), cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
-      // In a long chain B^T C is there before the state is, and what is behind the chunk goes out first; in a short one the
-      // state is there first, and A X waits for it.
-      const bool chained = size > 2;
-      if (chained) wait(bKv, i);
-      if (i > 0) wait(bYx, i - 1);                 // the product with the packed state of the chunk before is done
-      if (size > 1 && c > 0) {
-        wait(bIn + w, rank == 0 ? i - 1 : i);
-        if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
-      }
-      float down = 1.f;
-      if constexpr (kHalfRange) {
-        // the largest magnitude of the tile to 2^13 ... 2^14: X may lie outside fp16's range
-        uint32_t top = 0;
-#pragma unroll 2
-        for (int j = 0; j < NC; j += 4) {
-          const uint4 t = *reinterpret_cast<const uint4*>(in + 128 * j);
-          top = max(max(max(top, t.x & 0x7fffffffu), t.y & 0x7fffffffu), max(t.z & 0x7fffffffu, t.w & 0x7fffffffu));
+      wait(bKv + (i & 1), i >> 1);
+      tc_fence_after();
+      if constexpr (DK == 64) {
+        // all of a thread's 32 columns in registers: B^T C before the state arrives, then the state behind the chunk, which the
+        // next CTA waits for, and last the packing for this chunk's product
+        float2 v[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 16) {
+          uint32_t h[16];
+          tmem_ld16(kv + j, h);
+          if (two) {
+            uint32_t l[16];
+            tmem_ld16(kv + 64 + j, l);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[j / 2 + k] = add2(floats(h[2 * k], h[2 * k + 1]), floats(l[2 * k], l[2 * k + 1]));
+          } else {
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[j / 2 + k] = floats(h[2 * k], h[2 * k + 1]);
+          }
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) sMax[4 * (i & 1) + w] = top;
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
-        top = max(max(all.x, all.y), max(all.z, all.w));
-        const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
-        down = __uint_as_float((uint32_t)(127 - e) << 23);
-        if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
-      }
-      if (!chained) {
+        tc_fence_before();
+        arrive_on(bKvFree);
+        receive(i, c);
+        float4 x[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = *reinterpret_cast<const float4*>(in + 512 * q);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) *reinterpret_cast<float4*>(in + 512 * q) = stepped(x[q], decay, v[2 * q], v[2 * q + 1]);
+        send(c);
+        float down = 1.f;
+        if constexpr (kHalfRange) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) top = max(top, magnitude(x[q]));
+          down = scale_down(top, i);
+        }
+        if (i > 0) wait(bYx, i - 1);               // the product with the packed state of the chunk before is done
+#pragma unroll
+        for (int q = 0; q < 8; q += 2) pack(x[q], x[q + 1], down, 4 * q);
+      } else {
+        if (i > 0) wait(bYx, i - 1);
+        receive(i, c);
+        float down = 1.f;
+        if constexpr (kHalfRange) {
+          uint32_t top = 0;
+#pragma unroll 2
+          for (int j = 0; j < NC; j += 4) top = max(top, magnitude(*reinterpret_cast<const float4*>(in + 128 * j)));
+          down = scale_down(top, i);
+        }
 #pragma unroll 2
         for (int j = 0; j < NC; j += 8) {
-          const float4 x[2] = {*reinterpret_cast<const float4*>(in + 128 * j), *reinterpret_cast<const float4*>(in + 128 * j + 512)};
-          pack(x, down, j);
+          uint32_t h[8], l[8];
+          tmem_ld8(kv + j, h);
+          if (two) {
+            tmem_ld8(kv + 64 + j, l);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) l[k] = 0u;
+          }
+          const float4 x0 = *reinterpret_cast<const float4*>(in + 128 * j), x1 = *reinterpret_cast<const float4*>(in + 128 * j + 512);
+          pack(x0, x1, down, j);
+          tmem_wait_ld();
+          auto v = [&](int k) { return add2(floats(h[k], h[k + 1]), floats(l[k], l[k + 1])); };
+          *reinterpret_cast<float4*>(in + 128 * j) = stepped(x0, decay, v(0), v(2));
+          *reinterpret_cast<float4*>(in + 128 * j + 512) = stepped(x1, decay, v(4), v(6));
         }
-        fence_proxy_async();
-        arrive_on(bX + (i & 1));
-        wait(bKv, i);
+        send(c);
+        tc_fence_before();
+        arrive_on(bKvFree);
       }
-      tc_fence_after();
-#pragma unroll 2
-      for (int j = 0; j < NC; j += 8) {
-        uint32_t v[8], lo[8];
-        tmem_ld8(kv + j, v);
-        tmem_ld8(kv + 64 + j, lo);
-        const float4 x[2] = {*reinterpret_cast<const float4*>(in + 128 * j), *reinterpret_cast<const float4*>(in + 128 * j + 512)};
-        if (chained) pack(x, down, j);
-        tmem_wait_ld();
-        update(x, decay, v, lo, j);
-      }
-      tc_fence_before();
-      arrive_on(bKvFree);
-      if (size > 1 && c + 1 < sp.nch) {
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-          const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
-          copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
-        }
-      }
-      if (chained) {
-        fence_proxy_async();
-        arrive_on(bX + (i & 1));
-      }
+      fence_proxy_async();
+      arrive_on(bX + (i & 1));
     }
     // behind the last chunk (or, without one, behind none: rank 0 then)
     const int last = sp.nch > 0 ? (sp.nch - 1) % size : 0;
@@ -545,17 +633,20 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       const int cnt = sp.live(chunk(i));
       const float w = exp2f(g2 * (float)(rev ? r : max(0, cnt - 1 - r)));
       wait(bFullC + i % L::kC, i / L::kC);
-      if (cnt < kL) wait(bFull + i % 3, i / 3);
-      if (i > 0) wait(bKv, i - 1);                 // the products with the weighted C of the chunk before are done
-      weigh_c<T, CB>(r, cnt, w, smem + L::oC + (i % L::kC) * kBlk, smem + L::oW, smem + L::oB + (i % L::kB) * CB * kBlk);
-      arrive_on(bW);
+      if (cnt < kL) wait(bFull + i % L::kA, i / L::kA);
+      if (i >= n_w) wait(bKv + ((i - n_w) & 1), (i - n_w) >> 1);       // the product with what stood here is done
+      uint8_t* hi = smem + w_tile(i);
+      weigh_c<T, CB>(r, cnt, w, two, smem + L::oC + i % L::kC * kBlk, hi, hi + kBlk, smem + L::oB + i % L::kB * (CB * kBlk));
+      arrive_on(bW + (i & 1));
     }
   } else {
     // ---- weights of P, outputs -----------------------------------------------------------------------------------------
     const int r0 = 32 * (warp & 3), r = r0 + lane, hb = warp >> 2;    // token r, half of the columns
     const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
-    // A weight lambda^(i-j) of a block of 16 columns below the diagonal is a factor of the column times one of the (row, block);
-    // the two blocks that the diagonal crosses in a warp's rows take an exponential each.
+    // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
+    // diagonal the latter exceeds 1, up to lambda^-15, which is in range for every decay above 2^-8 a token; the others take an
+    // exponential each there.
+    const bool mild = g2 >= -8.f;
     float2 wcol[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -582,21 +673,33 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           tmem_ld16(s + 16 * k, v);
           const float row = exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15));
           tmem_wait_ld();
+          const int d = rev ? j0 - r : r - j0, sign = rev ? 1 : -1;    // i - j of the first column, and its change
           if (all) {
-            const float2 f = make_float2(row, row);
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
-              const float2 x = mul2(mul2(make_float2(__uint_as_float(v[2 * m]), __uint_as_float(v[2 * m + 1])), wcol[m]), f);
+              const float2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), both(row));
               p[m] = Op16<T>::pack(x.x, x.y);
             }
-          } else {
-            const int d = rev ? j0 - r : r - j0, sign = rev ? 1 : -1;
+          } else if (mild && cnt == kL) {
 #pragma unroll
-            for (int m = 0; m < 16; m += 2) {
-              const int d0 = d + sign * m, d1 = d0 + sign;
-              const float x0 = d0 >= 0 && j0 + m < cnt ? __uint_as_float(v[m]) * exp2f(g2 * (float)d0) : 0.f;
-              const float x1 = d1 >= 0 && j0 + m + 1 < cnt ? __uint_as_float(v[m + 1]) * exp2f(g2 * (float)d1) : 0.f;
-              p[m / 2] = Op16<T>::pack(x0, x1);
+            for (int m = 0; m < 8; ++m) {
+              const float2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), both(row));
+              p[m] = Op16<T>::pack(d + sign * (2 * m) >= 0 ? x.x : 0.f, d + sign * (2 * m + 1) >= 0 ? x.y : 0.f);
+            }
+          } else {
+#pragma unroll 1
+            for (int m = 0; m < 8; ++m) {
+              const int d0 = d + sign * (2 * m), d1 = d0 + sign, j = j0 + 2 * m;
+              uint32_t s0 = 0, s1 = 0;
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (q == m) { s0 = v[2 * q]; s1 = v[2 * q + 1]; }
+              const float x0 = d0 >= 0 && j < cnt ? __uint_as_float(s0) * exp2f(g2 * (float)d0) : 0.f;
+              const float x1 = d1 >= 0 && j + 1 < cnt ? __uint_as_float(s1) * exp2f(g2 * (float)d1) : 0.f;
+              const uint32_t t = Op16<T>::pack(x0, x1);
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (q == m) p[q] = t;
             }
           }
         }
@@ -625,11 +728,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         uint32_t q[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const uint32_t t = Op16<T>::pack(fmaf(fx, __uint_as_float(x[2 * m]), a.scale * __uint_as_float(y[2 * m])),
-                                           fmaf(fx, __uint_as_float(x[2 * m + 1]), a.scale * __uint_as_float(y[2 * m + 1])));
-          q[m] = r < cnt ? t : 0u;                 // rows behind the sequence: zeros
+          const float2 t = fma2(both(fx), floats(x[2 * m], x[2 * m + 1]), mul2(both(a.scale), floats(y[2 * m], y[2 * m + 1])));
+          q[m] = Op16<T>::pack(t.x, t.y);
         }
-        const uint4 o = make_uint4(q[0], q[1], q[2], q[3]);
+        uint4 o = make_uint4(q[0], q[1], q[2], q[3]);
+        if (r >= cnt) o = make_uint4(0u, 0u, 0u, 0u);        // rows behind the sequence: zeros
         if constexpr (L::kStage) *reinterpret_cast<uint4*>(smem + L::oOut + swz_off<128>(r, 4 * hb + k)) = o;
         else if (tok0 + r < a.N && 8 * k < cols) *reinterpret_cast<uint4*>(out + (long long)(tok0 + r) * u.os[2] + 8 * k) = o;
       }

@@ -75,7 +75,9 @@ def test_prefill_matches_the_recurrence(fb, cuda_dev, shape, dtype):
     y0, end0 = fb.decay_linear_prefill(q, k, v, ld, scale)
     y0_ref, end0_ref = O.decay_linear_recurrent(q, k, v, ld, scale)
     assert rel(y0, y0_ref) <= tol_y(dtype) and rel(end0, end0_ref) <= tol_state(dtype)
-    assert torch.equal(fb.decay_linear(q, k, v, ld, scale), y0)
+    # without a state to return, the weighted values of the chunks' sums are rounded to 16 bits like the weights inside a chunk:
+    # each share of an output carries one such rounding, so the bound is the same
+    assert rel(fb.decay_linear(q, k, v, ld, scale), y0_ref) <= tol_y(dtype)
     assert fb.device_status() == 0
 
 
