@@ -34,12 +34,25 @@ constexpr int kL = 128;                            // tokens of a chunk
 constexpr int kBlk = 128 * 128;                    // bytes of a [128 rows][64] tile
 
 struct DecayMaps {
-  CUtensorMap in[4], out[kDecayUnits];             // boxes of [128 tokens][64 features]
+  CUtensorMap in[4], out[kDecayUnits];             // boxes of [128 tokens][64 features], of the outputs [32][32]
   int ia[kDecayUnits], ib[kDecayUnits], ic[kDecayUnits];
 };
 
 __device__ __forceinline__ void arrive_on(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// A bounded wait, as short in instructions as it can be: the roles of a kernel wait in some thirty places.  A try suspends the
+// thread for a while by itself; after four million of them (seconds) the CTA's abort flag is set, every later wait of the CTA
+// returns at once, and the CTA ends, with the status word's bit set.
+constexpr int kTries = 1 << 22;
+__device__ __forceinline__ bool gave_up(int* abort_flag) { return *reinterpret_cast<volatile int*>(abort_flag) != 0; }
+__device__ __forceinline__ void wait_on(uint64_t* bar, int parity, int* abort_flag) {
+#pragma unroll 1
+  for (int n = 0; !mbar_try_wait(bar, parity & 1); ++n)
+    if (n == kTries || gave_up(abort_flag)) {
+      *reinterpret_cast<volatile int*>(abort_flag) = 1;
+      break;
+    }
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -209,14 +222,11 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto gave_up = [&] { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
-  auto wait = [&](uint64_t* bar, int parity) {
-    if (!mbar_try_wait(bar, parity & 1) && !gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag);
-  };
+  auto wait = [&](uint64_t* bar, int parity) { wait_on(bar, parity, abort_flag); };
   if (warp == 8) {
     const int nch = __reduce_max_sync(0xffffffffu, sp.nch);
     const uint32_t d = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
-    for (int c = 0; c < nch && !gave_up(); ++c) {
+    for (int c = 0; c < nch && !gave_up(abort_flag); ++c) {
       const int st = c % NST;
       wait(bW, c);
       if (c > 0) wait(bKvFree, c - 1);
@@ -232,7 +242,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         __syncwarp();
       }
     }
-    if (gave_up()) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
+    if (gave_up(abort_flag)) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
       const long long t0 = clock64();
       while (clock64() - t0 < (1LL << 22)) {}
     }
@@ -244,7 +254,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
     for (int j = 0; j < NC; ++j) X[j] = 0.f;
     const DecayStep full(ld, kL);
-    for (int c = 0; c < sp.nch && !gave_up(); ++c) {
+    for (int c = 0; c < sp.nch && !gave_up(abort_flag); ++c) {
       const int cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
       wait(bKv, c);
@@ -268,7 +278,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (c0 + col + j < u.Dc) *reinterpret_cast<float4*>(end + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
   } else {
     const float g2 = decay_log2(ld);
-    for (int c = 0; c < sp.nch && !gave_up(); ++c) {
+    for (int c = 0; c < sp.nch && !gave_up(abort_flag); ++c) {
       const int st = c % NST, cnt = sp.live(c);
       const float w = exp2f(g2 * (float)(sp.rev ? tid : max(0, cnt - 1 - tid)));
       wait(bFull + st, c / NST);
@@ -279,6 +289,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   }
   tc_fence_before();
   __syncthreads();
+  if (tid == 0 && status && gave_up(abort_flag)) atomicOr(status, kErrWaitTimeout);
   if (warp == 1) tmem_dealloc<128>(tmem);
 }
 
@@ -305,7 +316,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   grid_dep_sync();
   using L = WalkPlan<DK>;
   constexpr int F = Op16<T>::kFmt, CB = L::kCB;
-  constexpr bool kHalfRange = F == 0;              // fp16: the packed state is scaled by a power of two
+  constexpr bool kHalfRange = F == 0;              // fp16: the packed state is scaled by a power of two, the scale is applied last
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
@@ -372,12 +383,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   cluster_sync();                                  // every CTA's barriers stand before a state is sent
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // A wait that runs out marks the launch as failed and every later wait returns at once, so that the CTA ends.  Warps that
-  // meet at a named barrier go through all their chunks all the same.
-  auto gave_up = [&] { return *reinterpret_cast<volatile int*>(abort_flag) != 0; };
-  auto wait = [&](uint64_t* bar, int parity) {
-    if (!mbar_try_wait(bar, parity & 1) && !gave_up()) mbar_wait_hot(bar, parity & 1, status, abort_flag);
-  };
+  auto wait = [&](uint64_t* bar, int parity) { wait_on(bar, parity, abort_flag); };
 
   if (warp >= L::kWarpI) {
     // counts and addresses through a warp reduction: the compiler then keeps them, and the descriptors, in uniform registers
@@ -406,7 +412,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         __syncwarp();
       };
       if (n > 0) product_s(0);
-      for (int i = 0; i < n && !gave_up(); ++i) {
+      for (int i = 0; i < n && !gave_up(abort_flag); ++i) {
         if (L::kB > 1 && i + 1 < n) product_s(i + 1);
         wait(bP + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
@@ -438,7 +444,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         __syncwarp();
       };
       if (n > 0) product_bc(0);
-      for (int i = 0; i < n && !gave_up(); ++i) {
+      for (int i = 0; i < n && !gave_up(abort_flag); ++i) {
         if (i + 1 < n) product_bc(i + 1);
         wait(bX + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
@@ -458,7 +464,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       }
     } else {
       // ---- loads: a tile is refilled when the two products that read it have completed -----------------------------------
-      for (int i = 0; i < n && !gave_up(); ++i) {
+      for (int i = 0; i < n && !gave_up(abort_flag); ++i) {
         if (i + L::kB < n) {
           wait(bFreeB + i % L::kB, i / L::kB);
           if (elect_one()) load_b(i + L::kB);
@@ -475,7 +481,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           __syncwarp();
         }
       }
-      if (gave_up()) {                             // copies in flight end (within microseconds) before the CTA's memory is given back
+      if (gave_up(abort_flag)) {                             // copies in flight end (within microseconds) before the CTA's memory is given back
         const long long t0 = clock64();
         while (clock64() - t0 < (1LL << 22)) {}
       }
@@ -511,7 +517,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     };
     auto stepped = [&](const float4& x, const DecayStep& decay, const float2& v0, const float2& v1) {
       const float2 m = both(decay.mul), k = both(decay.keep), a0 = make_float2(x.x, x.y), a1 = make_float2(x.z, x.w);
-      const float2 y0 = add2(fma2(m, a0, mul2(k, a0)), v0), y1 = add2(fma2(m, a1, mul2(k, a1)), v1);
+      const float2 y0 = fma2(m, a0, fma2(k, a0, v0)), y1 = fma2(m, a1, fma2(k, a1, v1));
       return make_float4(y0.x, y0.y, y1.x, y1.y);
     };
     // the largest magnitude of an fp16 tile to 2^13 ... 2^14: X may lie outside fp16's range
@@ -629,7 +635,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   } else if (warp >= L::kWarpC) {
     // ---- weighted C ----------------------------------------------------------------------------------------------------
     const int r = tid - 32 * L::kWarpC;
-    for (int i = 0; i < mine && !gave_up(); ++i) {
+    for (int i = 0; i < mine && !gave_up(abort_flag); ++i) {
       const int cnt = sp.live(chunk(i));
       const float w = exp2f(g2 * (float)(rev ? r : max(0, cnt - 1 - r)));
       wait(bFullC + i % L::kC, i / L::kC);
@@ -651,7 +657,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       wcol[k] = make_float2(exp2f(g2 * (float)(rev ? 2 * k : 15 - 2 * k)), exp2f(g2 * (float)(rev ? 2 * k + 1 : 14 - 2 * k)));
-    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
+    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1)), scale_p = kHalfRange ? 1.f : a.scale;
     T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0 + 32 * hb;
     const int cols = u.Dc - c0 - 32 * hb;          // of this thread's 32 columns, those that exist
 
@@ -671,7 +677,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         } else {
           uint32_t v[16];
           tmem_ld16(s + 16 * k, v);
-          const float row = exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15));
+          const float row = scale_p * exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15));
           tmem_wait_ld();
           const int d = rev ? j0 - r : r - j0, sign = rev ? 1 : -1;    // i - j of the first column, and its change
           if (all) {
@@ -694,8 +700,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
               for (int q = 0; q < 8; ++q)
                 if (q == m) { s0 = v[2 * q]; s1 = v[2 * q + 1]; }
-              const float x0 = d0 >= 0 && j < cnt ? __uint_as_float(s0) * exp2f(g2 * (float)d0) : 0.f;
-              const float x1 = d1 >= 0 && j + 1 < cnt ? __uint_as_float(s1) * exp2f(g2 * (float)d1) : 0.f;
+              const float x0 = d0 >= 0 && j < cnt ? __uint_as_float(s0) * (scale_p * exp2f(g2 * (float)d0)) : 0.f;
+              const float x1 = d1 >= 0 && j + 1 < cnt ? __uint_as_float(s1) * (scale_p * exp2f(g2 * (float)d1)) : 0.f;
               const uint32_t t = Op16<T>::pack(x0, x1);
 #pragma unroll
               for (int q = 0; q < 8; ++q)
@@ -711,9 +717,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     };
     auto finish = [&](int i) {
       const int c = chunk(i), cnt = sp.live(c), tok0 = sp.first(c);
-      if constexpr (L::kStage) {                   // the tile of the chunk before has left shared memory
-        if (tid == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        asm volatile("bar.sync 2, 256;" ::: "memory");
+      uint8_t* tile = smem + L::oOut + warp * 2048;          // the warp's own [32 rows][32]
+      if constexpr (L::kStage) {                   // that of the chunk before has left shared memory
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
       }
       wait(bY, i);
       tc_fence_after();
@@ -728,20 +735,23 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         uint32_t q[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const float2 t = fma2(both(fx), floats(x[2 * m], x[2 * m + 1]), mul2(both(a.scale), floats(y[2 * m], y[2 * m + 1])));
+          float2 in_chunk = floats(y[2 * m], y[2 * m + 1]);
+          if constexpr (kHalfRange) in_chunk = mul2(both(a.scale), in_chunk);
+          const float2 t = fma2(both(fx), floats(x[2 * m], x[2 * m + 1]), in_chunk);
           q[m] = Op16<T>::pack(t.x, t.y);
         }
         uint4 o = make_uint4(q[0], q[1], q[2], q[3]);
         if (r >= cnt) o = make_uint4(0u, 0u, 0u, 0u);        // rows behind the sequence: zeros
-        if constexpr (L::kStage) *reinterpret_cast<uint4*>(smem + L::oOut + swz_off<128>(r, 4 * hb + k)) = o;
+        if constexpr (L::kStage) *reinterpret_cast<uint4*>(tile + swz_off<64>(lane, k)) = o;
         else if (tok0 + r < a.N && 8 * k < cols) *reinterpret_cast<uint4*>(out + (long long)(tok0 + r) * u.os[2] + 8 * k) = o;
       }
       tc_fence_before();
       arrive_on(bYFree);
       if constexpr (L::kStage) {
         fence_proxy_async();
-        asm volatile("bar.sync 2, 256;" ::: "memory");
-        if (tid == 0) tma_store_4d(&maps.out[blockIdx.z], smem + L::oOut, c0, tok0, h, b);      // clipped at N and at the last column
+        __syncwarp();
+        if (lane == 0 && tok0 + r0 < a.N && cols > 0)        // clipped at N and at the last column
+          tma_store_4d(&maps.out[blockIdx.z], tile, c0 + 32 * hb, tok0 + r0, h, b);
       }
     };
     // With two chunks of a and b in flight the next weights come before this chunk's outputs, else behind them.
@@ -760,10 +770,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (8 * k < cols) *reinterpret_cast<uint4*>(p + 8 * k) = z;
     }
     if constexpr (L::kStage)
-      if (tid == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   cluster_sync();                                  // no CTA leaves while another may still write into it
+  if (tid == 0 && status && gave_up(abort_flag)) atomicOr(status, kErrWaitTimeout);
   if (warp == 1) tmem_dealloc<512>(tmem);
 }
 
@@ -840,16 +851,16 @@ int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
   DecayMaps maps;
   const void* seen[4] = {};
   int n = 0, Da = 0, Dc = 0;
-  auto make = [&](CUtensorMap* m, const void* p, const long long (&s)[3], int D) {
+  auto make = [&](CUtensorMap* m, const void* p, const long long (&s)[3], int D, int cols, uint32_t rows) {
     // a dimension of one entry has no stride of its own: any valid one
     const uint64_t row = a.N > 1 ? s[2] : D, head = a.H > 1 ? s[1] : row * (uint64_t)a.N, batch = a.B > 1 ? s[0] : head * (uint64_t)a.H;
-    return make_tile_map_cols(m, p, dtype == FLARE_BF16 ? 1 : 0, D, 64, (uint64_t)a.N, (uint64_t)a.H, (uint64_t)a.B, 2 * row, 2 * head, 2 * batch, 128);
+    return make_tile_map_cols(m, p, dtype == FLARE_BF16 ? 1 : 0, D, cols, (uint64_t)a.N, (uint64_t)a.H, (uint64_t)a.B, 2 * row, 2 * head, 2 * batch, rows);
   };
   auto map_of = [&](const void* p, const long long (&s)[3], int D, int like) {
     // one tensor is an operand of several units; the same address with another shape is another tensor
     for (int i = 0; i < n; ++i)
       if (i == like && seen[i] == p) return i;
-    if (n == 4 || !make(&maps.in[n], p, s, D)) return -1;
+    if (n == 4 || !make(&maps.in[n], p, s, D, 64, 128)) return -1;
     seen[n] = p;
     return n++;
   };
@@ -857,7 +868,7 @@ int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
     const DecayUnit& u = a.u[i];
     Da = u.Da > Da ? u.Da : Da;
     Dc = u.Dc > Dc ? u.Dc : Dc;
-    if (!make(&maps.out[i], u.out, u.os, u.Dc)) return FLARE_EUNSUPPORTED;
+    if (!make(&maps.out[i], u.out, u.os, u.Dc, 32, 32)) return FLARE_EUNSUPPORTED;
   }
   // the operands in the order dy v k | (v dy) q | (k q dy): each tensor's map is made once
   const int order[3][3] = {{0, 1, 2}, {1, 0, 3}, {2, 3, 0}};
