@@ -41,18 +41,55 @@ struct DecayMaps {
 __device__ __forceinline__ void arrive_on(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-// A bounded wait, as short in instructions as it can be: the roles of a kernel wait in some thirty places.  A try suspends the
-// thread for a while by itself; after four million of them (seconds) the CTA's abort flag is set, every later wait of the CTA
-// returns at once, and the CTA ends, with the status word's bit set.
-constexpr int kTries = 1 << 22;
-__device__ __forceinline__ bool gave_up(int* abort_flag) { return *reinterpret_cast<volatile int*>(abort_flag) != 0; }
-__device__ __forceinline__ void wait_on(uint64_t* bar, int parity, int* abort_flag) {
-#pragma unroll 1
-  for (int n = 0; !mbar_try_wait(bar, parity & 1); ++n)
-    if (n == kTries || gave_up(abort_flag)) {
-      *reinterpret_cast<volatile int*>(abort_flag) = 1;
-      break;
-    }
+// A bounded wait, as short in instructions as it can be: the roles of a kernel wait in some thirty places, half of its warps are
+// waiting at any time, and what they poll with takes issue slots from those that work.  A try suspends the thread for about a
+// hundred clocks; after a second or so of them the wait gives up.
+constexpr uint32_t kTries = 1u << 24;
+__device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
+  uint32_t tries;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mov.u32 %0, 0;\n"
+      "again:\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra done;\n\t"
+      "add.u32 %0, %0, 1;\n\t"
+      "setp.lt.u32 p, %0, %3;\n\t"
+      "@p bra again;\n"
+      "done:\n\t}"
+      : "=&r"(tries) : "r"(smem_u32(bar)), "r"(parity), "n"(kTries) : "memory");
+  return tries < kTries;
+}
+// A thread's waits: once one has run out the others return at once, so that the CTA ends; the status word gets its bit.  Warps
+// that meet at a named barrier go through all their chunks all the same.
+struct Waits {
+  int* status;
+  bool dead = false;
+  __device__ __forceinline__ void operator()(uint64_t* bar, int parity) {
+    if (dead || poll(bar, (uint32_t)parity & 1)) return;
+    dead = true;
+    if (status) atomicOr(status, kErrWaitTimeout);
+  }
+};
+// The wait of a role of several warps: one of them polls, the others sleep at a named barrier.
+template <int ID, int THREADS>
+__device__ __forceinline__ void wait_together(Waits& wait, bool leader, uint64_t* bar, int parity) {
+  if (leader) wait(bar, parity);
+  asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(THREADS) : "memory");
+}
+// Position in a ring of N tiles: its index, and the parity of its barrier's phase.
+template <int N>
+struct Ring {
+  int at = 0, phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++at == N) { at = 0; phase ^= 1; }
+  }
+};
+// A kernel whose waits ran out may have copies in flight: they end (within microseconds) before its memory is given back.
+__device__ __forceinline__ void let_copies_end(bool dead) {
+  if (!dead) return;
+  const long long t0 = clock64();
+  while (clock64() - t0 < (1LL << 22)) {}
 }
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -195,7 +232,6 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
   uint64_t *bFull = bars, *bW = bars + 2, *bKv = bars + 3, *bKvFree = bars + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 5);
-  int* abort_flag = reinterpret_cast<int*>(bars + 6);
   const DecayUnit& u = a.u[blockIdx.z];
   const int n_cb = (u.Dc + 63) / 64;
   const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = u.rev ? blockIdx.y + 1 : blockIdx.y;
@@ -213,7 +249,6 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   if (tid == 0) {
     for (int i = 0; i < NST; ++i) mbar_init(bFull + i, 1);
     mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128);
-    *abort_flag = 0;
     fence_barrier_init();
     for (int c = 0; c < NST && c < sp.nch; ++c) load(c);
   }
@@ -222,11 +257,11 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto wait = [&](uint64_t* bar, int parity) { wait_on(bar, parity, abort_flag); };
+  Waits wait = {status};
   if (warp == 8) {
     const int nch = __reduce_max_sync(0xffffffffu, sp.nch);
     const uint32_t d = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
-    for (int c = 0; c < nch && !gave_up(abort_flag); ++c) {
+    for (int c = 0; c < nch && !wait.dead; ++c) {
       const int st = c % NST;
       wait(bW, c);
       if (c > 0) wait(bKvFree, c - 1);
@@ -242,10 +277,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         __syncwarp();
       }
     }
-    if (gave_up(abort_flag)) {                               // copies in flight end (within microseconds) before the CTA's memory is given back
-      const long long t0 = clock64();
-      while (clock64() - t0 < (1LL << 22)) {}
-    }
+    let_copies_end(wait.dead);
   } else if (warp >= 4) {
     constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
     const int r = tid - 128, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
@@ -254,7 +286,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
     for (int j = 0; j < NC; ++j) X[j] = 0.f;
     const DecayStep full(ld, kL);
-    for (int c = 0; c < sp.nch && !gave_up(abort_flag); ++c) {
+    for (int c = 0; c < sp.nch && !wait.dead; ++c) {
       const int cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
       wait(bKv, c);
@@ -278,7 +310,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (c0 + col + j < u.Dc) *reinterpret_cast<float4*>(end + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
   } else {
     const float g2 = decay_log2(ld);
-    for (int c = 0; c < sp.nch && !gave_up(abort_flag); ++c) {
+    for (int c = 0; c < sp.nch && !wait.dead; ++c) {
       const int st = c % NST, cnt = sp.live(c);
       const float w = exp2f(g2 * (float)(sp.rev ? tid : max(0, cnt - 1 - tid)));
       wait(bFull + st, c / NST);
@@ -289,7 +321,6 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   }
   tc_fence_before();
   __syncthreads();
-  if (tid == 0 && status && gave_up(abort_flag)) atomicOr(status, kErrWaitTimeout);
   if (warp == 1) tmem_dealloc<128>(tmem);
 }
 
@@ -324,7 +355,6 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
            *bX = bars + 19, *bW = bars + 21, *bKv = bars + 23, *bYx = bars + 25, *bKvFree = bars + 26, *bY = bars + 27, *bYFree = bars + 28,
            *bIn = bars + 29;                                 // bIn: one a warp of the state
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
-  int* abort_flag = reinterpret_cast<int*>(bars + 34);
   float* sExp = reinterpret_cast<float*>(bars + 36);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 38);   // [2][4]
 
@@ -344,18 +374,18 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const int n_w = two ? 1 : 2;                     // buffers of the weighted C
   auto w_tile = [&](int i) { return L::oW + (two ? 0 : (i & 1) * kBlk); };
 
-  // a and b of a chunk land on one barrier, c on its own
-  auto load = [&](uint8_t* tiles, uint64_t* full, int which, int st, int blocks, int col, int i) {
-    for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + (st * blocks + k) * kBlk, &maps.in[which], full, col + 64 * k, sp.first(chunk(i)), h, b);
+  // a and b of a chunk land on one barrier, c on its own; `at` is the tile in its ring
+  auto load = [&](uint8_t* tiles, uint64_t* full, int which, int blocks, int col, int i) {
+    for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + k * kBlk, &maps.in[which], full, col + 64 * k, sp.first(chunk(i)), h, b);
   };
-  auto load_a = [&](int i) { load(smem + L::oA, bFull + i % L::kA, maps.ia[blockIdx.z], i % L::kA, CB, 0, i); };
-  auto load_b = [&](int i) {
-    mbar_expect_tx(bFull + i % L::kA, 2 * CB * kBlk);
-    load(smem + L::oB, bFull + i % L::kA, maps.ib[blockIdx.z], i % L::kB, CB, 0, i);
+  auto load_a = [&](int i, int at) { load(smem + L::oA + at * (CB * kBlk), bFull + at, maps.ia[blockIdx.z], CB, 0, i); };
+  auto load_b = [&](int i, int at, int at_a) {
+    mbar_expect_tx(bFull + at_a, 2 * CB * kBlk);
+    load(smem + L::oB + at * (CB * kBlk), bFull + at_a, maps.ib[blockIdx.z], CB, 0, i);
   };
-  auto load_c = [&](int i) {
-    mbar_expect_tx(bFullC + i % L::kC, kBlk);
-    load(smem + L::oC, bFullC + i % L::kC, maps.ic[blockIdx.z], i % L::kC, 1, c0, i);
+  auto load_c = [&](int i, int at) {
+    mbar_expect_tx(bFullC + at, kBlk);
+    load(smem + L::oC + at * kBlk, bFullC + at, maps.ic[blockIdx.z], 1, c0, i);
   };
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) {
@@ -367,12 +397,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     }
     mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bY, 2); mbar_init(bYFree, 256);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
-    *abort_flag = 0;
     fence_barrier_init();
     for (int i = 0; i < mine; ++i) {
-      if (i < L::kB) load_b(i);
-      if (i < L::kA) load_a(i);
-      if (i < L::kC) load_c(i);
+      if (i < L::kB) load_b(i, i, i);
+      if (i < L::kA) load_a(i, i);
+      if (i < L::kC) load_c(i, i);
       if (i >= 2) break;
     }
     if (size > 1 && mine > (rank == 0 ? 1 : 0))                           // the first state that comes from another CTA
@@ -383,22 +412,25 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   cluster_sync();                                  // every CTA's barriers stand before a state is sent
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto wait = [&](uint64_t* bar, int parity) { wait_on(bar, parity, abort_flag); };
+  Waits wait = {status};
 
   if (warp >= L::kWarpI) {
     // counts and addresses through a warp reduction: the compiler then keeps them, and the descriptors, in uniform registers
     const int n = __reduce_max_sync(0xffffffffu, mine);
     const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
     constexpr uint32_t id_s = idesc_f16(128, 128, F, F, 0, 0), id_y = idesc_f16(128, 64, F, F, 0, 1);
-    auto tile_a = [&](int i) { return smem_desc<128>(base + L::oA + i % L::kA * (CB * kBlk)); };
+    auto tile_a = [&](int at) { return smem_desc<128>(base + L::oA + at * (CB * kBlk)); };
+    Ring<L::kA> ra;
+    Ring<L::kB> rb;
+    Ring<L::kC> rc;
     if (warp == L::kWarpI) {
       // ---- S = A B^T and P C -------------------------------------------------------------------------------------------
       auto product_s = [&](int i) {
-        wait(bFull + i % L::kA, i / L::kA);
+        wait(bFull + ra.at, ra.phase);
         if (sp.live(chunk(i)) < kL) wait(bW + (i & 1), i >> 1);        // rows behind the length are cleared first
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t dA = tile_a(i), dB = smem_desc<128>(base + L::oB + i % L::kB * (CB * kBlk));
+          const uint64_t dA = tile_a(ra.at), dB = smem_desc<128>(base + L::oB + rb.at * (CB * kBlk));
           const uint32_t d = tm + 128 * (i & 1);
 #pragma unroll
           for (int kk = 0; kk < DK / 16; ++kk) {
@@ -406,85 +438,93 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             mma_ss(d, dA + off, dB + off, id_s, kk > 0);
           }
           mma_commit(bS + (i & 1));
-          mma_commit(bFreeA + i % L::kA);
-          mma_commit(bFreeB + i % L::kB);
+          mma_commit(bFreeA + ra.at);
+          mma_commit(bFreeB + rb.at);
         }
         __syncwarp();
+        ra.next();
+        rb.next();
       };
       if (n > 0) product_s(0);
-      for (int i = 0; i < n && !gave_up(abort_flag); ++i) {
+      for (int i = 0; i < n && !wait.dead; ++i) {
         if (L::kB > 1 && i + 1 < n) product_s(i + 1);
         wait(bP + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t dC = smem_desc<128>(base + L::oC + i % L::kC * kBlk);
+          const uint64_t dC = smem_desc<128>(base + L::oC + rc.at * kBlk);
           const uint32_t p = tm + 128 * (i & 1);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
           mma_commit(bY);
-          mma_commit(bFreeC + i % L::kC);
+          mma_commit(bFreeC + rc.at);
         }
         __syncwarp();
+        rc.next();
         if (L::kB == 1 && i + 1 < n) product_s(i + 1);
       }
     } else if (warp == L::kWarpI + 1) {
       // ---- B^T C, a chunk ahead, and A X ---------------------------------------------------------------------------------
+      Ring<L::kA> rf;                              // of the operands' barriers, a chunk ahead of ra
       auto product_bc = [&](int i) {
-        wait(bFull + i % L::kA, i / L::kA);
+        wait(bFull + rf.at, rf.phase);
         wait(bW + (i & 1), i >> 1);
         if (i > 0) wait(bKvFree, i - 1);
         tc_fence_after();
         if (elect_one()) {
-          product_kv<DK, F>(tm + L::cKv, base + L::oB + i % L::kB * (CB * kBlk), base + w_tile(i), two);
+          product_kv<DK, F>(tm + L::cKv, base + L::oB + rb.at * (CB * kBlk), base + w_tile(i), two);
           mma_commit(bKv + (i & 1));
-          mma_commit(bFreeB + i % L::kB);
-          mma_commit(bFreeC + i % L::kC);          // c has been weighed
+          mma_commit(bFreeB + rb.at);
+          mma_commit(bFreeC + rc.at);              // c has been weighed
         }
         __syncwarp();
+        rf.next();
+        rb.next();
+        rc.next();
       };
       if (n > 0) product_bc(0);
-      for (int i = 0; i < n && !gave_up(abort_flag); ++i) {
+      for (int i = 0; i < n && !wait.dead; ++i) {
         if (i + 1 < n) product_bc(i + 1);
         wait(bX + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t dA = tile_a(i), dX = smem_desc<128>(base + L::oX);
+          const uint64_t dA = tile_a(ra.at), dX = smem_desc<128>(base + L::oX);
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int kk = 0; kk < DK / 16; ++kk)
               mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
           mma_commit(bYx);
-          mma_commit(bFreeA + i % L::kA);
+          mma_commit(bFreeA + ra.at);
           mma_commit(bY);
         }
         __syncwarp();
+        ra.next();
       }
     } else {
       // ---- loads: a tile is refilled when the two products that read it have completed -----------------------------------
-      for (int i = 0; i < n && !gave_up(abort_flag); ++i) {
+      for (int i = 0; i < n && !wait.dead; ++i) {
         if (i + L::kB < n) {
-          wait(bFreeB + i % L::kB, i / L::kB);
-          if (elect_one()) load_b(i + L::kB);
+          wait(bFreeB + rb.at, rb.phase);
+          if (elect_one()) load_b(i + L::kB, rb.at, (i + L::kB) % L::kA);
           __syncwarp();
+          rb.next();
         }
         if (i + L::kA < n) {
-          wait(bFreeA + i % L::kA, i / L::kA);
-          if (elect_one()) load_a(i + L::kA);
+          wait(bFreeA + ra.at, ra.phase);
+          if (elect_one()) load_a(i + L::kA, ra.at);
           __syncwarp();
+          ra.next();
         }
         if (i + L::kC < n) {
-          wait(bFreeC + i % L::kC, i / L::kC);
-          if (elect_one()) load_c(i + L::kC);
+          wait(bFreeC + rc.at, rc.phase);
+          if (elect_one()) load_c(i + L::kC, rc.at);
           __syncwarp();
+          rc.next();
         }
       }
-      if (gave_up(abort_flag)) {                             // copies in flight end (within microseconds) before the CTA's memory is given back
-        const long long t0 = clock64();
-        while (clock64() - t0 < (1LL << 22)) {}
-      }
+      let_copies_end(wait.dead);
     }
   } else if (warp >= L::kWarpX) {
     // ---- the state -----------------------------------------------------------------------------------------------------
@@ -551,7 +591,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     for (int i = 0; i < mine; ++i) {
       const int c = chunk(i), cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
-      wait(bKv + (i & 1), i >> 1);
+      wait_together<4, 128>(wait, w == 0, bKv + (i & 1), i >> 1);
       tc_fence_after();
       if constexpr (DK == 64) {
         // all of a thread's 32 columns in registers: B^T C before the state arrives, then the state behind the chunk, which the
@@ -589,11 +629,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           for (int q = 0; q < 8; ++q) top = max(top, magnitude(x[q]));
           down = scale_down(top, i);
         }
-        if (i > 0) wait(bYx, i - 1);               // the product with the packed state of the chunk before is done
+        if (i > 0) wait_together<4, 128>(wait, w == 0, bYx, i - 1);    // the product with the packed state of the chunk before is done
 #pragma unroll
         for (int q = 0; q < 8; q += 2) pack(x[q], x[q + 1], down, 4 * q);
       } else {
-        if (i > 0) wait(bYx, i - 1);
+        if (i > 0) wait_together<4, 128>(wait, w == 0, bYx, i - 1);
         receive(i, c);
         float down = 1.f;
         if constexpr (kHalfRange) {
@@ -635,15 +675,25 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   } else if (warp >= L::kWarpC) {
     // ---- weighted C ----------------------------------------------------------------------------------------------------
     const int r = tid - 32 * L::kWarpC;
-    for (int i = 0; i < mine && !gave_up(abort_flag); ++i) {
+    Ring<L::kA> ra;
+    Ring<L::kB> rb;
+    Ring<L::kC> rc;
+    const float w_full = exp2f(g2 * (float)(rev ? r : kL - 1 - r));
+    for (int i = 0; i < mine; ++i) {
       const int cnt = sp.live(chunk(i));
-      const float w = exp2f(g2 * (float)(rev ? r : max(0, cnt - 1 - r)));
-      wait(bFullC + i % L::kC, i / L::kC);
-      if (cnt < kL) wait(bFull + i % L::kA, i / L::kA);
-      if (i >= n_w) wait(bKv + ((i - n_w) & 1), (i - n_w) >> 1);       // the product with what stood here is done
+      const float w = rev || cnt == kL ? w_full : exp2f(g2 * (float)max(0, cnt - 1 - r));
+      if (warp == L::kWarpC) {
+        wait(bFullC + rc.at, rc.phase);
+        if (cnt < kL) wait(bFull + ra.at, ra.phase);
+        if (i >= n_w) wait(bKv + ((i - n_w) & 1), (i - n_w) >> 1);     // the product with what stood here is done
+      }
+      asm volatile("bar.sync 3, 128;" ::: "memory");
       uint8_t* hi = smem + w_tile(i);
-      weigh_c<T, CB>(r, cnt, w, two, smem + L::oC + i % L::kC * kBlk, hi, hi + kBlk, smem + L::oB + i % L::kB * (CB * kBlk));
+      weigh_c<T, CB>(r, cnt, w, two, smem + L::oC + rc.at * kBlk, hi, hi + kBlk, smem + L::oB + rb.at * (CB * kBlk));
       arrive_on(bW + (i & 1));
+      ra.next();
+      rb.next();
+      rc.next();
     }
   } else {
     // ---- weights of P, outputs -----------------------------------------------------------------------------------------
@@ -664,7 +714,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     auto weigh = [&](int i) {
       const int cnt = sp.live(chunk(i));
       const uint32_t s = lane_base + 128 * (i & 1) + 64 * hb;
-      wait(bS + (i & 1), i >> 1);
+      wait_together<2, 256>(wait, warp == 0, bS + (i & 1), i >> 1);
       tc_fence_after();
 #pragma unroll 1
       for (int k = 0; k < 4; ++k) {
@@ -722,7 +772,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
         __syncwarp();
       }
-      wait(bY, i);
+      wait_together<2, 256>(wait, warp == 0, bY, i);
       tc_fence_after();
       float fx = wx;
       if constexpr (kHalfRange) fx *= sExp[i & 3];
@@ -741,7 +791,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           q[m] = Op16<T>::pack(t.x, t.y);
         }
         uint4 o = make_uint4(q[0], q[1], q[2], q[3]);
-        if (r >= cnt) o = make_uint4(0u, 0u, 0u, 0u);        // rows behind the sequence: zeros
+        if (cnt < kL && r >= cnt) o = make_uint4(0u, 0u, 0u, 0u);      // rows behind the sequence: zeros
         if constexpr (L::kStage) *reinterpret_cast<uint4*>(tile + swz_off<64>(lane, k)) = o;
         else if (tok0 + r < a.N && 8 * k < cols) *reinterpret_cast<uint4*>(out + (long long)(tok0 + r) * u.os[2] + 8 * k) = o;
       }
@@ -774,7 +824,6 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   }
   tc_fence_before();
   cluster_sync();                                  // no CTA leaves while another may still write into it
-  if (tid == 0 && status && gave_up(abort_flag)) atomicOr(status, kErrWaitTimeout);
   if (warp == 1) tmem_dealloc<512>(tmem);
 }
 
