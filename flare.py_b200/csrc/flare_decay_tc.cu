@@ -1,7 +1,7 @@
 // Decayed linear attention on the tensor cores: 16-bit operands, up to 128 features in a and b, any number in c (in blocks of
 // 64 columns).  A sequence (one unit, b, h, column block) is taken in chunks of 128 tokens:
 //
-//   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 256 threads weigh, mask and pack it there
+//   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 128 threads weigh, mask and pack it there
 //   out = scale * (P C + lambda^(i+1) A X)          X: the state before the chunk, in two 16-bit terms; two accumulators
 //   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms where the state is a result, in one
 //                                                   where only outputs are, which round as much themselves; X itself in fp32
@@ -13,7 +13,7 @@
 // to chunk is one multiply-add of the state and its way to the next SM.  Where even clusters of eight leave SMs idle, the token axis is
 // cut into segments as well: k_decay_tc_sums adds up each, k_decay_prefix makes the states before them.
 //
-// Warps of the walk: 0-7 weights of P and the outputs, 8-11 weighted C, 12-15 the state, 16 and 17 products, 18 loads.  Everything
+// Warps of the walk: 0-3 weights of P, 4-7 outputs, 8-11 weighted C, 12-15 the state, 16 and 17 products, 18 loads.  Everything
 // that the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are cleared in shared memory
 // before a product reads them, so that padding may hold NaN.
 //
@@ -34,7 +34,7 @@ constexpr int kL = 128;                            // tokens of a chunk
 constexpr int kBlk = 128 * 128;                    // bytes of a [128 rows][64] tile
 
 struct DecayMaps {
-  CUtensorMap in[4], out[kDecayUnits];             // boxes of [128 tokens][64 features], of the outputs [32][32]
+  CUtensorMap in[4], out[kDecayUnits];             // boxes of [128 tokens][64 features], of the outputs [32][64]
   int ia[kDecayUnits], ib[kDecayUnits], ic[kDecayUnits];
 };
 
@@ -163,11 +163,12 @@ struct Span {
 // and in the tiles of b and c themselves.
 template <typename T, int CB>
 __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8_t* src, uint8_t* hi_t, uint8_t* lo_t, uint8_t* b_t) {
+  const uint32_t row = 128 * r + 16 * (r & 7);     // 16-byte piece ch of the swizzled row: row ^ 16 ch
   if (r >= cnt) {
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
     for (int ch = 0; ch < 8; ++ch) {
-      const uint32_t at = 128 * r + 16 * ch;
+      const uint32_t at = row ^ (16 * ch);
       *reinterpret_cast<uint4*>(src + at) = z;
       *reinterpret_cast<uint4*>(hi_t + at) = z;
       if (two) *reinterpret_cast<uint4*>(lo_t + at) = z;
@@ -175,9 +176,9 @@ __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8
       for (int i = 0; i < CB; ++i) *reinterpret_cast<uint4*>(b_t + i * kBlk + at) = z;
     }
   } else if (two) {
-#pragma unroll 2
+#pragma unroll 4
     for (int ch = 0; ch < 8; ++ch) {
-      const uint32_t at = swz_off<128>(r, ch);
+      const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       uint4 hi, lo;
       split2<T>(mul2(Op16<T>::unpack(x.x), both(w)), hi.x, lo.x);
@@ -192,9 +193,9 @@ __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8
       const float2 f = mul2(Op16<T>::unpack(x), both(w));
       return Op16<T>::pack(f.x, f.y);
     };
-#pragma unroll 4
+#pragma unroll
     for (int ch = 0; ch < 8; ++ch) {
-      const uint32_t at = swz_off<128>(r, ch);
+      const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       *reinterpret_cast<uint4*>(hi_t + at) = make_uint4(weighed(x.x), weighed(x.y), weighed(x.z), weighed(x.w));
     }
@@ -228,7 +229,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   using L = SumPlan<DK>;
   constexpr int F = Op16<T>::kFmt, NST = L::kStages, CB = L::kCB;
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);   // by an offset: the compiler keeps to shared-memory instructions
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
   uint64_t *bFull = bars, *bW = bars + 2, *bKv = bars + 3, *bKvFree = bars + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 5);
@@ -337,7 +338,7 @@ template <int DK> struct WalkPlan {
   static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + kW * kBlk,
                        oIn = oX + 2 * kXTile, oOut = oIn + kXBytes, oBars = oOut + (kStage ? kBlk : 0);
   static constexpr int kBytes = oBars + 512 + 1024;
-  static constexpr int kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 3);
+  static constexpr int kWarpY = 4, kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 3);
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
 };
 
@@ -349,11 +350,12 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   constexpr int F = Op16<T>::kFmt, CB = L::kCB;
   constexpr bool kHalfRange = F == 0;              // fp16: the packed state is scaled by a power of two, the scale is applied last
   extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);   // by an offset: the compiler keeps to shared-memory instructions
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
-  uint64_t *bFull = bars, *bFullC = bars + 3, *bFreeA = bars + 6, *bFreeB = bars + 9, *bFreeC = bars + 12, *bS = bars + 15, *bP = bars + 17,
-           *bX = bars + 19, *bW = bars + 21, *bKv = bars + 23, *bYx = bars + 25, *bKvFree = bars + 26, *bY = bars + 27, *bYFree = bars + 28,
-           *bIn = bars + 29;                                 // bIn: one a warp of the state
+  // bFree: a chunk's outputs are complete, and with them everything that read its tiles.  bFreeB: a single tile of b is free
+  // earlier.  bIn: one a warp of the state.
+  uint64_t *bFull = bars, *bFullC = bars + 3, *bFree = bars + 6, *bFreeB = bars + 9, *bS = bars + 10, *bP = bars + 12, *bX = bars + 14, *bW = bars + 16,
+           *bKv = bars + 18, *bYx = bars + 20, *bKvFree = bars + 21, *bYFree = bars + 22, *bIn = bars + 29;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
   float* sExp = reinterpret_cast<float*>(bars + 36);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 38);   // [2][4]
@@ -388,14 +390,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     load(smem + L::oC + at * kBlk, bFullC + at, maps.ic[blockIdx.z], 1, c0, i);
   };
   if (tid == 0) {
-    for (int i = 0; i < 3; ++i) {
-      mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1);
-      mbar_init(bFreeA + i, 2); mbar_init(bFreeB + i, 2); mbar_init(bFreeC + i, 2);       // two products each
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1);
-    }
-    mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bY, 2); mbar_init(bYFree, 256);
+    for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFree + i, 2); }     // bFree: A X and P C
+    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 128); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1); }
+    mbar_init(bFreeB, 2); mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bYFree, 128);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     fence_barrier_init();
     for (int i = 0; i < mine; ++i) {
@@ -438,8 +435,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             mma_ss(d, dA + off, dB + off, id_s, kk > 0);
           }
           mma_commit(bS + (i & 1));
-          mma_commit(bFreeA + ra.at);
-          mma_commit(bFreeB + rb.at);
+          if (L::kB == 1) mma_commit(bFreeB);
         }
         __syncwarp();
         ra.next();
@@ -455,9 +451,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           const uint64_t dC = smem_desc<128>(base + L::oC + rc.at * kBlk);
           const uint32_t p = tm + 128 * (i & 1);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
-          mma_commit(bY);
-          mma_commit(bFreeC + rc.at);
+          for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * kk, dC + 128 * kk, id_y, kk > 0);
+          mma_commit(bFree + rc.at);
         }
         __syncwarp();
         rc.next();
@@ -474,13 +469,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (elect_one()) {
           product_kv<DK, F>(tm + L::cKv, base + L::oB + rb.at * (CB * kBlk), base + w_tile(i), two);
           mma_commit(bKv + (i & 1));
-          mma_commit(bFreeB + rb.at);
-          mma_commit(bFreeC + rc.at);              // c has been weighed
+          if (L::kB == 1) mma_commit(bFreeB);
         }
         __syncwarp();
         rf.next();
         rb.next();
-        rc.next();
       };
       if (n > 0) product_bc(0);
       for (int i = 0; i < n && !wait.dead; ++i) {
@@ -496,32 +489,29 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             for (int kk = 0; kk < DK / 16; ++kk)
               mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
           mma_commit(bYx);
-          mma_commit(bFreeA + ra.at);
-          mma_commit(bY);
+          mma_commit(bFree + ra.at);
         }
         __syncwarp();
         ra.next();
       }
     } else {
-      // ---- loads: a tile is refilled when the two products that read it have completed -----------------------------------
+      // ---- loads: tiles are refilled when the chunk's products have completed ---------------------------------------------
+      static_assert(L::kA == L::kC, "one ring");
       for (int i = 0; i < n && !wait.dead; ++i) {
-        if (i + L::kB < n) {
-          wait(bFreeB + rb.at, rb.phase);
-          if (elect_one()) load_b(i + L::kB, rb.at, (i + L::kB) % L::kA);
+        if (L::kB == 1 && i + 1 < n) {
+          wait(bFreeB, i);
+          if (elect_one()) load_b(i + 1, 0, (i + 1) % L::kA);
           __syncwarp();
-          rb.next();
         }
         if (i + L::kA < n) {
-          wait(bFreeA + ra.at, ra.phase);
-          if (elect_one()) load_a(i + L::kA, ra.at);
+          wait(bFree + ra.at, ra.phase);
+          if (elect_one()) {
+            if (L::kB > 1) load_b(i + L::kA, ra.at, ra.at);
+            load_a(i + L::kA, ra.at);
+            load_c(i + L::kA, ra.at);
+          }
           __syncwarp();
           ra.next();
-        }
-        if (i + L::kC < n) {
-          wait(bFreeC + rc.at, rc.phase);
-          if (elect_one()) load_c(i + L::kC, rc.at);
-          __syncwarp();
-          rc.next();
         }
       }
       let_copies_end(wait.dead);
@@ -545,15 +535,22 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     }
     const DecayStep full(ld, kL);
     // eight columns of the state before the chunk, packed for the product
+    uint8_t* packed = smem + L::oX;
+    const uint32_t row = 128 * d + 16 * ((col / 8) ^ (d & 7));         // of the swizzled tile; its piece of columns j: row ^ 2 j
     auto pack = [&](const float4& x0, const float4& x1, float down, int j) {
       uint4 h, l;
-      split2<T>(mul2(make_float2(x0.x, x0.y), both(down)), h.x, l.x);
-      split2<T>(mul2(make_float2(x0.z, x0.w), both(down)), h.y, l.y);
-      split2<T>(mul2(make_float2(x1.x, x1.y), both(down)), h.z, l.z);
-      split2<T>(mul2(make_float2(x1.z, x1.w), both(down)), h.w, l.w);
-      const uint32_t at = L::oX + swz_off<128>(d, (col + j) / 8);
-      *reinterpret_cast<uint4*>(smem + at) = h;
-      *reinterpret_cast<uint4*>(smem + L::kXTile + at) = l;
+      auto term = [&](float a0, float a1, uint32_t& hi, uint32_t& lo) {
+        float2 x = make_float2(a0, a1);
+        if constexpr (kHalfRange) x = mul2(x, both(down));
+        split2<T>(x, hi, lo);
+      };
+      term(x0.x, x0.y, h.x, l.x);
+      term(x0.z, x0.w, h.y, l.y);
+      term(x1.x, x1.y, h.z, l.z);
+      term(x1.z, x1.w, h.w, l.w);
+      const uint32_t at = row ^ (2 * j);
+      *reinterpret_cast<uint4*>(packed + at) = h;
+      *reinterpret_cast<uint4*>(packed + L::kXTile + at) = l;
     };
     auto stepped = [&](const float4& x, const DecayStep& decay, const float2& v0, const float2& v1) {
       const float2 m = both(decay.mul), k = both(decay.keep), a0 = make_float2(x.x, x.y), a1 = make_float2(x.z, x.w);
@@ -695,10 +692,84 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       rb.next();
       rc.next();
     }
+  } else if (warp >= L::kWarpY) {
+    // ---- outputs -------------------------------------------------------------------------------------------------------
+    const int w = warp & 3, r = 32 * w + lane;     // token
+    const uint32_t y_at = tmem + ((uint32_t)(32 * w) << 16) + L::cY, x_at = y_at + (L::cYx - L::cY);
+    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
+    T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0;
+    const int cols = u.Dc - c0;                    // of the 64 columns, those that exist
+    uint8_t* tile = smem + L::oOut + w * 4096;     // the warp's [32 rows][64], swizzled: piece k of a row at row ^ 16 k
+    const uint32_t row = 128 * lane + 16 * (lane & 7);
+    Ring<L::kA> ra;
+    for (int i = 0; i < mine; ++i) {
+      const int c = chunk(i), cnt = sp.live(c), tok0 = sp.first(c);
+      if constexpr (L::kStage) {                   // the tile of the chunk before has left shared memory
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        __syncwarp();
+      }
+      wait_together<5, 128>(wait, w == 0, bFree + ra.at, ra.phase);
+      ra.next();
+      tc_fence_after();
+      float fx = wx;
+      if constexpr (kHalfRange) fx *= sExp[i & 3];
+      uint32_t y[2][16], x[2][16];
+      tmem_ld16(y_at, y[0]);
+      tmem_ld16(x_at, x[0]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        tmem_wait_ld();
+        if (k < 3) {
+          tmem_ld16(y_at + 16 * (k + 1), y[(k + 1) & 1]);
+          tmem_ld16(x_at + 16 * (k + 1), x[(k + 1) & 1]);
+        }
+        uint32_t q[8];
+#pragma unroll
+        for (int m = 0; m < 8; ++m) {
+          float2 in_chunk = floats(y[k & 1][2 * m], y[k & 1][2 * m + 1]);
+          if constexpr (kHalfRange) in_chunk = mul2(both(a.scale), in_chunk);
+          const float2 t = fma2(both(fx), floats(x[k & 1][2 * m], x[k & 1][2 * m + 1]), in_chunk);
+          q[m] = Op16<T>::pack(t.x, t.y);
+        }
+        if (k == 3) {
+          tc_fence_before();
+          arrive_on(bYFree);
+        }
+        if (cnt < kL && r >= cnt)                  // rows behind the sequence: zeros
+#pragma unroll
+          for (int m = 0; m < 8; ++m) q[m] = 0u;
+        const uint4 o0 = make_uint4(q[0], q[1], q[2], q[3]), o1 = make_uint4(q[4], q[5], q[6], q[7]);
+        if constexpr (L::kStage) {
+          *reinterpret_cast<uint4*>(tile + (row ^ (32 * k))) = o0;
+          *reinterpret_cast<uint4*>(tile + (row ^ (32 * k + 16))) = o1;
+        } else if (tok0 + r < a.N) {
+          T* p = out + (long long)(tok0 + r) * u.os[2] + 16 * k;
+          if (16 * k < cols) *reinterpret_cast<uint4*>(p) = o0;
+          if (16 * k + 8 < cols) *reinterpret_cast<uint4*>(p + 8) = o1;
+        }
+      }
+      if constexpr (L::kStage) {
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0 && tok0 + 32 * w < a.N) tma_store_4d(&maps.out[blockIdx.z], tile, c0, tok0 + 32 * w, h, b);      // clipped at N and the last column
+      }
+    }
+    // chunks of the segment that no live token is in: zeros
+    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
+    for (int tok = sp.n0 + kL * (sp.nch + rank) + r; tok < min(a.N, sp.n0 + a.seg_len);
+         tok = sp.n0 + (tok - sp.n0) / kL * kL + kL * size + r) {
+      T* p = out + (long long)tok * u.os[2];
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (8 * k < cols) *reinterpret_cast<uint4*>(p + 8 * k) = z;
+    }
+    if constexpr (L::kStage)
+      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   } else {
-    // ---- weights of P, outputs -----------------------------------------------------------------------------------------
-    const int r0 = 32 * (warp & 3), r = r0 + lane, hb = warp >> 2;    // token r, half of the columns
+    // ---- weights of P --------------------------------------------------------------------------------------------------
+    const int r0 = 32 * warp, r = r0 + lane;       // token
     const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
+    const float scale_p = kHalfRange ? 1.f : a.scale;
     // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
     // diagonal the latter exceeds 1, up to lambda^-15, which is in range for every decay above 2^-8 a token; the others take an
     // exponential each there.
@@ -707,28 +778,27 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       wcol[k] = make_float2(exp2f(g2 * (float)(rev ? 2 * k : 15 - 2 * k)), exp2f(g2 * (float)(rev ? 2 * k + 1 : 14 - 2 * k)));
-    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1)), scale_p = kHalfRange ? 1.f : a.scale;
-    T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0 + 32 * hb;
-    const int cols = u.Dc - c0 - 32 * hb;          // of this thread's 32 columns, those that exist
-
-    auto weigh = [&](int i) {
+    for (int i = 0; i < mine; ++i) {
       const int cnt = sp.live(chunk(i));
-      const uint32_t s = lane_base + 128 * (i & 1) + 64 * hb;
-      wait_together<2, 256>(wait, warp == 0, bS + (i & 1), i >> 1);
+      const uint32_t s = lane_base + 128 * (i & 1);
+      wait_together<2, 128>(wait, warp == 0, bS + (i & 1), i >> 1);
       tc_fence_after();
+      uint32_t next[16];
+      tmem_ld16(s, next);
 #pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
-        const int j0 = 64 * hb + 16 * k;           // the block's first column; the warp's rows are r0 ... r0 + 31
+      for (int k = 0; k < 8; ++k) {
+        const int j0 = 16 * k;                     // the block's first column; the warp's rows are r0 ... r0 + 31
         const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = (rev ? j0 >= r0 + 31 : j0 + 15 <= r0) && cnt == kL;
-        uint32_t p[8];
+        uint32_t v[16], p[8];
+        tmem_wait_ld();
+#pragma unroll
+        for (int m = 0; m < 16; ++m) v[m] = next[m];
+        if (k < 7) tmem_ld16(s + j0 + 16, next);   // the next block's columns are on their way
         if (none) {
 #pragma unroll
           for (int m = 0; m < 8; ++m) p[m] = 0u;
         } else {
-          uint32_t v[16];
-          tmem_ld16(s + 16 * k, v);
           const float row = scale_p * exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15));
-          tmem_wait_ld();
           const int d = rev ? j0 - r : r - j0, sign = rev ? 1 : -1;    // i - j of the first column, and its change
           if (all) {
 #pragma unroll
@@ -737,11 +807,22 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
               p[m] = Op16<T>::pack(x.x, x.y);
             }
           } else if (mild && cnt == kL) {
+            const int t = r - j0;                  // columns up to t, or from t on
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
               const float2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), both(row));
-              p[m] = Op16<T>::pack(d + sign * (2 * m) >= 0 ? x.x : 0.f, d + sign * (2 * m + 1) >= 0 ? x.y : 0.f);
+              v[2 * m] = __float_as_uint(x.x);
+              v[2 * m + 1] = __float_as_uint(x.y);
             }
+            if (rev) {
+#pragma unroll
+              for (int m = 0; m < 16; ++m) v[m] = m >= t ? v[m] : 0u;
+            } else {
+#pragma unroll
+              for (int m = 0; m < 16; ++m) v[m] = m <= t ? v[m] : 0u;
+            }
+#pragma unroll
+            for (int m = 0; m < 8; ++m) p[m] = Op16<T>::pack(__uint_as_float(v[2 * m]), __uint_as_float(v[2 * m + 1]));
           } else {
 #pragma unroll 1
             for (int m = 0; m < 8; ++m) {
@@ -759,68 +840,12 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             }
           }
         }
-        tmem_st8(s + 8 * k, p);                    // over columns of this thread that are read already
+        tmem_st8(s + 8 * k, p);                    // over columns that are read already
       }
       tmem_wait_st();
       tc_fence_before();
       arrive_on(bP + (i & 1));
-    };
-    auto finish = [&](int i) {
-      const int c = chunk(i), cnt = sp.live(c), tok0 = sp.first(c);
-      uint8_t* tile = smem + L::oOut + warp * 2048;          // the warp's own [32 rows][32]
-      if constexpr (L::kStage) {                   // that of the chunk before has left shared memory
-        if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        __syncwarp();
-      }
-      wait_together<2, 256>(wait, warp == 0, bY, i);
-      tc_fence_after();
-      float fx = wx;
-      if constexpr (kHalfRange) fx *= sExp[i & 3];
-#pragma unroll 2
-      for (int k = 0; k < 4; ++k) {
-        uint32_t y[8], x[8];
-        tmem_ld8(lane_base + L::cY + 32 * hb + 8 * k, y);
-        tmem_ld8(lane_base + L::cYx + 32 * hb + 8 * k, x);
-        tmem_wait_ld();
-        uint32_t q[4];
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          float2 in_chunk = floats(y[2 * m], y[2 * m + 1]);
-          if constexpr (kHalfRange) in_chunk = mul2(both(a.scale), in_chunk);
-          const float2 t = fma2(both(fx), floats(x[2 * m], x[2 * m + 1]), in_chunk);
-          q[m] = Op16<T>::pack(t.x, t.y);
-        }
-        uint4 o = make_uint4(q[0], q[1], q[2], q[3]);
-        if (cnt < kL && r >= cnt) o = make_uint4(0u, 0u, 0u, 0u);      // rows behind the sequence: zeros
-        if constexpr (L::kStage) *reinterpret_cast<uint4*>(tile + swz_off<64>(lane, k)) = o;
-        else if (tok0 + r < a.N && 8 * k < cols) *reinterpret_cast<uint4*>(out + (long long)(tok0 + r) * u.os[2] + 8 * k) = o;
-      }
-      tc_fence_before();
-      arrive_on(bYFree);
-      if constexpr (L::kStage) {
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0 && tok0 + r0 < a.N && cols > 0)        // clipped at N and at the last column
-          tma_store_4d(&maps.out[blockIdx.z], tile, c0 + 32 * hb, tok0 + r0, h, b);
-      }
-    };
-    // With two chunks of a and b in flight the next weights come before this chunk's outputs, else behind them.
-    constexpr int kAhead = L::kB > 1 ? 1 : 0;
-    for (int i = 0; i < mine + kAhead; ++i) {
-      if (i < mine) weigh(i);
-      if (i >= kAhead) finish(i - kAhead);
     }
-    // chunks of the segment that no live token is in: zeros
-    const uint4 z = make_uint4(0u, 0u, 0u, 0u);
-    for (int tok = sp.n0 + kL * (sp.nch + rank) + (tid & 127); tok < min(a.N, sp.n0 + a.seg_len);
-         tok = sp.n0 + (tok - sp.n0) / kL * kL + kL * size + (tid & 127)) {
-      T* p = out + (long long)tok * u.os[2];
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (8 * k < cols) *reinterpret_cast<uint4*>(p + 8 * k) = z;
-    }
-    if constexpr (L::kStage)
-      if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before();
   cluster_sync();                                  // no CTA leaves while another may still write into it
@@ -917,7 +942,7 @@ int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
     const DecayUnit& u = a.u[i];
     Da = u.Da > Da ? u.Da : Da;
     Dc = u.Dc > Dc ? u.Dc : Dc;
-    if (!make(&maps.out[i], u.out, u.os, u.Dc, 32, 32)) return FLARE_EUNSUPPORTED;
+    if (!make(&maps.out[i], u.out, u.os, u.Dc, 64, 32)) return FLARE_EUNSUPPORTED;
   }
   // the operands in the order dy v k | (v dy) q | (k q dy): each tensor's map is made once
   const int order[3][3] = {{0, 1, 2}, {1, 0, 3}, {2, 3, 0}};
