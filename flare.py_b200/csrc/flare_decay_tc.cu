@@ -1,7 +1,7 @@
 // Decayed linear attention on the tensor cores: 16-bit operands, up to 128 features in a and b, any number in c (in blocks of
 // 64 columns).  A sequence (one unit, b, h, column block) is taken in chunks of 128 tokens:
 //
-//   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 128 threads weigh, mask and pack it there
+//   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 256 threads weigh, mask and pack it there
 //   out = scale * (P C + lambda^(i+1) A X)          X: the state before the chunk, in two 16-bit terms; two accumulators
 //   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms where the state is a result, in one
 //                                                   where only outputs are, which round as much themselves; X itself in fp32
@@ -13,7 +13,7 @@
 // to chunk is one multiply-add of the state and its way to the next SM.  Where even clusters of eight leave SMs idle, the token axis is
 // cut into segments as well: k_decay_tc_sums adds up each, k_decay_prefix makes the states before them.
 //
-// Warps of the walk: 0-3 weights of P, 4-7 outputs, 8-11 weighted C, 12-15 the state, 16 and 17 products, 18 loads.  Everything
+// Warps of the walk: 0-7 weights of P, 8-11 weighted C, 12-15 the state, 16-19 outputs, 20 and 21 products, 22 loads.  Everything
 // that the mask or `lengths` hides is selected away, not multiplied by zero, and rows behind the length are cleared in shared memory
 // before a product reads them, so that padding may hold NaN.
 //
@@ -71,7 +71,8 @@ struct Waits {
     if (status) atomicOr(status, kErrWaitTimeout);
   }
 };
-// The wait of a role of several warps: one of them polls, the others sleep at a named barrier.
+// The wait of a role of several warps: one of them polls, the others sleep at a named barrier.  The polling warps are spread over
+// the four schedulers, which the warps' numbers modulo four stand for.
 template <int ID, int THREADS>
 __device__ __forceinline__ void wait_together(Waits& wait, bool leader, uint64_t* bar, int parity) {
   if (leader) wait(bar, parity);
@@ -119,31 +120,52 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// two values an instruction
-__device__ __forceinline__ uint64_t& as_u64(float2& x) { return reinterpret_cast<uint64_t&>(x); }
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(as_u64(r)) : "l"(as_u64(a)), "l"(as_u64(b)));
+// Two values an instruction.  A pair lives in one 64-bit register from where it is made, so that none is put together twice.
+struct F2 {
+  uint64_t v;
+  __device__ __forceinline__ F2() {}
+  __device__ __forceinline__ F2(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+  __device__ __forceinline__ float2 get() const {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+  }
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-  float2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(as_u64(r)) : "l"(as_u64(a)), "l"(as_u64(b)));
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(as_u64(r)) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
   return r;
 }
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-__device__ __forceinline__ float2 floats(uint32_t a, uint32_t b) { return make_float2(__uint_as_float(a), __uint_as_float(b)); }
+__device__ __forceinline__ F2 floats(uint32_t a, uint32_t b) { return F2(__uint_as_float(a), __uint_as_float(b)); }
+// one value twice; volatile, so that it is made where it stands and not again at every use
+__device__ __forceinline__ F2 both(float x) {
+  F2 r;
+  asm volatile("mov.b64 %0, {%1, %1};" : "=l"(r.v) : "f"(x));
+  return r;
+}
+template <typename T> __device__ __forceinline__ F2 unpack2(uint32_t w) {
+  const float2 f = Op16<T>::unpack(w);
+  return F2(f.x, f.y);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(F2 x) {
+  const float2 f = x.get();
+  return Op16<T>::pack(f.x, f.y);
+}
 // the hi and lo terms of a pair: lo is what rounding to 16 bits left of each
 template <typename T>
-__device__ __forceinline__ void split2(float2 x, uint32_t& hi, uint32_t& lo) {
-  hi = Op16<T>::pack(x.x, x.y);
-  const float2 r = fma2(Op16<T>::unpack(hi), both(-1.f), x);
-  lo = Op16<T>::pack(r.x, r.y);
+__device__ __forceinline__ void split2(F2 x, F2 minus_one, uint32_t& hi, uint32_t& lo) {
+  hi = pack2<T>(x);
+  lo = pack2<T>(fma2(unpack2<T>(hi), minus_one, x));
 }
 
 // What a chunk is to the CTA that takes it.
@@ -164,6 +186,7 @@ struct Span {
 template <typename T, int CB>
 __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8_t* src, uint8_t* hi_t, uint8_t* lo_t, uint8_t* b_t) {
   const uint32_t row = 128 * r + 16 * (r & 7);     // 16-byte piece ch of the swizzled row: row ^ 16 ch
+  const F2 w2 = both(w);
   if (r >= cnt) {
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
@@ -176,23 +199,21 @@ __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8
       for (int i = 0; i < CB; ++i) *reinterpret_cast<uint4*>(b_t + i * kBlk + at) = z;
     }
   } else if (two) {
+    const F2 minus_one = both(-1.f);
 #pragma unroll 4
     for (int ch = 0; ch < 8; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       uint4 hi, lo;
-      split2<T>(mul2(Op16<T>::unpack(x.x), both(w)), hi.x, lo.x);
-      split2<T>(mul2(Op16<T>::unpack(x.y), both(w)), hi.y, lo.y);
-      split2<T>(mul2(Op16<T>::unpack(x.z), both(w)), hi.z, lo.z);
-      split2<T>(mul2(Op16<T>::unpack(x.w), both(w)), hi.w, lo.w);
+      split2<T>(mul2(unpack2<T>(x.x), w2), minus_one, hi.x, lo.x);
+      split2<T>(mul2(unpack2<T>(x.y), w2), minus_one, hi.y, lo.y);
+      split2<T>(mul2(unpack2<T>(x.z), w2), minus_one, hi.z, lo.z);
+      split2<T>(mul2(unpack2<T>(x.w), w2), minus_one, hi.w, lo.w);
       *reinterpret_cast<uint4*>(hi_t + at) = hi;
       *reinterpret_cast<uint4*>(lo_t + at) = lo;
     }
   } else {
-    auto weighed = [&](uint32_t x) {
-      const float2 f = mul2(Op16<T>::unpack(x), both(w));
-      return Op16<T>::pack(f.x, f.y);
-    };
+    auto weighed = [&](uint32_t x) { return pack2<T>(mul2(unpack2<T>(x), w2)); };
 #pragma unroll
     for (int ch = 0; ch < 8; ++ch) {
       const uint32_t at = row ^ (16 * ch);
@@ -338,7 +359,7 @@ template <int DK> struct WalkPlan {
   static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + kW * kBlk,
                        oIn = oX + 2 * kXTile, oOut = oIn + kXBytes, oBars = oOut + (kStage ? kBlk : 0);
   static constexpr int kBytes = oBars + 512 + 1024;
-  static constexpr int kWarpY = 4, kWarpC = 8, kWarpX = 12, kWarpI = 16, kThreads = 32 * (kWarpI + 3);
+  static constexpr int kWarpC = 8, kWarpX = 12, kWarpY = 16, kWarpI = 20, kThreads = 32 * (kWarpI + 3);
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
 };
 
@@ -391,7 +412,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   };
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFree + i, 2); }     // bFree: A X and P C
-    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 128); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1); }
     mbar_init(bFreeB, 2); mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bYFree, 128);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     fence_barrier_init();
@@ -451,7 +472,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           const uint64_t dC = smem_desc<128>(base + L::oC + rc.at * kBlk);
           const uint32_t p = tm + 128 * (i & 1);
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * kk, dC + 128 * kk, id_y, kk > 0);
+          for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
           mma_commit(bFree + rc.at);
         }
         __syncwarp();
@@ -516,187 +537,12 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       }
       let_copies_end(wait.dead);
     }
-  } else if (warp >= L::kWarpX) {
-    // ---- the state -----------------------------------------------------------------------------------------------------
-    // It lives in sIn: a thread's quads of columns q = 0, 1, ... stand at 512 q + 16 lane of its warp's quarter.  They are read,
-    // packed for this chunk's product, and replaced by the state behind the chunk, which is then copied to the CTA that takes
-    // the next one.  That CTA's copy further on cannot arrive here before this one has been read: each waits for the one before.
-    constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
-    const int r = tid - 32 * L::kWarpX, w = warp & 3, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
-    const uint32_t kv = tmem + ((uint32_t)(w * 32) << 16) + L::cKv + col;
-    uint8_t* in = smem + L::oIn + w * (L::kXBytes / 4) + 16 * lane;
-    const long long own = (long long)d * u.Dc + c0 + col;
-    const int cols = d < u.Da ? u.Dc - c0 - col : 0;         // of this thread's columns, those that exist
-    if (rank == 0) {
-      const float* before = a.n_seg > 1 ? u.seg + ((long long)bh * a.n_seg + seg) * u.Da * u.Dc : u.state_in ? u.state_in + (long long)bh * u.Da * u.Dc : nullptr;
-#pragma unroll 2
-      for (int j = 0; j < NC; j += 4)
-        *reinterpret_cast<float4*>(in + 128 * j) = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    const DecayStep full(ld, kL);
-    // eight columns of the state before the chunk, packed for the product
-    uint8_t* packed = smem + L::oX;
-    const uint32_t row = 128 * d + 16 * ((col / 8) ^ (d & 7));         // of the swizzled tile; its piece of columns j: row ^ 2 j
-    auto pack = [&](const float4& x0, const float4& x1, float down, int j) {
-      uint4 h, l;
-      auto term = [&](float a0, float a1, uint32_t& hi, uint32_t& lo) {
-        float2 x = make_float2(a0, a1);
-        if constexpr (kHalfRange) x = mul2(x, both(down));
-        split2<T>(x, hi, lo);
-      };
-      term(x0.x, x0.y, h.x, l.x);
-      term(x0.z, x0.w, h.y, l.y);
-      term(x1.x, x1.y, h.z, l.z);
-      term(x1.z, x1.w, h.w, l.w);
-      const uint32_t at = row ^ (2 * j);
-      *reinterpret_cast<uint4*>(packed + at) = h;
-      *reinterpret_cast<uint4*>(packed + L::kXTile + at) = l;
-    };
-    auto stepped = [&](const float4& x, const DecayStep& decay, const float2& v0, const float2& v1) {
-      const float2 m = both(decay.mul), k = both(decay.keep), a0 = make_float2(x.x, x.y), a1 = make_float2(x.z, x.w);
-      const float2 y0 = fma2(m, a0, fma2(k, a0, v0)), y1 = fma2(m, a1, fma2(k, a1, v1));
-      return make_float4(y0.x, y0.y, y1.x, y1.y);
-    };
-    // the largest magnitude of an fp16 tile to 2^13 ... 2^14: X may lie outside fp16's range
-    auto scale_down = [&](uint32_t top, int i) {
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) sMax[4 * (i & 1) + w] = top;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
-      top = max(max(all.x, all.y), max(all.z, all.w));
-      const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
-      if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
-      return __uint_as_float((uint32_t)(127 - e) << 23);
-    };
-    auto magnitude = [](const float4& x) {
-      return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
-    };
-    auto send = [&](int c) {                       // what this warp has written, to the CTA of the next chunk
-      if (size == 1 || c + 1 == sp.nch) return;
-      fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) {
-        const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
-        copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
-      }
-    };
-    auto receive = [&](int i, int c) {
-      if (size == 1 || c == 0) return;
-      wait(bIn + w, rank == 0 ? i - 1 : i);
-      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
-    };
-    for (int i = 0; i < mine; ++i) {
-      const int c = chunk(i), cnt = sp.live(c);
-      const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
-      wait_together<4, 128>(wait, w == 0, bKv + (i & 1), i >> 1);
-      tc_fence_after();
-      if constexpr (DK == 64) {
-        // all of a thread's 32 columns in registers: B^T C before the state arrives, then the state behind the chunk, which the
-        // next CTA waits for, and last the packing for this chunk's product
-        float2 v[16];
-#pragma unroll
-        for (int j = 0; j < 32; j += 16) {
-          uint32_t h[16];
-          tmem_ld16(kv + j, h);
-          if (two) {
-            uint32_t l[16];
-            tmem_ld16(kv + 64 + j, l);
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[j / 2 + k] = add2(floats(h[2 * k], h[2 * k + 1]), floats(l[2 * k], l[2 * k + 1]));
-          } else {
-            tmem_wait_ld();
-#pragma unroll
-            for (int k = 0; k < 8; ++k) v[j / 2 + k] = floats(h[2 * k], h[2 * k + 1]);
-          }
-        }
-        tc_fence_before();
-        arrive_on(bKvFree);
-        receive(i, c);
-        float4 x[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) x[q] = *reinterpret_cast<const float4*>(in + 512 * q);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) *reinterpret_cast<float4*>(in + 512 * q) = stepped(x[q], decay, v[2 * q], v[2 * q + 1]);
-        send(c);
-        float down = 1.f;
-        if constexpr (kHalfRange) {
-          uint32_t top = 0;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) top = max(top, magnitude(x[q]));
-          down = scale_down(top, i);
-        }
-        if (i > 0) wait_together<4, 128>(wait, w == 0, bYx, i - 1);    // the product with the packed state of the chunk before is done
-#pragma unroll
-        for (int q = 0; q < 8; q += 2) pack(x[q], x[q + 1], down, 4 * q);
-      } else {
-        if (i > 0) wait_together<4, 128>(wait, w == 0, bYx, i - 1);
-        receive(i, c);
-        float down = 1.f;
-        if constexpr (kHalfRange) {
-          uint32_t top = 0;
-#pragma unroll 2
-          for (int j = 0; j < NC; j += 4) top = max(top, magnitude(*reinterpret_cast<const float4*>(in + 128 * j)));
-          down = scale_down(top, i);
-        }
-#pragma unroll 2
-        for (int j = 0; j < NC; j += 8) {
-          uint32_t h[8], l[8];
-          tmem_ld8(kv + j, h);
-          if (two) {
-            tmem_ld8(kv + 64 + j, l);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) l[k] = 0u;
-          }
-          const float4 x0 = *reinterpret_cast<const float4*>(in + 128 * j), x1 = *reinterpret_cast<const float4*>(in + 128 * j + 512);
-          pack(x0, x1, down, j);
-          tmem_wait_ld();
-          auto v = [&](int k) { return add2(floats(h[k], h[k + 1]), floats(l[k], l[k + 1])); };
-          *reinterpret_cast<float4*>(in + 128 * j) = stepped(x0, decay, v(0), v(2));
-          *reinterpret_cast<float4*>(in + 128 * j + 512) = stepped(x1, decay, v(4), v(6));
-        }
-        send(c);
-        tc_fence_before();
-        arrive_on(bKvFree);
-      }
-      fence_proxy_async();
-      arrive_on(bX + (i & 1));
-    }
-    // behind the last chunk (or, without one, behind none: rank 0 then)
-    const int last = sp.nch > 0 ? (sp.nch - 1) % size : 0;
-    if (u.state_out && seg == a.n_seg - 1 && rank == last)
-#pragma unroll 2
-      for (int j = 0; j < NC; j += 4)
-        if (j < cols) *reinterpret_cast<float4*>(u.state_out + (long long)bh * u.Da * u.Dc + own + j) = *reinterpret_cast<const float4*>(in + 128 * j);
-  } else if (warp >= L::kWarpC) {
-    // ---- weighted C ----------------------------------------------------------------------------------------------------
-    const int r = tid - 32 * L::kWarpC;
-    Ring<L::kA> ra;
-    Ring<L::kB> rb;
-    Ring<L::kC> rc;
-    const float w_full = exp2f(g2 * (float)(rev ? r : kL - 1 - r));
-    for (int i = 0; i < mine; ++i) {
-      const int cnt = sp.live(chunk(i));
-      const float w = rev || cnt == kL ? w_full : exp2f(g2 * (float)max(0, cnt - 1 - r));
-      if (warp == L::kWarpC) {
-        wait(bFullC + rc.at, rc.phase);
-        if (cnt < kL) wait(bFull + ra.at, ra.phase);
-        if (i >= n_w) wait(bKv + ((i - n_w) & 1), (i - n_w) >> 1);     // the product with what stood here is done
-      }
-      asm volatile("bar.sync 3, 128;" ::: "memory");
-      uint8_t* hi = smem + w_tile(i);
-      weigh_c<T, CB>(r, cnt, w, two, smem + L::oC + rc.at * kBlk, hi, hi + kBlk, smem + L::oB + rb.at * (CB * kBlk));
-      arrive_on(bW + (i & 1));
-      ra.next();
-      rb.next();
-      rc.next();
-    }
   } else if (warp >= L::kWarpY) {
     // ---- outputs -------------------------------------------------------------------------------------------------------
     const int w = warp & 3, r = 32 * w + lane;     // token
     const uint32_t y_at = tmem + ((uint32_t)(32 * w) << 16) + L::cY, x_at = y_at + (L::cYx - L::cY);
     const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
+    const F2 scale2 = both(a.scale);
     T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0;
     const int cols = u.Dc - c0;                    // of the 64 columns, those that exist
     uint8_t* tile = smem + L::oOut + w * 4096;     // the warp's [32 rows][64], swizzled: piece k of a row at row ^ 16 k
@@ -711,8 +557,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       wait_together<5, 128>(wait, w == 0, bFree + ra.at, ra.phase);
       ra.next();
       tc_fence_after();
-      float fx = wx;
-      if constexpr (kHalfRange) fx *= sExp[i & 3];
+      const F2 fx = both(kHalfRange ? wx * sExp[i & 3] : wx);
       uint32_t y[2][16], x[2][16];
       tmem_ld16(y_at, y[0]);
       tmem_ld16(x_at, x[0]);
@@ -726,10 +571,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         uint32_t q[8];
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
-          float2 in_chunk = floats(y[k & 1][2 * m], y[k & 1][2 * m + 1]);
-          if constexpr (kHalfRange) in_chunk = mul2(both(a.scale), in_chunk);
-          const float2 t = fma2(both(fx), floats(x[k & 1][2 * m], x[k & 1][2 * m + 1]), in_chunk);
-          q[m] = Op16<T>::pack(t.x, t.y);
+          F2 in_chunk = floats(y[k & 1][2 * m], y[k & 1][2 * m + 1]);
+          if constexpr (kHalfRange) in_chunk = mul2(scale2, in_chunk);
+          q[m] = pack2<T>(fma2(fx, floats(x[k & 1][2 * m], x[k & 1][2 * m + 1]), in_chunk));
         }
         if (k == 3) {
           tc_fence_before();
@@ -765,52 +609,222 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     }
     if constexpr (L::kStage)
       if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  } else if (warp >= L::kWarpX) {
+    // ---- the state -----------------------------------------------------------------------------------------------------
+    // It lives in sIn: a thread's quads of columns q = 0, 1, ... stand at 512 q + 16 lane of its warp's quarter.  They are read,
+    // packed for this chunk's product, and replaced by the state behind the chunk, which is then copied to the CTA that takes
+    // the next one.  That CTA's copy further on cannot arrive here before this one has been read: each waits for the one before.
+    constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
+    const int r = tid - 32 * L::kWarpX, w = warp & 3, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
+    const uint32_t kv = tmem + ((uint32_t)(w * 32) << 16) + L::cKv + col;
+    uint8_t* in = smem + L::oIn + w * (L::kXBytes / 4) + 16 * lane;
+    const long long own = (long long)d * u.Dc + c0 + col;
+    const int cols = d < u.Da ? u.Dc - c0 - col : 0;         // of this thread's columns, those that exist
+    if (rank == 0) {
+      const float* before = a.n_seg > 1 ? u.seg + ((long long)bh * a.n_seg + seg) * u.Da * u.Dc : u.state_in ? u.state_in + (long long)bh * u.Da * u.Dc : nullptr;
+#pragma unroll 2
+      for (int j = 0; j < NC; j += 4)
+        *reinterpret_cast<float4*>(in + 128 * j) = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    const DecayStep full(ld, kL);
+    // eight columns of the state before the chunk, packed for the product
+    uint8_t* packed = smem + L::oX;
+    const F2 minus_one = both(-1.f);
+    const uint32_t row = 128 * d + 16 * ((col / 8) ^ (d & 7));         // of the swizzled tile; its piece of columns j: row ^ 2 j
+    auto pack = [&](const float4& x0, const float4& x1, float down, int j) {
+      uint4 h, l;
+      auto term = [&](float a0, float a1, uint32_t& hi, uint32_t& lo) {
+        split2<T>(kHalfRange ? F2(a0 * down, a1 * down) : F2(a0, a1), minus_one, hi, lo);
+      };
+      term(x0.x, x0.y, h.x, l.x);
+      term(x0.z, x0.w, h.y, l.y);
+      term(x1.x, x1.y, h.z, l.z);
+      term(x1.z, x1.w, h.w, l.w);
+      const uint32_t at = row ^ (2 * j);
+      *reinterpret_cast<uint4*>(packed + at) = h;
+      *reinterpret_cast<uint4*>(packed + L::kXTile + at) = l;
+    };
+    F2 mul, keep;                                  // of the chunk's decay: X <- mul X + keep X
+    auto stepped = [&](const float4& x, F2 v0, F2 v1) {
+      const F2 a0(x.x, x.y), a1(x.z, x.w);
+      const float2 y0 = fma2(mul, a0, fma2(keep, a0, v0)).get(), y1 = fma2(mul, a1, fma2(keep, a1, v1)).get();
+      return make_float4(y0.x, y0.y, y1.x, y1.y);
+    };
+    // the largest magnitude of an fp16 tile to 2^13 ... 2^14: X may lie outside fp16's range
+    auto scale_down = [&](uint32_t top, int i) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) sMax[4 * (i & 1) + w] = top;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
+      top = max(max(all.x, all.y), max(all.z, all.w));
+      const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
+      if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
+      return __uint_as_float((uint32_t)(127 - e) << 23);
+    };
+    auto magnitude = [](const float4& x) {
+      return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+    };
+    auto send = [&](int c) {                       // what this warp has written, to the CTA of the next chunk
+      if (size == 1 || c + 1 == sp.nch) return;
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
+        copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
+      }
+    };
+    auto receive = [&](int i, int c) {
+      if (size == 1 || c == 0) return;
+      wait(bIn + w, rank == 0 ? i - 1 : i);
+      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
+    };
+    for (int i = 0; i < mine; ++i) {
+      const int c = chunk(i), cnt = sp.live(c);
+      const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
+      mul = both(decay.mul);
+      keep = both(decay.keep);
+      wait_together<4, 128>(wait, w == 2, bKv + (i & 1), i >> 1);
+      tc_fence_after();
+      if constexpr (DK == 64) {
+        // all of a thread's 32 columns in registers: B^T C before the state arrives, then the state behind the chunk, which the
+        // next CTA waits for, and last the packing for this chunk's product
+        F2 v[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 16) {
+          uint32_t h[16];
+          tmem_ld16(kv + j, h);
+          if (two) {
+            uint32_t l[16];
+            tmem_ld16(kv + 64 + j, l);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[j / 2 + k] = add2(floats(h[2 * k], h[2 * k + 1]), floats(l[2 * k], l[2 * k + 1]));
+          } else {
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[j / 2 + k] = floats(h[2 * k], h[2 * k + 1]);
+          }
+        }
+        tc_fence_before();
+        arrive_on(bKvFree);
+        receive(i, c);
+        float4 x[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = *reinterpret_cast<const float4*>(in + 512 * q);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) *reinterpret_cast<float4*>(in + 512 * q) = stepped(x[q], v[2 * q], v[2 * q + 1]);
+        send(c);
+        float down = 1.f;
+        if constexpr (kHalfRange) {
+          uint32_t top = 0;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) top = max(top, magnitude(x[q]));
+          down = scale_down(top, i);
+        }
+        if (i > 0) wait_together<4, 128>(wait, w == 2, bYx, i - 1);    // the product with the packed state of the chunk before is done
+#pragma unroll
+        for (int q = 0; q < 8; q += 2) pack(x[q], x[q + 1], down, 4 * q);
+      } else {
+        if (i > 0) wait_together<4, 128>(wait, w == 2, bYx, i - 1);
+        receive(i, c);
+        float down = 1.f;
+        if constexpr (kHalfRange) {
+          uint32_t top = 0;
+#pragma unroll 2
+          for (int j = 0; j < NC; j += 4) top = max(top, magnitude(*reinterpret_cast<const float4*>(in + 128 * j)));
+          down = scale_down(top, i);
+        }
+#pragma unroll 2
+        for (int j = 0; j < NC; j += 8) {
+          uint32_t h[8], l[8];
+          tmem_ld8(kv + j, h);
+          if (two) {
+            tmem_ld8(kv + 64 + j, l);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) l[k] = 0u;
+          }
+          const float4 x0 = *reinterpret_cast<const float4*>(in + 128 * j), x1 = *reinterpret_cast<const float4*>(in + 128 * j + 512);
+          pack(x0, x1, down, j);
+          tmem_wait_ld();
+          auto v = [&](int k) { return add2(floats(h[k], h[k + 1]), floats(l[k], l[k + 1])); };
+          *reinterpret_cast<float4*>(in + 128 * j) = stepped(x0, v(0), v(2));
+          *reinterpret_cast<float4*>(in + 128 * j + 512) = stepped(x1, v(4), v(6));
+        }
+        send(c);
+        tc_fence_before();
+        arrive_on(bKvFree);
+      }
+      fence_proxy_async();
+      arrive_on(bX + (i & 1));
+    }
+    // behind the last chunk (or, without one, behind none: rank 0 then)
+    const int last = sp.nch > 0 ? (sp.nch - 1) % size : 0;
+    if (u.state_out && seg == a.n_seg - 1 && rank == last)
+#pragma unroll 2
+      for (int j = 0; j < NC; j += 4)
+        if (j < cols) *reinterpret_cast<float4*>(u.state_out + (long long)bh * u.Da * u.Dc + own + j) = *reinterpret_cast<const float4*>(in + 128 * j);
+  } else if (warp >= L::kWarpC) {
+    // ---- weighted C ----------------------------------------------------------------------------------------------------
+    const int r = tid - 32 * L::kWarpC;
+    Ring<L::kA> ra;
+    Ring<L::kB> rb;
+    const float w_full = exp2f(g2 * (float)(rev ? r : kL - 1 - r));
+    for (int i = 0; i < mine; ++i) {
+      const int cnt = sp.live(chunk(i));
+      const float w = rev || cnt == kL ? w_full : exp2f(g2 * (float)max(0, cnt - 1 - r));
+      if (warp == L::kWarpC + 2) {
+        wait(bFullC + ra.at, ra.phase);
+        if (cnt < kL) wait(bFull + ra.at, ra.phase);
+        if (i >= n_w) wait(bKv + ((i - n_w) & 1), (i - n_w) >> 1);     // the product with what stood here is done
+      }
+      asm volatile("bar.sync 3, 128;" ::: "memory");
+      uint8_t* hi = smem + w_tile(i);
+      weigh_c<T, CB>(r, cnt, w, two, smem + L::oC + ra.at * kBlk, hi, hi + kBlk, smem + L::oB + rb.at * (CB * kBlk));
+      arrive_on(bW + (i & 1));
+      ra.next();
+      rb.next();
+    }
   } else {
     // ---- weights of P --------------------------------------------------------------------------------------------------
-    const int r0 = 32 * warp, r = r0 + lane;       // token
+    const int r0 = 32 * (warp & 3), r = r0 + lane, hb = warp >> 2;    // token, half of the columns
     const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
     const float scale_p = kHalfRange ? 1.f : a.scale;
     // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
     // diagonal the latter exceeds 1, up to lambda^-15, which is in range for every decay above 2^-8 a token; the others take an
     // exponential each there.
     const bool mild = g2 >= -8.f;
-    float2 wcol[8];
+    F2 wcol[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      wcol[k] = make_float2(exp2f(g2 * (float)(rev ? 2 * k : 15 - 2 * k)), exp2f(g2 * (float)(rev ? 2 * k + 1 : 14 - 2 * k)));
+      wcol[k] = F2(exp2f(g2 * (float)(rev ? 2 * k : 15 - 2 * k)), exp2f(g2 * (float)(rev ? 2 * k + 1 : 14 - 2 * k)));
     for (int i = 0; i < mine; ++i) {
       const int cnt = sp.live(chunk(i));
-      const uint32_t s = lane_base + 128 * (i & 1);
-      wait_together<2, 128>(wait, warp == 0, bS + (i & 1), i >> 1);
+      const uint32_t s = lane_base + 128 * (i & 1) + 64 * hb;
+      wait_together<2, 256>(wait, warp == 3, bS + (i & 1), i >> 1);
       tc_fence_after();
-      uint32_t next[16];
-      tmem_ld16(s, next);
 #pragma unroll 1
-      for (int k = 0; k < 8; ++k) {
-        const int j0 = 16 * k;                     // the block's first column; the warp's rows are r0 ... r0 + 31
+      for (int k = 0; k < 4; ++k) {
+        const int j0 = 64 * hb + 16 * k;           // the block's first column; the warp's rows are r0 ... r0 + 31
         const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = (rev ? j0 >= r0 + 31 : j0 + 15 <= r0) && cnt == kL;
-        uint32_t v[16], p[8];
-        tmem_wait_ld();
-#pragma unroll
-        for (int m = 0; m < 16; ++m) v[m] = next[m];
-        if (k < 7) tmem_ld16(s + j0 + 16, next);   // the next block's columns are on their way
+        uint32_t p[8];
         if (none) {
 #pragma unroll
           for (int m = 0; m < 8; ++m) p[m] = 0u;
         } else {
-          const float row = scale_p * exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15));
+          uint32_t v[16];
+          tmem_ld16(s + 16 * k, v);
+          const F2 row = both(scale_p * exp2f(g2 * (float)(rev ? j0 - r : r - j0 - 15)));
           const int d = rev ? j0 - r : r - j0, sign = rev ? 1 : -1;    // i - j of the first column, and its change
+          tmem_wait_ld();
           if (all) {
 #pragma unroll
-            for (int m = 0; m < 8; ++m) {
-              const float2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), both(row));
-              p[m] = Op16<T>::pack(x.x, x.y);
-            }
+            for (int m = 0; m < 8; ++m) p[m] = pack2<T>(mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), row));
           } else if (mild && cnt == kL) {
             const int t = r - j0;                  // columns up to t, or from t on
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
-              const float2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), both(row));
+              const float2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), row).get();
               v[2 * m] = __float_as_uint(x.x);
               v[2 * m + 1] = __float_as_uint(x.y);
             }
