@@ -120,6 +120,9 @@ __device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, const void*
                ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+__device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3) : "memory");
+}
 // Two values an instruction.  A pair lives in one 64-bit register from where it is made, so that none is put together twice.
 struct F2 {
   uint64_t v;
@@ -181,16 +184,16 @@ struct Span {
   __device__ __forceinline__ int live(int c) const { return min(kL, n1 - first(c)); }
 };
 
-// C weighted by the decay to the chunk's end, in two terms or one; one thread a row.  Rows behind the length are cleared, here
+// C weighted by the decay to the chunk's end, in two terms or one; a thread takes PIECES of the eight 16-byte pieces of a row.  Rows behind the length are cleared, here
 // and in the tiles of b and c themselves.
-template <typename T, int CB>
-__device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8_t* src, uint8_t* hi_t, uint8_t* lo_t, uint8_t* b_t) {
+template <typename T, int CB, int PIECES = 8>
+__device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, bool two, uint8_t* src, uint8_t* hi_t, uint8_t* lo_t, uint8_t* b_t) {
   const uint32_t row = 128 * r + 16 * (r & 7);     // 16-byte piece ch of the swizzled row: row ^ 16 ch
   const F2 w2 = both(w);
   if (r >= cnt) {
     const uint4 z = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll 1
-    for (int ch = 0; ch < 8; ++ch) {
+    for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       *reinterpret_cast<uint4*>(src + at) = z;
       *reinterpret_cast<uint4*>(hi_t + at) = z;
@@ -201,7 +204,7 @@ __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8
   } else if (two) {
     const F2 minus_one = both(-1.f);
 #pragma unroll 4
-    for (int ch = 0; ch < 8; ++ch) {
+    for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       uint4 hi, lo;
@@ -215,7 +218,7 @@ __device__ __forceinline__ void weigh_c(int r, int cnt, float w, bool two, uint8
   } else {
     auto weighed = [&](uint32_t x) { return pack2<T>(mul2(unpack2<T>(x), w2)); };
 #pragma unroll
-    for (int ch = 0; ch < 8; ++ch) {
+    for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       *reinterpret_cast<uint4*>(hi_t + at) = make_uint4(weighed(x.x), weighed(x.y), weighed(x.z), weighed(x.w));
@@ -236,11 +239,11 @@ __device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t
 }
 
 // ---- the sums of the segments ----------------------------------------------------------------------------------------------
-// Warps 0-3 weighted C, 4-7 the sum (in registers), 8 loads and products.
+// Warps 0-7 weighted C, 8-11 the sum (in registers), 12 products, 13 loads.
 template <int DK> struct SumPlan {
-  static constexpr int kCB = DK / 64, kStages = 2;
-  static constexpr int oB = 0, oC = kStages * kCB * kBlk, oW = oC + kStages * kBlk, oBars = oW + 2 * kBlk, kBytes = oBars + 256 + 1024;
-  static constexpr int kThreads = 288;
+  static constexpr int kCB = DK / 64, kStages = 3;
+  static constexpr int oB = 0, oC = kStages * kCB * kBlk, oW = oC + kStages * kBlk, oBars = oW + 4 * kBlk, kBytes = oBars + 256 + 1024;
+  static constexpr int kThreads = 448;
 };
 
 template <typename T, int DK>
@@ -252,8 +255,8 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023);   // by an offset: the compiler keeps to shared-memory instructions
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
-  uint64_t *bFull = bars, *bW = bars + 2, *bKv = bars + 3, *bKvFree = bars + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 5);
+  uint64_t *bFull = bars, *bFree = bars + 3, *bW = bars + 6, *bKv = bars + 8, *bKvFree = bars + 10;      // bW, bKv, bKvFree: two buffers each
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
   const DecayUnit& u = a.u[blockIdx.z];
   const int n_cb = (u.Dc + 63) / 64;
   const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = u.rev ? blockIdx.y + 1 : blockIdx.y;
@@ -261,69 +264,74 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb, tid = threadIdx.x, warp = tid >> 5;
   const float ld = a.log_decay[h];
   const Span sp(a, decay_live(a, b), seg, u.rev != 0);
-  auto load = [&](int c) {
-    const int st = c % NST, t0 = sp.first(c);
+  auto load = [&](int c, int st) {
+    const int t0 = sp.first(c);
     mbar_expect_tx(bFull + st, (CB + 1) * kBlk);
 #pragma unroll
     for (int i = 0; i < CB; ++i) tma_load_4d(smem + L::oB + (st * CB + i) * kBlk, &maps.in[maps.ib[blockIdx.z]], bFull + st, 64 * i, t0, h, b);
     tma_load_4d(smem + L::oC + st * kBlk, &maps.in[maps.ic[blockIdx.z]], bFull + st, c0, t0, h, b);
   };
   if (tid == 0) {
-    for (int i = 0; i < NST; ++i) mbar_init(bFull + i, 1);
-    mbar_init(bW, 128); mbar_init(bKv, 1); mbar_init(bKvFree, 128);
+    for (int i = 0; i < NST; ++i) { mbar_init(bFull + i, 1); mbar_init(bFree + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bW + i, 256); mbar_init(bKv + i, 1); mbar_init(bKvFree + i, 128); }
     fence_barrier_init();
-    for (int c = 0; c < NST && c < sp.nch; ++c) load(c);
+    for (int c = 0; c < NST && c < sp.nch; ++c) load(c, c);
   }
-  if (warp == 1) tmem_alloc<128>(tmem_slot);
+  if (warp == 1) tmem_alloc<256>(tmem_slot);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   Waits wait = {status};
-  if (warp == 8) {
+  Ring<NST> ring;
+  if (warp == 13) {
     const int nch = __reduce_max_sync(0xffffffffu, sp.nch);
-    const uint32_t d = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
-    for (int c = 0; c < nch && !wait.dead; ++c) {
-      const int st = c % NST;
-      wait(bW, c);
-      if (c > 0) wait(bKvFree, c - 1);
-      tc_fence_after();
-      if (elect_one()) {
-        product_kv<DK, F>(d, base + L::oB + st * CB * kBlk, base + L::oW, true);
-        mma_commit(bKv);
-      }
+    for (int c = 0; c + NST < nch && !wait.dead; ++c) {
+      wait(bFree + ring.at, ring.phase);
+      if (elect_one()) load(c + NST, ring.at);
       __syncwarp();
-      if (c + NST < nch) {
-        wait(bKv, c);
-        if (elect_one()) load(c + NST);
-        __syncwarp();
-      }
+      ring.next();
     }
     let_copies_end(wait.dead);
-  } else if (warp >= 4) {
+  } else if (warp == 12) {
+    const int nch = __reduce_max_sync(0xffffffffu, sp.nch);
+    const uint32_t tm = __reduce_max_sync(0xffffffffu, tmem), base = smem_u32(smem);
+    for (int c = 0; c < nch && !wait.dead; ++c) {
+      wait(bW + (c & 1), c >> 1);
+      if (c > 1) wait(bKvFree + (c & 1), (c - 2) >> 1);
+      tc_fence_after();
+      if (elect_one()) {
+        product_kv<DK, F>(tm + 128 * (c & 1), base + L::oB + ring.at * (CB * kBlk), base + L::oW + (c & 1) * (2 * kBlk), true);
+        mma_commit(bKv + (c & 1));
+        mma_commit(bFree + ring.at);
+      }
+      __syncwarp();
+      ring.next();
+    }
+  } else if (warp >= 8) {
     constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
-    const int r = tid - 128, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
-    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col;
+    const int r = tid - 256, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
+    const uint32_t kv = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col;
     float X[NC];
 #pragma unroll
     for (int j = 0; j < NC; ++j) X[j] = 0.f;
     const DecayStep full(ld, kL);
-    for (int c = 0; c < sp.nch && !wait.dead; ++c) {
+    for (int c = 0; c < sp.nch; ++c) {
       const int cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
-      wait(bKv, c);
+      wait_together<2, 128>(wait, warp == 8, bKv + (c & 1), c >> 1);
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < NC; j += 16) {
         uint32_t v[16], lo[16];
-        tmem_ld16(lane_base + j, v);
-        tmem_ld16(lane_base + 64 + j, lo);
+        tmem_ld16(kv + 128 * (c & 1) + j, v);
+        tmem_ld16(kv + 128 * (c & 1) + 64 + j, lo);
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 16; ++i) X[j + i] = decay(X[j + i]) + (__uint_as_float(v[i]) + __uint_as_float(lo[i]));
       }
       tc_fence_before();
-      arrive_on(bKvFree);
+      arrive_on(bKvFree + (c & 1));
     }
     float* end = u.seg + ((long long)bh * a.n_seg + seg) * u.Da * u.Dc + (long long)d * u.Dc + c0 + col;
     if (d < u.Da)
@@ -332,18 +340,24 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (c0 + col + j < u.Dc) *reinterpret_cast<float4*>(end + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
   } else {
     const float g2 = decay_log2(ld);
-    for (int c = 0; c < sp.nch && !wait.dead; ++c) {
-      const int st = c % NST, cnt = sp.live(c);
-      const float w = exp2f(g2 * (float)(sp.rev ? tid : max(0, cnt - 1 - tid)));
-      wait(bFull + st, c / NST);
-      if (c > 0) wait(bKv, c - 1);                 // the products with the weighted C of the chunk before are done
-      weigh_c<T, CB>(tid, cnt, w, true, smem + L::oC + st * kBlk, smem + L::oW, smem + L::oW + kBlk, smem + L::oB + st * CB * kBlk);
-      arrive_on(bW);
+    const int r = tid & 127, half = tid >> 7;      // row, half of its pieces
+    for (int c = 0; c < sp.nch; ++c) {
+      const int cnt = sp.live(c);
+      const float w = exp2f(g2 * (float)(sp.rev ? r : max(0, cnt - 1 - r)));
+      if (warp == 1) {
+        wait(bFull + ring.at, ring.phase);
+        if (c > 1) wait(bKv + (c & 1), (c - 2) >> 1);        // the product with what stood here is done
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      uint8_t* hi = smem + L::oW + (c & 1) * (2 * kBlk);
+      weigh_c<T, CB, 4>(r, 4 * half, cnt, w, true, smem + L::oC + ring.at * kBlk, hi, hi + kBlk, smem + L::oB + ring.at * (CB * kBlk));
+      arrive_on(bW + (c & 1));
+      ring.next();
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) tmem_dealloc<128>(tmem);
+  if (warp == 1) tmem_dealloc<256>(tmem);
 }
 
 // ---- the walk --------------------------------------------------------------------------------------------------------------
@@ -521,7 +535,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       for (int i = 0; i < n && !wait.dead; ++i) {
         if (L::kB == 1 && i + 1 < n) {
           wait(bFreeB, i);
-          if (elect_one()) load_b(i + 1, 0, (i + 1) % L::kA);
+          if (elect_one()) {
+            load_b(i + 1, 0, (i + 1) % L::kA);
+            if (i + 2 < n)                         // the next one is asked into L2: with a single tile its way is waited for
+              for (int k = 0; k < CB; ++k) tma_prefetch_4d(&maps.in[maps.ib[blockIdx.z]], 64 * k, sp.first(chunk(i + 2)), h, b);
+          }
           __syncwarp();
         }
         if (i + L::kA < n) {
@@ -780,7 +798,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       }
       asm volatile("bar.sync 3, 128;" ::: "memory");
       uint8_t* hi = smem + w_tile(i);
-      weigh_c<T, CB>(r, cnt, w, two, smem + L::oC + ra.at * kBlk, hi, hi + kBlk, smem + L::oB + rb.at * (CB * kBlk));
+      weigh_c<T, CB>(r, 0, cnt, w, two, smem + L::oC + ra.at * kBlk, hi, hi + kBlk, smem + L::oB + rb.at * (CB * kBlk));
       arrive_on(bW + (i & 1));
       ra.next();
       rb.next();
@@ -879,19 +897,36 @@ int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluste
   return cudaLaunchKernelExC(&cfg, kernel, args) == cudaSuccess ? FLARE_OK : FLARE_ECUDA;
 }
 
-// How a call is spread: CTAs of a sequence (a cluster) and segments of the token axis.
+// How a call is spread: the CTAs of a sequence (a cluster) and the segments of the token axis, whichever the times below say is
+// shortest.  Measured (us, 64 / 128 features): a chunk in a CTA 2.0 / 3.5; a chunk's step of the state from CTA to CTA 0.65 /
+// 1.25, which bounds what a cluster gains on a long sequence (clusters of eight on 32 or more are not worth having); a chunk's
+// sum 0.6 / 0.8; the ends of a launch 7.  E.g. B = 1, H = 8, N = 65536, D = 64: 902 us with one CTA a head, 465, 352 and 271 in
+// clusters of 2, 4 and 8; B = 4, H = 16, N = 8192, D = 64: 128 us, 82 in clusters of 2, 125 in two segments.
 struct Spread { int cluster, segments; };
-Spread pick_spread(int B, int H, int N, int Dc, int n_units) {
+Spread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
   const long long seqs = (long long)B * H * ((Dc + 63) / 64) * n_units;
   const int chunks = (int)(((long long)N + kL - 1) / kL), sms = num_sms();
-  Spread s = {1, 1};
-  while (s.cluster < 8 && seqs * s.cluster * 2 <= sms + sms / 8 && s.cluster * 2 <= chunks) s.cluster *= 2;
-  if (s.cluster == 8) {
-    long long n = sms / (seqs * 8);
-    if (n > chunks / 16) n = chunks / 16;
-    s.segments = n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  const bool wide = Da > 64;
+  const float chunk = wide ? 3.5f : 2.f, step = wide ? 1.25f : 0.65f, sum = wide ? 0.8f : 0.6f, ends = 7.f;
+  auto waves = [&](long long ctas, int room) { return (float)((ctas + room - 1) / room); };
+  Spread best = {1, 1};
+  float least = 1e30f;
+  for (int c = 1; c <= 8; c *= 2) {
+    if (c > chunks) break;
+    const int room = c == 8 ? sms * 3 / 4 : sms / c * c;     // clusters of eight do not fill the GPCs
+    const long long full = sms / (seqs * c);                 // segments that fill the GPU once
+    for (int k = 0; k < 4; ++k) {
+      long long s = k == 0 ? 1 : k == 1 ? full / 2 : k == 2 ? full : 2 * full;
+      if (s > chunks / (2 * c)) s = chunks / (2 * c);
+      if (s > 256) s = 256;
+      if (s < 1) s = 1;
+      const int len = (int)((chunks + s - 1) / s), own = (len + c - 1) / c;
+      float t = waves(seqs * c * s, room) * ((c > 1 && len * step > own * chunk ? len * step : own * chunk) + ends);
+      if (s > 1) t += waves(seqs * (s - 1), sms) * (len * sum + ends) + 4.f;
+      if (t < least) { least = t; best = {c, (int)s}; }
+    }
   }
-  return s;
+  return best;
 }
 
 template <typename T, int DK>
@@ -931,8 +966,7 @@ bool decay_tc_supported(const DecayArgs& a, int dtype) {
 }
 
 int decay_tc_segments(int B, int H, int N, int Da, int Dc, int n_units) {
-  (void)Da;
-  return pick_spread(B, H, N, Dc, n_units).segments;
+  return pick_spread(B, H, N, Da, Dc, n_units).segments;
 }
 
 int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
@@ -967,7 +1001,7 @@ int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
     maps.ic[i] = map_of(u.c, u.cs, u.Dc, order[i][2]);
     if (maps.ia[i] < 0 || maps.ib[i] < 0 || maps.ic[i] < 0) return FLARE_EUNSUPPORTED;
   }
-  const int cluster = pick_spread(a.B, a.H, a.N, Dc, a.n_units).cluster;
+  const int cluster = pick_spread(a.B, a.H, a.N, Da, Dc, a.n_units).cluster;
   if (dtype == FLARE_BF16) return Da <= 64 ? launch_all<__nv_bfloat16, 64>(maps, a, Dc, cluster, st) : launch_all<__nv_bfloat16, 128>(maps, a, Dc, cluster, st);
   return Da <= 64 ? launch_all<__half, 64>(maps, a, Dc, cluster, st) : launch_all<__half, 128>(maps, a, Dc, cluster, st);
 }
