@@ -60,6 +60,16 @@ __device__ __forceinline__ bool poll(uint64_t* bar, uint32_t parity) {
       : "=&r"(tries) : "r"(smem_u32(bar)), "r"(parity), "n"(kTries) : "memory");
   return tries < kTries;
 }
+// Whether a phase is over, without waiting for it; the same answer in all lanes of the warp.
+__device__ __forceinline__ bool is_over(uint64_t* bar, int parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(smem_u32(bar)), "r"((uint32_t)parity & 1) : "memory");
+  return __all_sync(0xffffffffu, ok != 0);
+}
 // A thread's waits: once one has run out the others return at once, so that the CTA ends; the status word gets its bit.  Warps
 // that meet at a named barrier go through all their chunks all the same.
 struct Waits {
@@ -494,7 +504,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (L::kB == 1 && i + 1 < n) product_s(i + 1);
       }
     } else if (warp == L::kWarpI + 1) {
-      // ---- B^T C, a chunk ahead, and A X ---------------------------------------------------------------------------------
+      // ---- B^T C, a chunk ahead where its operands are there, and A X ----------------------------------------------------
       Ring<L::kA> rf;                              // of the operands' barriers, a chunk ahead of ra
       auto product_bc = [&](int i) {
         wait(bFull + rf.at, rf.phase);
@@ -512,7 +522,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       };
       if (n > 0) product_bc(0);
       for (int i = 0; i < n && !wait.dead; ++i) {
-        if (i + 1 < n) product_bc(i + 1);
+        // With two tiles of c the next one's weights may be late: A X does not wait for them then (218 -> 197 us at B = 9,
+        // H = 8, N = 8192, D = 128; with three tiles it is better to wait, 126 against 135 us at H = 16, D = 64).
+        const bool ahead = i + 1 < n && (L::kB > 1 || is_over(bW + ((i + 1) & 1), (i + 1) >> 1));
+        if (ahead) product_bc(i + 1);
         wait(bX + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
         tc_fence_after();
@@ -528,6 +541,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         }
         __syncwarp();
         ra.next();
+        if (!ahead && i + 1 < n) product_bc(i + 1);
       }
     } else {
       // ---- loads: tiles are refilled when the chunk's products have completed ---------------------------------------------
@@ -537,8 +551,14 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           wait(bFreeB, i);
           if (elect_one()) {
             load_b(i + 1, 0, (i + 1) % L::kA);
-            if (i + 2 < n)                         // the next one is asked into L2: with a single tile its way is waited for
-              for (int k = 0; k < CB; ++k) tma_prefetch_4d(&maps.in[maps.ib[blockIdx.z]], 64 * k, sp.first(chunk(i + 2)), h, b);
+            if (i + 3 < n) {                       // with so few tiles their way is waited for: it starts in L2
+              const int t0 = sp.first(chunk(i + 3));
+              for (int k = 0; k < CB; ++k) {
+                tma_prefetch_4d(&maps.in[maps.ib[blockIdx.z]], 64 * k, t0, h, b);
+                tma_prefetch_4d(&maps.in[maps.ia[blockIdx.z]], 64 * k, t0, h, b);
+              }
+              tma_prefetch_4d(&maps.in[maps.ic[blockIdx.z]], c0, t0, h, b);
+            }
           }
           __syncwarp();
         }
