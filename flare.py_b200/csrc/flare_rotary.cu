@@ -2,9 +2,11 @@
 // position * freqs[i].  Pairs are (i, i + R/2) or (2i, 2i + 1) for the first R features; the rest is copied.
 //
 // The angle is reduced to a part of a turn in 64 bits (position * freq is off by 0.06 rad at position 10^6 in 32), its sine
-// and cosine are taken in 32.  No table is kept: a thread computes the angles of its pairs once and then takes the heads of
-// one or two tensors (q and k) one after the other, so that a token's angles are shared by all of its heads.
-// What bounds it is HBM: every element is read and written once, 16 bytes an access.
+// and cosine are taken in 32.  No table is kept: a thread computes the angles of its pairs once and then takes several heads of
+// one or two tensors (q and k) one after the other.  Angles made once a block, in shared memory, were slower (81 against 55 us
+// for q and k at B = 4, H = 16, N = 8192, D = 64 bf16: two more dependent accesses a head), and so were the loads of four heads
+// ahead of their use (82 us: at 111 registers too few threads fit).
+// What bounds it is HBM: every element is read and written once, 16 bytes an access; 4.9 TB/s at that size, 74 % of a copy's.
 #include <cstdarg>
 #include <cstdio>
 #include "common.cuh"
@@ -37,7 +39,8 @@ struct RotArgs {
   RotTensor t[2];
   int B, N, D, half;                               // R = 2 * half features are rotated
   int items, rot_items;                            // pieces of a row: rotated ones first, then copied ones
-  int heads, group;                                // heads of both tensors together; heads of one thread
+  int heads, groups;                               // heads of both tensors together; threads that share them
+  int heads_inner;                                 // whether heads lie closer together than tokens
   const double* freqs;
   const void* positions;                           // or null: offset + n
   int pos32;
@@ -57,11 +60,15 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ Rot
   using P = Pack<T, VEC>;
   constexpr int PAIRS = INTER && VEC > 1 ? VEC / 2 : VEC;
   constexpr int WIDTH = INTER ? 2 * PAIRS : VEC;   // columns from one rotated item to the next
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long tok = i / a.items;
-  const int item = (int)(i % a.items);
-  if (tok >= (long long)a.B * a.N) return;
-  const int b = (int)(tok / a.N), n = (int)(tok % a.N);
+  // Neighbouring threads go along a row, then along whichever of heads and tokens lies closer in memory.
+  const uint32_t i = blockIdx.x * kThreads + threadIdx.x;    // the host keeps items and shares of all tokens below 2^32
+  const uint32_t row = i / (uint32_t)a.items, toks = (uint32_t)a.B * (uint32_t)a.N;
+  const int item = (int)(i - row * (uint32_t)a.items);
+  const uint32_t by = a.heads_inner ? (uint32_t)a.groups : toks, quot = row / by, rest = row - quot * by;
+  const uint32_t tok = a.heads_inner ? quot : rest;
+  const int share = (int)(a.heads_inner ? rest : quot);
+  if (tok >= toks || share >= a.groups) return;
+  const int b = (int)(tok / (uint32_t)a.N), n = (int)(tok - (uint32_t)b * (uint32_t)a.N);
   const bool rot = item < a.rot_items;
   const int col = rot ? item * WIDTH : 2 * a.half + (item - a.rot_items) * VEC;
   float cs[PAIRS], sn[PAIRS];
@@ -80,9 +87,8 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ Rot
       sn[j] *= a.mag * a.sign;
     }
   }
-  const int h0 = blockIdx.y * a.group, h1 = min(a.heads, h0 + a.group);
-#pragma unroll 4
-  for (int hh = h0; hh < h1; ++hh) {
+#pragma unroll 8
+  for (int hh = share; hh < a.heads; hh += a.groups) {
     const bool second = hh >= a.t[0].H;
     const RotTensor& t = a.t[second ? 1 : 0];
     const int h = second ? hh - a.t[0].H : hh;
@@ -121,13 +127,16 @@ template <typename T, int VEC>
 void go(RotArgs& a, bool interleaved, cudaStream_t st) {
   a.rot_items = interleaved && VEC > 1 ? 2 * a.half / VEC : a.half / VEC;
   a.items = a.rot_items + (a.D - 2 * a.half) / VEC;
+  // Threads that share a token's heads compute its angles each: as many as give the GPU some 4600 threads per SM (55 us where
+  // 303,000 threads in all take 61, B = 4, H = 16, N = 8192, D = 64 bf16; beyond that the angles cost more: 62 us at 16 shares).
   const long long threads = (long long)a.B * a.N * a.items;
-  // heads of one thread: as many as leave the GPU two thousand threads per SM, since each group computes its angles anew
-  const long long want = (2048LL * num_sms() + threads - 1) / threads;
-  long long groups = want < a.heads ? want : a.heads;
+  long long groups = (4608LL * num_sms() + threads / 2) / threads;
+  if (groups > a.heads) groups = a.heads;
   if (groups < 1) groups = 1;
-  a.group = (int)((a.heads + groups - 1) / groups);
-  const dim3 grid((unsigned)((threads + kThreads - 1) / kThreads), (unsigned)((a.heads + a.group - 1) / a.group));
+  while (groups > 1 && threads * groups > 0xffff0000LL) --groups;
+  a.groups = (int)groups;
+  a.heads_inner = a.t[0].xs[1] <= a.t[0].xs[2];
+  const dim3 grid((unsigned)((threads * groups + kThreads - 1) / kThreads));
   if (interleaved) launch_dep(k_rotary<T, VEC, true>, grid, dim3(kThreads), 0, st, a);
   else launch_dep(k_rotary<T, VEC, false>, grid, dim3(kThreads), 0, st, a);
 }
@@ -167,7 +176,7 @@ extern "C" int flare_rotary(int B, int Hq, int Hk, int N, int D, int R, int dtyp
   if (!q || !q_out || !q_stride || !q_out_stride || !freqs || (k && (!k_out || !k_stride || !k_out_stride)) || (positions && !position_stride))
     return refuse(FLARE_EINVAL, "rotary: null pointer");
   if (dtype != FLARE_F32 && dtype != FLARE_F16 && dtype != FLARE_BF16) return refuse(FLARE_EINVAL, "rotary: bad dtype %d", dtype);
-  if (((long long)B * N * D + kThreads - 1) / kThreads > 0x7fffffffLL || (long long)Hq + Hk > 65535)
+  if ((long long)B * N > 0xffff0000LL / D || (k && Hq > 0x7fffffff - Hk))
     return refuse(FLARE_EUNSUPPORTED, "rotary: B*N*D or the number of heads is too large");
   RotArgs a = {};
   a.t[0].x = q; a.t[0].out = q_out; a.t[0].H = Hq;
