@@ -36,9 +36,10 @@ int refuse(int code, const char* fmt, ...) {
 template <typename T>
 __device__ __forceinline__ void load_rows(float* dst, int pitch, const T* src, long long row_stride, int tok0, int step, int cnt,
                                           int col0, int cols, int D, bool vec) {
-  const int quads = cols / 4;
-  for (int e = threadIdx.x; e < kSub * quads; e += kThreads) {
-    const int r = e / quads, c = 4 * (e % quads), col = col0 + c;
+  const int quads = cols / 4, per_pass = kThreads / quads, r0 = threadIdx.x / quads, c = 4 * (threadIdx.x - r0 * quads), col = col0 + c;
+  if (r0 >= per_pass) return;                      // threads beyond whole rows have none
+#pragma unroll 4
+  for (int r = r0; r < kSub; r += per_pass) {
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < cnt && col < D) {
       const T* p = src + (long long)(tok0 + r * step) * row_stride + col;
@@ -84,7 +85,7 @@ __device__ __forceinline__ void load_cv(const float* p, float (&x)[CV]) {
 // What bounds it: fp32 FMA issue.  Tiles of 4 x 4 results per thread take 8 16-byte loads for 64 multiply-adds; blocks of
 // the masked product above the diagonal are left out.
 template <typename T, int CV, bool WALK>
-__global__ void __launch_bounds__(kThreads, CV == 4 ? 2 : 1) k_decay_simt(const __grid_constant__ DecayArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constant__ DecayArgs a) {
   grid_dep_sync();
   constexpr int DVB = 16 * CV;
   extern __shared__ __align__(16) float sm[];
@@ -102,10 +103,7 @@ __global__ void __launch_bounds__(kThreads, CV == 4 ? 2 : 1) k_decay_simt(const 
   float* sA = sQ + kSub * pitch;                   // [64][kPitchA]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const float ld = a.log_decay[h];
-  if (tid <= kSub) {
-    const double g = ld < -140.f ? -140.0 : (double)ld;     // NaN stays NaN
-    sW[tid] = (float)exp(g * tid);
-  }
+  if (tid <= kSub) sW[tid] = exp2f(decay_log2(ld) * (float)tid);
   const int live = decay_live(a, b);
   const int n0 = seg * a.seg_len, n1 = min(live, n0 + a.seg_len), n_end = min(a.N, n0 + a.seg_len);
   const T* pa = static_cast<const T*>(u.a) + b * u.as[0] + h * u.as[1];
@@ -430,8 +428,8 @@ int run_decode(const DecodeArgs& a0, cudaStream_t st) {
 int pick_segments(int B, int H, int N, int Dc, int n_units) {
   const int cb = (Dc + 63) / 64;
   const long long ctas = (long long)B * H * cb * n_units;
-  long long s = (2LL * num_sms() + ctas - 1) / ctas;         // two CTAs' worth of work per SM
-  const long long max_s = ((long long)N + 2 * kSub - 1) / (2 * kSub);
+  long long s = 2LL * num_sms() / ctas;                      // the two CTAs that an SM holds
+  const long long max_s = ((long long)N + kSub - 1) / kSub;
   if (s > max_s) s = max_s;
   if (s > 256) s = 256;
   return s < 1 ? 1 : (int)s;
