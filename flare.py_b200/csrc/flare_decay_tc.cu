@@ -450,6 +450,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, L::kXBytes / 4);
   }
   if (warp == 1) tmem_alloc<512>(tmem_slot);
+  if (L::kStage && tid == 64) prefetch_tmap(&maps.out[blockIdx.z]);
   tc_fence_before();
   cluster_sync();                                  // every CTA's barriers stand before a state is sent
   tc_fence_after();
@@ -831,20 +832,20 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
     // diagonal the latter exceeds 1, up to lambda^-15, which is in range for every decay above 2^-8 a token; the others take an
     // exponential each there.
+    // Columns behind the length are zero in S already: its rows of b were cleared.
     const bool mild = g2 >= -8.f;
     F2 wcol[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       wcol[k] = F2(exp2f(g2 * (float)(rev ? 2 * k : 15 - 2 * k)), exp2f(g2 * (float)(rev ? 2 * k + 1 : 14 - 2 * k)));
     for (int i = 0; i < mine; ++i) {
-      const int cnt = sp.live(chunk(i));
       const uint32_t s = lane_base + 128 * (i & 1) + 64 * hb;
       wait_together<2, 256>(wait, warp == 3, bS + (i & 1), i >> 1);
       tc_fence_after();
 #pragma unroll 1
       for (int k = 0; k < 4; ++k) {
         const int j0 = 64 * hb + 16 * k;           // the block's first column; the warp's rows are r0 ... r0 + 31
-        const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = (rev ? j0 >= r0 + 31 : j0 + 15 <= r0) && cnt == kL;
+        const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = rev ? j0 >= r0 + 31 : j0 + 15 <= r0;
         uint32_t p[8];
         if (none) {
 #pragma unroll
@@ -858,7 +859,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           if (all) {
 #pragma unroll
             for (int m = 0; m < 8; ++m) p[m] = pack2<T>(mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), row));
-          } else if (mild && cnt == kL) {
+          } else if (mild) {
             const int t = r - j0;                  // columns up to t, or from t on
 #pragma unroll
             for (int m = 0; m < 8; ++m) {
@@ -878,13 +879,13 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           } else {
 #pragma unroll 1
             for (int m = 0; m < 8; ++m) {
-              const int d0 = d + sign * (2 * m), d1 = d0 + sign, j = j0 + 2 * m;
+              const int d0 = d + sign * (2 * m), d1 = d0 + sign;
               uint32_t s0 = 0, s1 = 0;
 #pragma unroll
               for (int q = 0; q < 8; ++q)
                 if (q == m) { s0 = v[2 * q]; s1 = v[2 * q + 1]; }
-              const float x0 = d0 >= 0 && j < cnt ? __uint_as_float(s0) * (scale_p * exp2f(g2 * (float)d0)) : 0.f;
-              const float x1 = d1 >= 0 && j + 1 < cnt ? __uint_as_float(s1) * (scale_p * exp2f(g2 * (float)d1)) : 0.f;
+              const float x0 = d0 >= 0 ? __uint_as_float(s0) * (scale_p * exp2f(g2 * (float)d0)) : 0.f;
+              const float x1 = d1 >= 0 ? __uint_as_float(s1) * (scale_p * exp2f(g2 * (float)d1)) : 0.f;
               const uint32_t t = Op16<T>::pack(x0, x1);
 #pragma unroll
               for (int q = 0; q < 8; ++q)
