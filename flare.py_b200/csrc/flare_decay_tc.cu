@@ -441,9 +441,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     fence_barrier_init();
     for (int i = 0; i < mine; ++i) {
+      if (i < L::kC) load_c(i, i);
       if (i < L::kB) load_b(i, i, i);
       if (i < L::kA) load_a(i, i);
-      if (i < L::kC) load_c(i, i);
       if (i >= 2) break;
     }
     if (size > 1 && mine > (rank == 0 ? 1 : 0))                           // the first state that comes from another CTA
@@ -566,9 +566,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (i + L::kA < n) {
           wait(bFree + ra.at, ra.phase);
           if (elect_one()) {
+            load_c(i + L::kA, ra.at);              // c first: its weighting starts the chunk's longest chain
             if (L::kB > 1) load_b(i + L::kA, ra.at, ra.at);
             load_a(i + L::kA, ra.at);
-            load_c(i + L::kA, ra.at);
           }
           __syncwarp();
           ra.next();
