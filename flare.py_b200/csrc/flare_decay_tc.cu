@@ -3,8 +3,10 @@
 //
 //   P   = (a_i . b_j) lambda^(i-j)  for j <= i      S = A B^T in tensor memory; 256 threads weigh, mask and pack it there
 //   out = scale * (P C + lambda^(i+1) A X)          X: the state before the chunk, in two 16-bit terms; two accumulators
-//   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in two 16-bit terms where the state is a result, in one
-//                                                   where only outputs are, which round as much themselves; X itself in fp32
+//   X  <- lambda^128 X + B^T (lambda^(127-j) C)     the weighted C in one to three 16-bit terms; X itself in fp32
+//
+// One term of the weighted C is enough for the outputs, which round as much themselves.  Where the state is a result, the chunks
+// that count in it take two or three (terms_of).
 //
 // The mirror image in time (n >= t) walks the chunks from the last and mirrors the weights.
 //
@@ -183,21 +185,32 @@ __device__ __forceinline__ void split2(F2 x, F2 minus_one, uint32_t& hi, uint32_
 
 // What a chunk is to the CTA that takes it.
 struct Span {
-  int n0, n1, nch;                                 // live tokens of the segment, its chunks
+  int n0, n1, nch, end;                            // live tokens of the segment, its chunks; live tokens of the sequence
   bool rev;
-  __device__ __forceinline__ Span(const DecayArgs& a, int live, int seg, bool reverse) : rev(reverse) {
+  __device__ __forceinline__ Span(const DecayArgs& a, int live, int seg, bool reverse) : end(live), rev(reverse) {
     n0 = seg * a.seg_len;
     n1 = min(live, n0 + a.seg_len);
     nch = n1 > n0 ? (n1 - n0 + kL - 1) / kL : 0;
   }
   __device__ __forceinline__ int first(int c) const { return n0 + kL * (rev ? nch - 1 - c : c); }   // of the c-th chunk walked
   __device__ __forceinline__ int live(int c) const { return min(kL, n1 - first(c)); }
+  __device__ __forceinline__ int behind(int c) const { return end - first(c) - live(c); }             // live tokens after it
 };
 
-// C weighted by the decay to the chunk's end, in two terms or one; a thread takes PIECES of the eight 16-byte pieces of a row.  Rows behind the length are cleared, here
-// and in the tiles of b and c themselves.
+// 16-bit terms of a chunk's weighted C.  A chunk counts in the state behind the sequence by the decay over the tokens after it.
+// One, two and three bf16 terms leave 2e-3, 3e-6 and 4e-9 of a chunk (fp16: 2e-4, 4e-8): with these borders the state is right
+// to 4e-7, as sums in 32 bits are.  Without a state (training) every chunk takes one.
+template <typename T>
+__device__ __forceinline__ int terms_of(float g2, int behind) {
+  const float x = g2 * (float)behind;
+  return x > -3.f ? (Op16<T>::kFmt == 1 ? 3 : 2) : x > -13.f ? 2 : 1;
+}
+
+// C weighted by the decay to the chunk's end; a thread takes PIECES of the eight 16-byte pieces of a row.  `which` of its terms
+// are written, bit by bit: 1, 2 and 4 for the first, second and third, to w_t and the tiles behind it, but the third alone to w_t.
+// Rows behind the length are cleared, here and in the tiles of b and c themselves.
 template <typename T, int CB, int PIECES = 8>
-__device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, bool two, uint8_t* src, uint8_t* hi_t, uint8_t* lo_t, uint8_t* b_t) {
+__device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, int which, uint8_t* src, uint8_t* w_t, uint8_t* b_t) {
   const uint32_t row = 128 * r + 16 * (r & 7);     // 16-byte piece ch of the swizzled row: row ^ 16 ch
   const F2 w2 = both(w);
   if (r >= cnt) {
@@ -205,54 +218,64 @@ __device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, bool tw
 #pragma unroll 1
     for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
+      *reinterpret_cast<uint4*>(w_t + at) = z;
+      if (which & 2) *reinterpret_cast<uint4*>(w_t + kBlk + at) = z;
+      if (which == 7) *reinterpret_cast<uint4*>(w_t + 2 * kBlk + at) = z;
+      if (which == 4) continue;                    // they are clear, and products may be reading them
       *reinterpret_cast<uint4*>(src + at) = z;
-      *reinterpret_cast<uint4*>(hi_t + at) = z;
-      if (two) *reinterpret_cast<uint4*>(lo_t + at) = z;
 #pragma unroll
       for (int i = 0; i < CB; ++i) *reinterpret_cast<uint4*>(b_t + i * kBlk + at) = z;
     }
-  } else if (two) {
-    const F2 minus_one = both(-1.f);
-#pragma unroll 4
-    for (int ch = p0; ch < p0 + PIECES; ++ch) {
-      const uint32_t at = row ^ (16 * ch);
-      const uint4 x = *reinterpret_cast<const uint4*>(src + at);
-      uint4 hi, lo;
-      split2<T>(mul2(unpack2<T>(x.x), w2), minus_one, hi.x, lo.x);
-      split2<T>(mul2(unpack2<T>(x.y), w2), minus_one, hi.y, lo.y);
-      split2<T>(mul2(unpack2<T>(x.z), w2), minus_one, hi.z, lo.z);
-      split2<T>(mul2(unpack2<T>(x.w), w2), minus_one, hi.w, lo.w);
-      *reinterpret_cast<uint4*>(hi_t + at) = hi;
-      *reinterpret_cast<uint4*>(lo_t + at) = lo;
-    }
-  } else {
+  } else if (which == 1) {
     auto weighed = [&](uint32_t x) { return pack2<T>(mul2(unpack2<T>(x), w2)); };
 #pragma unroll
     for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
-      *reinterpret_cast<uint4*>(hi_t + at) = make_uint4(weighed(x.x), weighed(x.y), weighed(x.z), weighed(x.w));
+      *reinterpret_cast<uint4*>(w_t + at) = make_uint4(weighed(x.x), weighed(x.y), weighed(x.z), weighed(x.w));
+    }
+  } else {
+    const F2 minus_one = both(-1.f);
+    uint8_t* third = w_t + (which == 7 ? 2 * kBlk : 0);
+#pragma unroll 2
+    for (int ch = p0; ch < p0 + PIECES; ++ch) {
+      const uint32_t at = row ^ (16 * ch);
+      const uint4 x = *reinterpret_cast<const uint4*>(src + at);
+      uint4 t0, t1, t2;
+      auto split3 = [&](uint32_t v, uint32_t& a0, uint32_t& a1, uint32_t& a2) {
+        F2 y = mul2(unpack2<T>(v), w2);
+        a0 = pack2<T>(y);
+        y = fma2(unpack2<T>(a0), minus_one, y);
+        a1 = pack2<T>(y);
+        a2 = pack2<T>(fma2(unpack2<T>(a1), minus_one, y));
+      };
+      split3(x.x, t0.x, t1.x, t2.x);
+      split3(x.y, t0.y, t1.y, t2.y);
+      split3(x.z, t0.z, t1.z, t2.z);
+      split3(x.w, t0.w, t1.w, t2.w);
+      if (which & 1) *reinterpret_cast<uint4*>(w_t + at) = t0;
+      if (which & 2) *reinterpret_cast<uint4*>(w_t + kBlk + at) = t1;
+      if (which & 4) *reinterpret_cast<uint4*>(third + at) = t2;
     }
   }
   fence_proxy_async();
 }
 
-// B^T (hi | lo): 128 x 128 with the lo terms in the upper columns, or B^T hi alone.  For 64 features the 128 rows are the
-// features twice (the second block of the operand starts where the first does), so that each of the state's 128 threads has
-// half a row to update.
+// B^T (first term | second term): 128 x 128, or B^T times one tile: 128 x 64.  For 64 features the 128 rows are the features twice
+// (the second block of the operand starts where the first does), so that each of the state's 128 threads has half a row to update.
 template <int DK, int F>
-__device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t w_tile, bool two) {
+__device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t w_tile, bool two, bool add) {
   const uint64_t dB = smem_desc_mn128(b_tile, DK == 128 ? kBlk : 0, 1024), dW = smem_desc_mn128(w_tile, kBlk, 1024);
   const uint32_t id = two ? idesc_f16(128, 128, F, F, 1, 1) : idesc_f16(128, 64, F, F, 1, 1);
 #pragma unroll
-  for (int kk = 0; kk < 8; ++kk) mma_ss(d, dB + 128 * kk, dW + 128 * kk, id, kk > 0);
+  for (int kk = 0; kk < 8; ++kk) mma_ss(d, dB + 128 * kk, dW + 128 * kk, id, add || kk > 0);
 }
 
 // ---- the sums of the segments ----------------------------------------------------------------------------------------------
 // Warps 0-7 weighted C, 8-11 the sum (in registers), 12 products, 13 loads.
 template <int DK> struct SumPlan {
-  static constexpr int kCB = DK / 64, kStages = 3;
-  static constexpr int oB = 0, oC = kStages * kCB * kBlk, oW = oC + kStages * kBlk, oBars = oW + 4 * kBlk, kBytes = oBars + 256 + 1024;
+  static constexpr int kCB = DK / 64, kStages = DK == 64 ? 3 : 2;
+  static constexpr int oB = 0, oC = kStages * kCB * kBlk, oW = oC + kStages * kBlk, oBars = oW + 6 * kBlk, kBytes = oBars + 256 + 1024;
   static constexpr int kThreads = 448;
 };
 
@@ -272,8 +295,9 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = u.rev ? blockIdx.y + 1 : blockIdx.y;
   if (cb >= n_cb) return;
   const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb, tid = threadIdx.x, warp = tid >> 5;
-  const float ld = a.log_decay[h];
+  const float ld = a.log_decay[h], g2 = decay_log2(ld);
   const Span sp(a, decay_live(a, b), seg, u.rev != 0);
+  auto terms = [&](int c) { return u.state_out ? terms_of<T>(g2, sp.behind(c)) : 1; };
   auto load = [&](int c, int st) {
     const int t0 = sp.first(c);
     mbar_expect_tx(bFull + st, (CB + 1) * kBlk);
@@ -311,7 +335,10 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if (c > 1) wait(bKvFree + (c & 1), (c - 2) >> 1);
       tc_fence_after();
       if (elect_one()) {
-        product_kv<DK, F>(tm + 128 * (c & 1), base + L::oB + ring.at * (CB * kBlk), base + L::oW + (c & 1) * (2 * kBlk), true);
+        const uint32_t b_at = base + L::oB + ring.at * (CB * kBlk), w_at = base + L::oW + (c & 1) * (3 * kBlk), kv = tm + 128 * (c & 1);
+        const int t = terms(c);
+        product_kv<DK, F>(kv, b_at, w_at, t > 1, false);
+        if (t == 3) product_kv<DK, F>(kv + 64, b_at, w_at + 2 * kBlk, false, true);
         mma_commit(bKv + (c & 1));
         mma_commit(bFree + ring.at);
       }
@@ -329,13 +356,19 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     for (int c = 0; c < sp.nch; ++c) {
       const int cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
+      const bool more = terms(c) > 1;
       wait_together<2, 128>(wait, warp == 8, bKv + (c & 1), c >> 1);
       tc_fence_after();
 #pragma unroll
       for (int j = 0; j < NC; j += 16) {
         uint32_t v[16], lo[16];
         tmem_ld16(kv + 128 * (c & 1) + j, v);
-        tmem_ld16(kv + 128 * (c & 1) + 64 + j, lo);
+        if (more) {
+          tmem_ld16(kv + 128 * (c & 1) + 64 + j, lo);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) lo[i] = 0u;
+        }
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 16; ++i) X[j + i] = decay(X[j + i]) + (__uint_as_float(v[i]) + __uint_as_float(lo[i]));
@@ -349,7 +382,6 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       for (int j = 0; j < NC; j += 4)
         if (c0 + col + j < u.Dc) *reinterpret_cast<float4*>(end + j) = make_float4(X[j], X[j + 1], X[j + 2], X[j + 3]);
   } else {
-    const float g2 = decay_log2(ld);
     const int r = tid & 127, half = tid >> 7;      // row, half of its pieces
     for (int c = 0; c < sp.nch; ++c) {
       const int cnt = sp.live(c);
@@ -359,8 +391,8 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (c > 1) wait(bKv + (c & 1), (c - 2) >> 1);        // the product with what stood here is done
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      uint8_t* hi = smem + L::oW + (c & 1) * (2 * kBlk);
-      weigh_c<T, CB, 4>(r, 4 * half, cnt, w, true, smem + L::oC + ring.at * kBlk, hi, hi + kBlk, smem + L::oB + ring.at * (CB * kBlk));
+      weigh_c<T, CB, 4>(r, 4 * half, cnt, w, (1 << terms(c)) - 1, smem + L::oC + ring.at * kBlk, smem + L::oW + (c & 1) * (3 * kBlk),
+                        smem + L::oB + ring.at * (CB * kBlk));
       arrive_on(bW + (c & 1));
       ring.next();
     }
@@ -376,7 +408,7 @@ template <int DK> struct WalkPlan {
   // Tiles in flight: three chunks of 64 features; of 128 features two, and one of b, which is free as soon as S and B^T C have
   // been formed.
   static constexpr int kA = DK == 64 ? 3 : 2, kB = DK == 64 ? 3 : 1, kC = DK == 64 ? 3 : 2;
-  static constexpr int kW = 2;                     // tiles for the weighted C: two terms, or two buffers of one
+  static constexpr int kW = 2;                     // tiles for the weighted C: two terms at a time, or two chunks of one
   static constexpr bool kStage = DK == 64;         // outputs leave through shared memory and the TMA
   static constexpr int kXTile = DK * 128;          // one term of the packed state: [DK][64]
   static constexpr int kXBytes = DK * 64 * 4;      // the state in fp32 as it arrives
@@ -387,7 +419,7 @@ template <int DK> struct WalkPlan {
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
 };
 
-template <typename T, int DK>
+template <typename T, int DK, bool STATE>
 __global__ void __launch_bounds__(WalkPlan<DK>::kThreads, 1)
 k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ DecayArgs a, int* status) {
   grid_dep_sync();
@@ -400,7 +432,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   // bFree: a chunk's outputs are complete, and with them everything that read its tiles.  bFreeB: a single tile of b is free
   // earlier.  bIn: one a warp of the state.
   uint64_t *bFull = bars, *bFullC = bars + 3, *bFree = bars + 6, *bFreeB = bars + 9, *bS = bars + 10, *bP = bars + 12, *bX = bars + 14, *bW = bars + 16,
-           *bKv = bars + 18, *bYx = bars + 20, *bKvFree = bars + 21, *bYFree = bars + 22, *bIn = bars + 29;
+           *bKv = bars + 18, *bYx = bars + 20, *bKvFree = bars + 21, *bYFree = bars + 22, *bEv = bars + 23, *bIn = bars + 29;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
   float* sExp = reinterpret_cast<float*>(bars + 36);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 38);   // [2][4]
@@ -417,9 +449,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const int mine = (sp.nch - rank + size - 1) / size;        // chunks rank, rank + size, ... are this CTA's: 0, 1, ... below
   const float ld = a.log_decay[h], g2 = decay_log2(ld);
   auto chunk = [&](int i) { return rank + size * i; };
-  const bool two = u.state_out != nullptr;
-  const int n_w = two ? 1 : 2;                     // buffers of the weighted C
-  auto w_tile = [&](int i) { return L::oW + (two ? 0 : (i & 1) * kBlk); };
+  // The weighted C comes in events e = 0, 1, ...: a chunk of one term is one, in the tiles in turn; two terms are one in both
+  // tiles; a third is another, in the first tile.
+  auto terms = [&](int i) { return STATE ? terms_of<T>(g2, sp.behind(chunk(i))) : 1; };
 
   // a and b of a chunk land on one barrier, c on its own; `at` is the tile in its ring
   auto load = [&](uint8_t* tiles, uint64_t* full, int which, int blocks, int col, int i) {
@@ -436,7 +468,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   };
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFree + i, 2); }     // bFree: A X and P C
-    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1); mbar_init(bEv + i, 1); }
     mbar_init(bFreeB, 2); mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bYFree, 128);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     fence_barrier_init();
@@ -468,9 +500,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     Ring<L::kC> rc;
     if (warp == L::kWarpI) {
       // ---- S = A B^T and P C -------------------------------------------------------------------------------------------
+      int ev = 0;
       auto product_s = [&](int i) {
         wait(bFull + ra.at, ra.phase);
-        if (sp.live(chunk(i)) < kL) wait(bW + (i & 1), i >> 1);        // rows behind the length are cleared first
+        if (sp.live(chunk(i)) < kL) wait(bW + (ev & 1), ev >> 1);      // rows behind the length are cleared first
+        ev += terms(i) == 3 ? 2 : 1;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dA = tile_a(ra.at), dB = smem_desc<128>(base + L::oB + rb.at * (CB * kBlk));
@@ -507,17 +541,33 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     } else if (warp == L::kWarpI + 1) {
       // ---- B^T C, a chunk ahead where its operands are there, and A X ----------------------------------------------------
       Ring<L::kA> rf;                              // of the operands' barriers, a chunk ahead of ra
+      int ev = 0;
       auto product_bc = [&](int i) {
         wait(bFull + rf.at, rf.phase);
-        wait(bW + (i & 1), i >> 1);
+        wait(bW + (ev & 1), ev >> 1);
         if (i > 0) wait(bKvFree, i - 1);
         tc_fence_after();
+        const int t = terms(i);
+        const uint32_t b_at = base + L::oB + rb.at * (CB * kBlk);
+        if (t == 3) {                              // the first two, and the third by itself
+          if (elect_one()) {
+            product_kv<DK, F>(tm + L::cKv, b_at, base + L::oW, true, false);
+            mma_commit(bEv + (ev & 1));
+          }
+          __syncwarp();
+          ++ev;
+          wait(bW + (ev & 1), ev >> 1);
+          tc_fence_after();
+        }
         if (elect_one()) {
-          product_kv<DK, F>(tm + L::cKv, base + L::oB + rb.at * (CB * kBlk), base + w_tile(i), two);
+          if (STATE && t == 2) product_kv<DK, F>(tm + L::cKv, b_at, base + L::oW, true, false);
+          else product_kv<DK, F>(tm + L::cKv + (t == 3 ? 64 : 0), b_at, base + L::oW + (t == 3 ? 0 : (ev & 1) * kBlk), false, t == 3);
+          if (STATE) mma_commit(bEv + (ev & 1));
           mma_commit(bKv + (i & 1));
           if (L::kB == 1) mma_commit(bFreeB);
         }
         __syncwarp();
+        ++ev;
         rf.next();
         rb.next();
       };
@@ -525,7 +575,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       for (int i = 0; i < n && !wait.dead; ++i) {
         // With two tiles of c the next one's weights may be late: A X does not wait for them then (218 -> 197 us at B = 9,
         // H = 8, N = 8192, D = 128; with three tiles it is better to wait, 126 against 135 us at H = 16, D = 64).
-        const bool ahead = i + 1 < n && (L::kB > 1 || is_over(bW + ((i + 1) & 1), (i + 1) >> 1));
+        const bool ahead = i + 1 < n && (L::kB > 1 || is_over(bW + (ev & 1), ev >> 1));
         if (ahead) product_bc(i + 1);
         wait(bX + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
@@ -722,6 +772,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
       mul = both(decay.mul);
       keep = both(decay.keep);
+      const bool two = terms(i) > 1;
       wait_together<4, 128>(wait, w == 2, bKv + (i & 1), i >> 1);
       tc_fence_after();
       if constexpr (DK == 64) {
@@ -809,18 +860,26 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     Ring<L::kA> ra;
     Ring<L::kB> rb;
     const float w_full = exp2f(g2 * (float)(rev ? r : kL - 1 - r));
+    int ev = 0, before = 1;                        // events so far, terms of the last
     for (int i = 0; i < mine; ++i) {
       const int cnt = sp.live(chunk(i));
       const float w = rev || cnt == kL ? w_full : exp2f(g2 * (float)max(0, cnt - 1 - r));
-      if (warp == L::kWarpC + 2) {
+      const int t = terms(i), parts = t == 3 ? 2 : 1;
+      const bool leader = warp == L::kWarpC + 2;
+      if (leader) {
         wait(bFullC + ra.at, ra.phase);
         if (cnt < kL) wait(bFull + ra.at, ra.phase);
-        if (i >= n_w) wait(bKv + ((i - n_w) & 1), (i - n_w) >> 1);     // the product with what stood here is done
       }
-      asm volatile("bar.sync 3, 128;" ::: "memory");
-      uint8_t* hi = smem + w_tile(i);
-      weigh_c<T, CB>(r, 0, cnt, w, two, smem + L::oC + ra.at * kBlk, hi, hi + kBlk, smem + L::oB + rb.at * (CB * kBlk));
-      arrive_on(bW + (i & 1));
+      for (int part = 0; part < parts; ++part, ++ev) {
+        // the product with what stood here is done: the event before the last one, or the last where either takes both tiles
+        const int back = t > 1 || before > 1 ? 1 : 2;
+        if (leader && ev >= back) wait((STATE ? bEv : bKv) + ((ev - back) & 1), (ev - back) >> 1);
+        asm volatile("bar.sync 3, 128;" ::: "memory");
+        weigh_c<T, CB>(r, 0, cnt, w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
+                       smem + L::oB + rb.at * (CB * kBlk));
+        arrive_on(bW + (ev & 1));
+        before = t;
+      }
       ra.next();
       rb.next();
     }
@@ -955,7 +1014,8 @@ int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, int cluster, c
   using W = WalkPlan<DK>;
   using S = SumPlan<DK>;
   int* status = tc_status_ptr();
-  const void* walk = reinterpret_cast<const void*>(&k_decay_tc_walk<T, DK>);
+  const void* walk = a.u[0].state_out ? reinterpret_cast<const void*>(&k_decay_tc_walk<T, DK, true>)
+                                      : reinterpret_cast<const void*>(&k_decay_tc_walk<T, DK, false>);
   if (tc_set_dyn_smem(walk, W::kBytes) != FLARE_OK ||
       tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_tc_sums<T, DK>), S::kBytes) != FLARE_OK)
     return FLARE_ECUDA;
