@@ -176,7 +176,7 @@ extern "C" int flare_rotary(int B, int Hq, int Hk, int N, int D, int R, int dtyp
   if (!q || !q_out || !q_stride || !q_out_stride || !freqs || (k && (!k_out || !k_stride || !k_out_stride)) || (positions && !position_stride))
     return refuse(FLARE_EINVAL, "rotary: null pointer");
   if (dtype != FLARE_F32 && dtype != FLARE_F16 && dtype != FLARE_BF16) return refuse(FLARE_EINVAL, "rotary: bad dtype %d", dtype);
-  if ((long long)B * N > 0xffff0000LL / D || (k && Hq > 0x7fffffff - Hk))
+  if ((long long)B * N > 0xffff0000LL / D || (long long)Hq + (k ? Hk : 0) >= 1LL << 30)
     return refuse(FLARE_EUNSUPPORTED, "rotary: B*N*D or the number of heads is too large");
   RotArgs a = {};
   a.t[0].x = q; a.t[0].out = q_out; a.t[0].H = Hq;
