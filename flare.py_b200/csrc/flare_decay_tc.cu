@@ -889,10 +889,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
     const float scale_p = kHalfRange ? 1.f : a.scale;
     // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
-    // diagonal the latter exceeds 1, up to lambda^-15, which is in range for every decay above 2^-8 a token; the others take an
-    // exponential each there.
+    // diagonal the latter exceeds 1, up to lambda^-15, and the former makes up for it: products as small as 2^-66 stay normal
+    // numbers on the way for every decay above 2^-4 a token; stronger ones take an exponential for each value there.
     // Columns behind the length are zero in S already: its rows of b were cleared.
-    const bool mild = g2 >= -8.f;
+    const bool mild = g2 >= -4.f;
     F2 wcol[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)

@@ -171,6 +171,23 @@ def test_decays_at_the_ends_of_their_range(fb, cuda_dev, dtype):
             assert rel(g[:, h], w[:, h]) <= tol_y(dtype), ends[h]
 
 
+@pytest.mark.parametrize("rate", [2.0, 2.9, 5.5, 9.0])
+def test_small_values_under_strong_decays(fb, cuda_dev, rate):
+    """The weights inside a block of 16 tokens span exp(15 * rate): no product may leave the range of 32 bits on its way."""
+    q, k, v, _ = make(cuda_dev, 1, 2, 300, 64, 64, torch.bfloat16, seed=21)
+    ld = torch.full((2,), -rate, device=cuda_dev)
+    for size in (1.0, 1e-3, 1e-5):
+        a, b = (size * q.float()).bfloat16(), (size * k.float()).bfloat16()
+        leaves = [t.clone().requires_grad_(True) for t in (a, b, v)]
+        dy = torch.randn_like(v)
+        y = fb.decay_linear(*leaves, ld)
+        got = (y, *torch.autograd.grad(y, leaves, dy))
+        ref = [t.double().requires_grad_(True) for t in (a, b, v)]
+        y_ref = O.decay_linear_dense(*ref, ld, 1.0)
+        for x, w in zip(got, (y_ref, *torch.autograd.grad(y_ref, ref, dy.double()))):
+            assert rel(x, w) <= tol_y(torch.bfloat16)
+
+
 def test_fp16_states_beyond_the_range_of_fp16(fb, cuda_dev):
     """A state that a long undamped sum has taken past 65504: the outputs (small scale) and the state stay right."""
     B, H, N, D = 1, 2, 1500, 64
