@@ -245,9 +245,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
   if constexpr (WALK) {
     if (u.state_out && seg == a.n_seg - 1) end = u.state_out + st_off;
     const int z0 = max(n0, live);                  // rows behind the sequence: zeros
-    for (int e = tid; e < (n_end - z0) * DVB; e += kThreads) {
-      const int c = c0 + e % DVB;
-      if (c < u.Dc) po[(long long)(z0 + e / DVB) * u.os[2] + c] = from_f32<T>(0.f);
+    for (int n = z0 + tid / DVB; n < n_end; n += kThreads / DVB) {
+      const int c = c0 + tid % DVB;
+      if (c < u.Dc) po[n * u.os[2] + c] = from_f32<T>(0.f);
     }
   } else {
     end = u.seg + ((long long)bh * a.n_seg + seg) * Da * u.Dc;
