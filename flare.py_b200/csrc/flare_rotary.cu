@@ -124,26 +124,29 @@ __global__ void __launch_bounds__(kThreads) k_rotary(const __grid_constant__ Rot
 }
 
 template <typename T, int VEC>
-void go(RotArgs& a, bool interleaved, cudaStream_t st) {
+int go(RotArgs& a, bool interleaved, cudaStream_t st) {
   a.rot_items = interleaved && VEC > 1 ? 2 * a.half / VEC : a.half / VEC;
   a.items = a.rot_items + (a.D - 2 * a.half) / VEC;
   // Threads that share a token's heads compute its angles each: as many as give the GPU some 4600 threads per SM (55 us where
   // 303,000 threads in all take 61, B = 4, H = 16, N = 8192, D = 64 bf16; beyond that the angles cost more: 62 us at 16 shares).
   const long long threads = (long long)a.B * a.N * a.items;
+  constexpr long long kMost = 0xffff0000LL;        // thread numbers are 32-bit
+  if (threads > kMost) return refuse(FLARE_EUNSUPPORTED, "rotary: B*N=%lld tokens of %d accesses are too many", (long long)a.B * a.N, a.items);
   long long groups = (4608LL * num_sms() + threads / 2) / threads;
   if (groups > a.heads) groups = a.heads;
   if (groups < 1) groups = 1;
-  while (groups > 1 && threads * groups > 0xffff0000LL) --groups;
+  while (groups > 1 && threads * groups > kMost) --groups;
   a.groups = (int)groups;
   a.heads_inner = a.t[0].xs[1] <= a.t[0].xs[2];
   const dim3 grid((unsigned)((threads * groups + kThreads - 1) / kThreads));
   if (interleaved) launch_dep(k_rotary<T, VEC, true>, grid, dim3(kThreads), 0, st, a);
   else launch_dep(k_rotary<T, VEC, false>, grid, dim3(kThreads), 0, st, a);
+  return FLARE_OK;
 }
 
 // The widest access (16 bytes, 8 of 16-bit values, one value) that every pointer, stride and column border allows.
 template <typename T>
-void run(RotArgs& a, bool interleaved, cudaStream_t st) {
+int run(RotArgs& a, bool interleaved, cudaStream_t st) {
   auto fits = [&](int vec) {
     const int bytes = vec * (int)sizeof(T);
     if (a.D % vec || (interleaved ? 2 * a.half : a.half) % vec) return false;
@@ -156,9 +159,9 @@ void run(RotArgs& a, bool interleaved, cudaStream_t st) {
     return true;
   };
   constexpr int kWide = 16 / sizeof(T);
-  if (fits(kWide)) go<T, kWide>(a, interleaved, st);
-  else if (sizeof(T) == 2 && fits(4)) go<T, 4>(a, interleaved, st);
-  else go<T, 1>(a, interleaved, st);
+  if (fits(kWide)) return go<T, kWide>(a, interleaved, st);
+  if (sizeof(T) == 2 && fits(4)) return go<T, 4>(a, interleaved, st);
+  return go<T, 1>(a, interleaved, st);
 }
 
 }  // namespace
@@ -176,8 +179,8 @@ extern "C" int flare_rotary(int B, int Hq, int Hk, int N, int D, int R, int dtyp
   if (!q || !q_out || !q_stride || !q_out_stride || !freqs || (k && (!k_out || !k_stride || !k_out_stride)) || (positions && !position_stride))
     return refuse(FLARE_EINVAL, "rotary: null pointer");
   if (dtype != FLARE_F32 && dtype != FLARE_F16 && dtype != FLARE_BF16) return refuse(FLARE_EINVAL, "rotary: bad dtype %d", dtype);
-  if ((long long)B * N > 0xffff0000LL / D || (long long)Hq + (k ? Hk : 0) >= 1LL << 30)
-    return refuse(FLARE_EUNSUPPORTED, "rotary: B*N*D or the number of heads is too large");
+  if ((long long)Hq + (k ? Hk : 0) >= 1LL << 30) return refuse(FLARE_EUNSUPPORTED, "rotary: 2^30 heads or more");
+  if ((long long)B * N > 0xffff0000LL) return refuse(FLARE_EUNSUPPORTED, "rotary: B*N is too large");
   RotArgs a = {};
   a.t[0].x = q; a.t[0].out = q_out; a.t[0].H = Hq;
   a.t[1].x = k; a.t[1].out = k_out; a.t[1].H = k ? Hk : 0;
@@ -194,9 +197,9 @@ extern "C" int flare_rotary(int B, int Hq, int Hk, int N, int D, int R, int dtyp
   a.mag = mag;
   a.sign = back ? -1.f : 1.f;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == FLARE_F32) run<float>(a, interleaved != 0, st);
-  else if (dtype == FLARE_F16) run<__half>(a, interleaved != 0, st);
-  else run<__nv_bfloat16>(a, interleaved != 0, st);
+  const int rc = dtype == FLARE_F32 ? run<float>(a, interleaved != 0, st)
+                 : dtype == FLARE_F16 ? run<__half>(a, interleaved != 0, st) : run<__nv_bfloat16>(a, interleaved != 0, st);
+  if (rc != FLARE_OK) return rc;
   const cudaError_t e = cudaPeekAtLastError();
   if (e != cudaSuccess) return refuse(FLARE_ECUDA, "rotary: %s", cudaGetErrorString(e));
   return FLARE_OK;

@@ -145,4 +145,4 @@ def test_null_pointers_and_workspaces_are_refused(cabi):
 
     assert rot(B=0) == -1 and rot(N=0) == -1 and rot(R=3) == -1 and rot(R=0) == -1 and rot(R=66) == -1 and rot(dtype=4) == -1
     assert rot(q=None) == -1 and rot(f=None) == -1 and rot(qs=None) == -1 and rot(k=16, Hk=1) == -1 and rot(pos=16, ps=None) == -1
-    assert rot(B=1 << 20, N=1 << 20) == -5 and rot(Hq=1 << 30) == -5
+    assert rot(B=1 << 20, N=1 << 20) == -5 and rot(B=1 << 10, N=1 << 20) == -5 and rot(Hq=1 << 30) == -5

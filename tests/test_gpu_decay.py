@@ -123,6 +123,67 @@ def test_gradients_match_differences(fb, cuda_dev):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 1, 9000, 64, 64), (2, 1, 7001, 128, 64), (1, 3, 5000, 48, 136)])
+def test_long_sequences_in_clusters_and_segments(fb, cuda_dev, shape, dtype):
+    """Few heads, so that a sequence is many CTAs' work; one entry of the batch ends early.  log_decay 0 keeps every token."""
+    B, H, N, Dk, Dv = shape
+    q, k, v, ld = make(cuda_dev, *shape, dtype, seed=5)
+    ld[0] = 0.0
+    lengths = torch.tensor([N - 1000] + [N] * (B - 1), device=cuda_dev)
+    state = torch.randn(B, H, Dk, Dv, device=cuda_dev)
+    y, end = fb.decay_linear_prefill(q, k, v, ld, 0.1, state=state, lengths=lengths)
+    y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld, 0.1, state, lengths)
+    assert rel(y, y_ref) <= tol_y(dtype) and rel(end, end_ref) <= tol_state(dtype)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dy = torch.randn_like(v)
+    got = torch.autograd.grad(fb.decay_linear(*leaves, ld, 0.1, lengths), leaves, dy)
+    # the gradients are the same sum with the roles exchanged, those of k and v over the tokens from the last to the first
+    live = (torch.arange(N, device=cuda_dev) < lengths[:, None])[:, None, :, None]
+    dy = torch.where(live, dy, torch.zeros_like(dy))
+    back = lambda *ts: (O.decay_linear_recurrent(*[t.detach().flip(2) for t in ts], ld, 0.1)[0].flip(2) * live)
+    want = (O.decay_linear_recurrent(dy, v.detach(), k.detach(), ld, 0.1)[0], back(v, dy, q), back(k, q, dy))
+    for g, w in zip(got, want):
+        assert rel(g, w) <= tol_y(dtype)
+    assert fb.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_that_pass_32_bits(fb, cuda_dev, dtype):
+    B, H, N, D = 2, 2, 140, 64
+    far = 2 ** 31 + 64
+    store = torch.empty(far + 3 * H * N * D, dtype=dtype, device=cuda_dev)
+    q, k, v = [store.as_strided((B, H, N, D), (far, N * D, D, 1), i * H * N * D) for i in range(3)]
+    for t in (q, k, v):
+        t.copy_(torch.randn(B, H, N, D, device=cuda_dev))
+    ld = torch.tensor([-0.1, -0.01], device=cuda_dev)
+    y, end = fb.decay_linear_prefill(q, k, v, ld)
+    y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld)
+    assert rel(y, y_ref) <= tol_y(dtype) and rel(end, end_ref) <= tol_state(dtype)
+    state = end.clone()
+    step = fb.decay_linear_decode(q[:, :, :1], k[:, :, :1], v[:, :, :1], ld, state)
+    step_ref, state_ref = O.decay_linear_recurrent(q[:, :, :1], k[:, :, :1], v[:, :, :1], ld, 1.0, end)
+    assert rel(step, step_ref) <= tol_y(dtype) and rel(state, state_ref) <= F32
+    dy = torch.randn_like(y)
+    got = torch.ops.flare_b200.decay_bwd(q, k, v, dy, ld, 1.0, None)
+    ref = [t.double().requires_grad_(True) for t in (q, k, v)]
+    for g, w in zip(got, torch.autograd.grad(O.decay_linear_dense(*ref, ld, 1.0), ref, dy.double())):
+        assert rel(g, w) <= tol_y(dtype)
+
+
+def test_states_that_pass_32_bits(fb, cuda_dev):
+    """2^31 elements of state and more: its last heads are decoded as its first."""
+    B, H, D = 1, 2 ** 17 + 3, 128
+    state = torch.zeros(B, H, D, D, device=cuda_dev)
+    state[:, -2:] = torch.randn(2, D, D, device=cuda_dev)
+    q, k, v = [torch.randn(B, H, 1, D, device=cuda_dev) for _ in range(3)]
+    ld = torch.full((H,), -0.25, device=cuda_dev)
+    tail = slice(H - 4, H)
+    want_y, want = O.decay_linear_recurrent(q[:, tail], k[:, tail], v[:, tail], ld[tail], 1.0, state[:, tail])
+    y = fb.decay_linear_decode(q, k, v, ld, state)
+    assert rel(y[:, tail], want_y) <= F32 and rel(state[:, tail], want) <= F32
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("N,Dk,Dv", [(300, 64, 64), (257, 128, 32), (190, 64, 128), (150, 20, 36)])
 def test_padding_may_hold_anything(fb, cuda_dev, dtype, N, Dk, Dv):
     lens = [0, 1, 64, 127, 128, 129, N - 1, N, N + 50, -3]

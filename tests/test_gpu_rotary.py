@@ -190,3 +190,17 @@ def test_empty_and_refusals(fb, cuda_dev):
         fb.rotary(x, freqs.cpu())
     with pytest.raises(NotImplementedError):
         fb.rotary(x, freqs.clone().requires_grad_(True))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_offsets_that_pass_32_bits(fb, cuda_dev, dtype):
+    B, H, N, D = 2, 3, 21, 64
+    far = 2 ** 31 + 64
+    store = torch.empty(far + H * N * D, dtype=dtype, device=cuda_dev)
+    x = store.as_strided((B, H, N, D), (far, N * D, D, 1))
+    x.copy_(torch.randn(B, H, N, D, device=cuda_dev))
+    freqs = fb.rotary_frequencies(D)[0].to(cuda_dev)
+    offset = 2 ** 33                                 # as a position may
+    y = fb.rotary(x, freqs, offset=offset)
+    # 2^33 radians and more leave 2^-19 of a radian of a 64-bit angle
+    assert rel(y, O.rotary_complex(x, freqs, offset + torch.arange(N, device=cuda_dev))) <= tol(dtype) + 2 ** -18
