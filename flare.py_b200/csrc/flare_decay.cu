@@ -32,7 +32,17 @@ int refuse(int code, const char* fmt, ...) {
   return code;
 }
 
+// 16 or 4 bytes into shared memory without waiting for them; zeros where `in` is false
+template <int BYTES>
+__device__ __forceinline__ void copy_async(float* dst, const void* src, bool in) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst), n = in ? BYTES : 0;
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // rows r < 64 of one operand into shared memory as fp32, zeros behind row cnt and column D.  Row r is token tok0 + r * step.
+// fp32 rows are on their way when this returns, 16-bit ones are there.
 template <typename T>
 __device__ __forceinline__ void load_rows(float* dst, int pitch, const T* src, long long row_stride, int tok0, int step, int cnt,
                                           int col0, int cols, int D, bool vec) {
@@ -40,25 +50,30 @@ __device__ __forceinline__ void load_rows(float* dst, int pitch, const T* src, l
   if (r0 >= per_pass) return;                      // threads beyond whole rows have none
 #pragma unroll 4
   for (int r = r0; r < kSub; r += per_pass) {
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < cnt && col < D) {
-      const T* p = src + (long long)(tok0 + r * step) * row_stride + col;
+    const bool in = r < cnt && col < D;
+    const T* p = in ? src + (long long)(tok0 + r * step) * row_stride + col : src;
+    float* d = dst + r * pitch + c;
+    if constexpr (sizeof(T) == 4) {
       if (vec) {                                   // D and every stride a multiple of four elements, bases aligned alike
-        if constexpr (sizeof(T) == 4) {
-          x = *reinterpret_cast<const float4*>(p);
-        } else {
-          const uint2 t = *reinterpret_cast<const uint2*>(p);
-          const T* h = reinterpret_cast<const T*>(&t);
-          x = make_float4(to_f32(h[0]), to_f32(h[1]), to_f32(h[2]), to_f32(h[3]));
-        }
+        copy_async<16>(d, p, in);
       } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) copy_async<4>(d + i, in && col + i < D ? p + i : src, in && col + i < D);
+      }
+    } else {
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (in && vec) {
+        const uint2 t = *reinterpret_cast<const uint2*>(p);
+        const T* h = reinterpret_cast<const T*>(&t);
+        x = make_float4(to_f32(h[0]), to_f32(h[1]), to_f32(h[2]), to_f32(h[3]));
+      } else if (in) {
         x.x = to_f32(p[0]);
         if (col + 1 < D) x.y = to_f32(p[1]);
         if (col + 2 < D) x.z = to_f32(p[2]);
         if (col + 3 < D) x.w = to_f32(p[3]);
       }
+      *reinterpret_cast<float4*>(d) = x;
     }
-    *reinterpret_cast<float4*>(dst + r * pitch + c) = x;
   }
 }
 
@@ -85,7 +100,7 @@ __device__ __forceinline__ void load_cv(const float* p, float (&x)[CV]) {
 // What bounds it: fp32 FMA issue.  Tiles of 4 x 4 results per thread take 8 16-byte loads for 64 multiply-adds; blocks of
 // the masked product above the diagonal are left out.
 template <typename T, int CV, bool WALK>
-__global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constant__ DecayArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constant__ DecayArgs a, int bufs) {
   grid_dep_sync();
   constexpr int DVB = 16 * CV;
   extern __shared__ __align__(16) float sm[];
@@ -95,12 +110,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
   if (cb >= n_cb) return;
   const int b = bh / a.H, h = bh % a.H;
   const int Da = u.Da, Dap = (Da + 3) & ~3, pitch = Dap + 4, c0 = cb * DVB;
+  const int b_size = kSub * pitch, buf_size = b_size + kSub * DVB;
   float* sS = sm;                                  // [Dap][DVB]
-  float* sB = sS + Dap * DVB;                      // [64][pitch]
-  float* sC = sB + kSub * pitch;                   // [64][DVB]
-  float* sW = sC + kSub * DVB;                     // lambda^0 ... lambda^64
-  float* sQ = sW + 72;                             // [64][pitch]
-  float* sA = sQ + kSub * pitch;                   // [64][kPitchA]
+  float* sBC = sS + Dap * DVB;                     // bufs times: b [64][pitch], c [64][DVB]
+  float* sW = sBC + bufs * buf_size;               // lambda^0 ... lambda^64
+  float* sQ = sW + 72;                             // [64][pitch], and the masked products in its place
+  float* sA = sQ;                                  // [64][kPitchA]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const float ld = a.log_decay[h];
   if (tid <= kSub) sW[tid] = exp2f(decay_log2(ld) * (float)tid);
@@ -116,11 +131,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
     if (a.n_seg > 1) before = u.seg + ((long long)bh * a.n_seg + seg) * Da * u.Dc;
     else if (u.state_in) before = u.state_in + st_off;
   }
-  for (int e = tid; e < Dap * DVB; e += kThreads) {
+  const bool vs = u.Dc % 4 == 0 && reinterpret_cast<uintptr_t>(before) % 16 == 0;
+  for (int e = 4 * tid; e < Dap * DVB; e += 4 * kThreads) {
     const int d = e / DVB, c = c0 + e % DVB;
-    sS[e] = before && d < Da && c < u.Dc ? before[(long long)d * u.Dc + c] : 0.f;
+    if (!before || d >= Da || c >= u.Dc) {
+      *reinterpret_cast<float4*>(sS + e) = make_float4(0.f, 0.f, 0.f, 0.f);
+      continue;
+    }
+    const float* p = before + (long long)d * u.Dc + c;
+    if (vs) {
+      copy_async<16>(sS + e, p, true);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) copy_async<4>(sS + e + i, c + i < u.Dc ? p + i : p, c + i < u.Dc);
+    }
   }
-  const DecayStep full(ld, kSub);
   T* po = nullptr;
   bool vo = false;
   if constexpr (WALK) {
@@ -128,14 +153,29 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
     vo = quads_aligned<T>(u.out, u.os, u.Dc);
   }
 
-  for (int s = 0; n0 + s * kSub < n1; ++s) {
-    const int cnt = min(kSub, n1 - n0 - s * kSub);
-    const int tok0 = u.rev ? n1 - 1 - s * kSub : n0 + s * kSub, step = u.rev ? -1 : 1;
+  const int subs = n1 > n0 ? (n1 - n0 + kSub - 1) / kSub : 0, step = u.rev ? -1 : 1;
+  auto rows_of = [&](int s) { return min(kSub, n1 - n0 - s * kSub); };
+  auto first_of = [&](int s) { return u.rev ? n1 - 1 - s * kSub : n0 + s * kSub; };
+  auto fetch = [&](int s, int buf) {
+    load_rows(sBC + buf * buf_size, pitch, pb, u.bs[2], first_of(s), step, rows_of(s), 0, Dap, Da, vb);
+    load_rows(sBC + buf * buf_size + b_size, DVB, pc, u.cs[2], first_of(s), step, rows_of(s), c0, DVB, u.Dc, vc);
+  };
+  auto fetch_a = [&](int s) { load_rows(sQ, pitch, pa, u.as[2], first_of(s), step, rows_of(s), 0, Dap, Da, va); };
+  if (subs > 0) {
+    if constexpr (WALK) fetch_a(0);
+    fetch(0, 0);
+  }
+  const DecayStep full(ld, kSub);
+  for (int s = 0; s < subs; ++s) {
+    const int cnt = rows_of(s), tok0 = first_of(s), buf = bufs == 2 ? s & 1 : 0;
+    float *sB = sBC + buf * buf_size, *sC = sB + b_size;
+    if (bufs == 1 && s > 0) {
+      __syncthreads();
+      fetch(s, 0);
+    }
+    copies_done();
     __syncthreads();
-    load_rows(sB, pitch, pb, u.bs[2], tok0, step, cnt, 0, Dap, Da, vb);
-    load_rows(sC, DVB, pc, u.cs[2], tok0, step, cnt, c0, DVB, u.Dc, vc);
-    if constexpr (WALK) load_rows(sQ, pitch, pa, u.as[2], tok0, step, cnt, 0, Dap, Da, va);
-    __syncthreads();
+    if (bufs == 2 && s + 1 < subs) fetch(s + 1, buf ^ 1);
     if constexpr (WALK) {
       // (a_i . b_j) for j <= i: thread rows i = ty + 16 p, columns j = tx + 16 r; r > p is above the diagonal
       float acc[4][4] = {};
@@ -151,13 +191,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
           for (int r = 0; r <= p; ++r)
             acc[p][r] = fmaf(x[p].x, y[r].x, fmaf(x[p].y, y[r].y, fmaf(x[p].z, y[r].z, fmaf(x[p].w, y[r].w, acc[p][r]))));
       }
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-#pragma unroll
-        for (int r = 0; r <= p; ++r) {
-          const int i = ty + 16 * p, j = tx + 16 * r;
-          sA[i * kPitchA + j] = j <= i ? acc[p][r] * sW[i - j] : 0.f;
-        }
       // lambda^(i+1) (A S) first, then the masked product on top
       float out[4][CV] = {};
       for (int k = 0; k < Dap; k += 4) {
@@ -180,6 +213,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
 #pragma unroll
         for (int c = 0; c < CV; ++c) out[p][c] *= w;
       }
+      __syncthreads();                             // a has been read
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int r = 0; r <= p; ++r) {
+          const int i = ty + 16 * p, j = tx + 16 * r;
+          sA[i * kPitchA + j] = j <= i ? acc[p][r] * sW[i - j] : 0.f;
+        }
       __syncthreads();
 #pragma unroll
       for (int jb = 0; jb < 4; ++jb)
@@ -214,11 +255,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
             if (col + c < u.Dc) o[c] = t[c];
         }
       }
-      __syncthreads();                             // the products with S are done
+      if (s + 1 < subs) {
+        __syncthreads();                           // the masked products have been read
+        fetch_a(s + 1);
+      }
     }
     const DecayStep decay = cnt == kSub ? full : DecayStep(ld, cnt);
     for (int k0 = 4 * ty; k0 < Dap; k0 += 64) {
       float acc[4][CV] = {};
+#pragma unroll 4
       for (int i = 0; i < cnt; ++i) {
         const float4 x = *reinterpret_cast<const float4*>(sB + i * pitch + k0);
         const float w = sW[cnt - 1 - i];
@@ -232,14 +277,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
         }
       }
 #pragma unroll
-      for (int p = 0; p < 4; ++p)
+      for (int p = 0; p < 4; ++p) {
+        float* e = sS + (k0 + p) * DVB + CV * tx;
+        float x[CV];
+        load_cv<CV>(e, x);
 #pragma unroll
-        for (int c = 0; c < CV; ++c) {
-          float* e = sS + (k0 + p) * DVB + CV * tx + c;
-          *e = decay(*e) + acc[p][c];
-        }
+        for (int c = 0; c < CV; ++c) x[c] = decay(x[c]) + acc[p][c];
+        if constexpr (CV == 4) *reinterpret_cast<float4*>(e) = make_float4(x[0], x[1], x[2], x[3]);
+        else *reinterpret_cast<float2*>(e) = make_float2(x[0], x[1]);
+      }
     }
   }
+  copies_done();                                   // the state, where no token was taken
   __syncthreads();
   float* end = nullptr;
   if constexpr (WALK) {
@@ -435,25 +484,32 @@ int pick_segments(int B, int H, int N, int Dc, int n_units) {
   return s < 1 ? 1 : (int)s;
 }
 
-size_t simt_smem(int Da, int CV, bool walk) {
-  const int Dap = (Da + 3) & ~3, DVB = 16 * CV;
-  const size_t f = (size_t)Dap * DVB + kSub * (Dap + 4) + kSub * DVB + 72 + (walk ? kSub * (Dap + 4) + kSub * kPitchA : 0);
+size_t simt_smem(int Da, int CV, bool walk, int bufs) {
+  const int Dap = (Da + 3) & ~3, DVB = 16 * CV, pitch = Dap + 4;
+  const size_t f = (size_t)Dap * DVB + bufs * (kSub * pitch + kSub * DVB) + 72 + (walk ? kSub * (pitch > kPitchA ? pitch : kPitchA) : 0);
   return f * sizeof(float);
+}
+
+template <typename T, int CV, bool WALK>
+void run_simt_pass(const DecayArgs& a, int Da, int Dc, cudaStream_t st) {
+  const dim3 grid((unsigned)(a.B * a.H * ((Dc + 16 * CV - 1) / (16 * CV))), (unsigned)a.n_seg, (unsigned)a.n_units);
+  // Two tiles of b and c, the next one on its way, unless they would cost the SM its second CTA or do not fit.
+  constexpr size_t kOne = 227 * 1024, kTwo = 113 * 1024;
+  const size_t one = simt_smem(Da, CV, WALK, 1), two = simt_smem(Da, CV, WALK, 2);
+  const int bufs = two <= (one <= kTwo ? kTwo : kOne) ? 2 : 1;
+  launch_dep(k_decay_simt<T, CV, WALK>, grid, dim3(kThreads), bufs == 2 ? two : one, st, a, bufs);
 }
 
 template <typename T, int CV>
 int run_simt_cv(const DecayArgs& a, int Da, int Dc, cudaStream_t st) {
-  const int cb = (Dc + 16 * CV - 1) / (16 * CV);
-  const dim3 grid((unsigned)(a.B * a.H * cb), (unsigned)a.n_seg, (unsigned)a.n_units);
-  const size_t sm_w = simt_smem(Da, CV, true), sm_s = simt_smem(Da, CV, false);
   if (tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_simt<T, CV, true>), 227 * 1024) != FLARE_OK ||
       tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_simt<T, CV, false>), 227 * 1024) != FLARE_OK)
     return refuse(FLARE_ECUDA, "decay: cudaFuncSetAttribute failed");
   if (a.n_seg > 1) {
-    launch_dep(k_decay_simt<T, CV, false>, grid, dim3(kThreads), sm_s, st, a);
+    run_simt_pass<T, CV, false>(a, Da, Dc, st);
     launch_decay_prefix(a, st);
   }
-  launch_dep(k_decay_simt<T, CV, true>, grid, dim3(kThreads), sm_w, st, a);
+  run_simt_pass<T, CV, true>(a, Da, Dc, st);
   return FLARE_OK;
 }
 
