@@ -84,6 +84,19 @@ __device__ __forceinline__ bool quads_aligned(const void* p, const long long (&s
 
 __device__ __forceinline__ float at4(const float4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+// two fp32 values in a register pair, multiplied and added by one instruction
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float2 halves(Pair v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+
 // CV columns of a thread: a column block is 16 * CV wide.
 template <int CV>
 __device__ __forceinline__ void load_cv(const float* p, float (&x)[CV]) {
@@ -177,34 +190,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
     __syncthreads();
     if (bufs == 2 && s + 1 < subs) fetch(s + 1, buf ^ 1);
     if constexpr (WALK) {
-      // (a_i . b_j) for j <= i: thread rows i = ty + 16 p, columns j = tx + 16 r; r > p is above the diagonal
-      float acc[4][4] = {};
-      for (int k = 0; k < Dap; k += 4) {
-        float4 x[4], y[4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const float4*>(sQ + (ty + 16 * p) * pitch + k);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[r] = *reinterpret_cast<const float4*>(sB + (tx + 16 * r) * pitch + k);
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-          for (int r = 0; r <= p; ++r)
-            acc[p][r] = fmaf(x[p].x, y[r].x, fmaf(x[p].y, y[r].y, fmaf(x[p].z, y[r].z, fmaf(x[p].w, y[r].w, acc[p][r]))));
-      }
-      // lambda^(i+1) (A S) first, then the masked product on top
+      // (a_i . b_j) for j <= i, thread rows i = ty + 16 p, columns j = tx + 16 r (r > p is above the diagonal), even and odd
+      // features apart; and A S
+      Pair dot[4][4];
       float out[4][CV] = {};
-      for (int k = 0; k < Dap; k += 4) {
-        float4 x[4];
 #pragma unroll
-        for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const float4*>(sQ + (ty + 16 * p) * pitch + k);
+      for (int p = 0; p < 4; ++p)
+#pragma unroll
+        for (int r = 0; r <= p; ++r) dot[p][r] = 0;
+      for (int k = 0; k < Dap; k += 4) {
+        ulonglong2 x[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) x[p] = *reinterpret_cast<const ulonglong2*>(sQ + (ty + 16 * p) * pitch + k);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const ulonglong2 y = *reinterpret_cast<const ulonglong2*>(sB + (tx + 16 * r) * pitch + k);
+#pragma unroll
+          for (int p = r; p < 4; ++p) dot[p][r] = fma_pair(x[p].y, y.y, fma_pair(x[p].x, y.x, dot[p][r]));
+        }
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           float y[CV];
           load_cv<CV>(sS + (k + kk) * DVB + CV * tx, y);
 #pragma unroll
-          for (int p = 0; p < 4; ++p)
+          for (int p = 0; p < 4; ++p) {
+            const float2 xx = halves(kk < 2 ? x[p].x : x[p].y);
 #pragma unroll
-            for (int c = 0; c < CV; ++c) out[p][c] = fmaf(at4(x[p], kk), y[c], out[p][c]);
+            for (int c = 0; c < CV; ++c) out[p][c] = fmaf(kk % 2 ? xx.y : xx.x, y[c], out[p][c]);
+          }
         }
       }
 #pragma unroll
@@ -219,7 +232,8 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
 #pragma unroll
         for (int r = 0; r <= p; ++r) {
           const int i = ty + 16 * p, j = tx + 16 * r;
-          sA[i * kPitchA + j] = j <= i ? acc[p][r] * sW[i - j] : 0.f;
+          const float2 d = halves(dot[p][r]);
+          sA[i * kPitchA + j] = j <= i ? (d.x + d.y) * sW[i - j] : 0.f;
         }
       __syncthreads();
 #pragma unroll
@@ -255,26 +269,27 @@ __global__ void __launch_bounds__(kThreads, 2) k_decay_simt(const __grid_constan
             if (col + c < u.Dc) o[c] = t[c];
         }
       }
-      if (s + 1 < subs) {
-        __syncthreads();                           // the masked products have been read
-        fetch_a(s + 1);
-      }
+      __syncthreads();                             // the masked products and c have been read
+      if (s + 1 < subs) fetch_a(s + 1);
     }
+    for (int e = 4 * tid; e < cnt * DVB; e += 4 * kThreads) {
+      const float w = sW[cnt - 1 - e / DVB];
+      float4* x = reinterpret_cast<float4*>(sC + e);
+      *x = make_float4(x->x * w, x->y * w, x->z * w, x->w * w);
+    }
+    __syncthreads();
     const DecayStep decay = cnt == kSub ? full : DecayStep(ld, cnt);
     for (int k0 = 4 * ty; k0 < Dap; k0 += 64) {
       float acc[4][CV] = {};
 #pragma unroll 4
       for (int i = 0; i < cnt; ++i) {
         const float4 x = *reinterpret_cast<const float4*>(sB + i * pitch + k0);
-        const float w = sW[cnt - 1 - i];
         float y[CV];
         load_cv<CV>(sC + i * DVB + CV * tx, y);
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          const float xw = at4(x, p) * w;
+        for (int p = 0; p < 4; ++p)
 #pragma unroll
-          for (int c = 0; c < CV; ++c) acc[p][c] = fmaf(xw, y[c], acc[p][c]);
-        }
+          for (int c = 0; c < CV; ++c) acc[p][c] = fmaf(at4(x, p), y[c], acc[p][c]);
       }
 #pragma unroll
       for (int p = 0; p < 4; ++p) {
