@@ -21,6 +21,7 @@
 //
 // The roles' loops are kept short on purpose: four roles share a scheduler, and unrolled to straight lines they waited for
 // instructions more than for data.
+#include <type_traits>
 #include "decay.h"
 #include "launch.h"
 #include "tc_common.cuh"
@@ -205,6 +206,11 @@ __device__ __forceinline__ int terms_of(float g2, int behind) {
   const float x = g2 * (float)behind;
   return x > -3.f ? (Op16<T>::kFmt == 1 ? 3 : 2) : x > -13.f ? 2 : 1;
 }
+// Where the decay over a chunk is small, B^T C itself, which needs no rounding, is taken beside two terms of (weight - 1) C: those
+// leave 3e-6 of the 0.24 or less that the weights differ from 1 by.  The third term's second turn at the tiles is spared where
+// it would come most often, in heads of long memory.
+template <typename T>
+__device__ __forceinline__ bool near_one(float g2) { return Op16<T>::kFmt == 1 && fabsf(g2) <= 0.4f / kL; }
 
 // C weighted by the decay to the chunk's end; a thread takes PIECES of the eight 16-byte pieces of a row.  `which` of its terms
 // are written, bit by bit: 1, 2 and 4 for the first, second and third, to w_t and the tiles behind it, but the third alone to w_t.
@@ -228,7 +234,7 @@ __device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, int whi
     }
   } else if (which == 1) {
     auto weighed = [&](uint32_t x) { return pack2<T>(mul2(unpack2<T>(x), w2)); };
-#pragma unroll
+#pragma unroll 4
     for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
@@ -241,21 +247,24 @@ __device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, int whi
     for (int ch = p0; ch < p0 + PIECES; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
-      uint4 t0, t1, t2;
-      auto split3 = [&](uint32_t v, uint32_t& a0, uint32_t& a1, uint32_t& a2) {
-        F2 y = mul2(unpack2<T>(v), w2);
+      uint4 t0, t1;
+      F2 rest[4];                                  // what the first term leaves
+      auto split = [&](uint32_t v, uint32_t& a0, uint32_t& a1, F2& left) {
+        const F2 y = mul2(unpack2<T>(v), w2);
         a0 = pack2<T>(y);
-        y = fma2(unpack2<T>(a0), minus_one, y);
-        a1 = pack2<T>(y);
-        a2 = pack2<T>(fma2(unpack2<T>(a1), minus_one, y));
+        left = fma2(unpack2<T>(a0), minus_one, y);
+        a1 = pack2<T>(left);
       };
-      split3(x.x, t0.x, t1.x, t2.x);
-      split3(x.y, t0.y, t1.y, t2.y);
-      split3(x.z, t0.z, t1.z, t2.z);
-      split3(x.w, t0.w, t1.w, t2.w);
+      split(x.x, t0.x, t1.x, rest[0]);
+      split(x.y, t0.y, t1.y, rest[1]);
+      split(x.z, t0.z, t1.z, rest[2]);
+      split(x.w, t0.w, t1.w, rest[3]);
       if (which & 1) *reinterpret_cast<uint4*>(w_t + at) = t0;
       if (which & 2) *reinterpret_cast<uint4*>(w_t + kBlk + at) = t1;
-      if (which & 4) *reinterpret_cast<uint4*>(third + at) = t2;
+      if (which & 4) {
+        auto third_of = [&](uint32_t a1, F2 left) { return pack2<T>(fma2(unpack2<T>(a1), minus_one, left)); };
+        *reinterpret_cast<uint4*>(third + at) = make_uint4(third_of(t1.x, rest[0]), third_of(t1.y, rest[1]), third_of(t1.z, rest[2]), third_of(t1.w, rest[3]));
+      }
     }
   }
   fence_proxy_async();
@@ -267,7 +276,7 @@ template <int DK, int F>
 __device__ __forceinline__ void product_kv(uint32_t d, uint32_t b_tile, uint32_t w_tile, bool two, bool add) {
   const uint64_t dB = smem_desc_mn128(b_tile, DK == 128 ? kBlk : 0, 1024), dW = smem_desc_mn128(w_tile, kBlk, 1024);
   const uint32_t id = two ? idesc_f16(128, 128, F, F, 1, 1) : idesc_f16(128, 64, F, F, 1, 1);
-#pragma unroll
+#pragma unroll 2
   for (int kk = 0; kk < 8; ++kk) mma_ss(d, dB + 128 * kk, dW + 128 * kk, id, add || kk > 0);
 }
 
@@ -297,7 +306,11 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb, tid = threadIdx.x, warp = tid >> 5;
   const float ld = a.log_decay[h], g2 = decay_log2(ld);
   const Span sp(a, decay_live(a, b), seg, u.rev != 0);
-  auto terms = [&](int c) { return u.state_out ? terms_of<T>(g2, sp.behind(c)) : 1; };
+  const bool plus = near_one<T>(g2);               // two terms are those beside C itself
+  auto terms = [&](int c) {
+    const int t = u.state_out ? terms_of<T>(g2, sp.behind(c)) : 1;
+    return plus ? min(t, 2) : t;
+  };
   auto load = [&](int c, int st) {
     const int t0 = sp.first(c);
     mbar_expect_tx(bFull + st, (CB + 1) * kBlk);
@@ -339,6 +352,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         const int t = terms(c);
         product_kv<DK, F>(kv, b_at, w_at, t > 1, false);
         if (t == 3) product_kv<DK, F>(kv + 64, b_at, w_at + 2 * kBlk, false, true);
+        if (t == 2 && plus) product_kv<DK, F>(kv, b_at, base + L::oC + ring.at * kBlk, false, true);
         mma_commit(bKv + (c & 1));
         mma_commit(bFree + ring.at);
       }
@@ -391,7 +405,8 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (c > 1) wait(bKv + (c & 1), (c - 2) >> 1);        // the product with what stood here is done
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
-      weigh_c<T, CB, 4>(r, 4 * half, cnt, w, (1 << terms(c)) - 1, smem + L::oC + ring.at * kBlk, smem + L::oW + (c & 1) * (3 * kBlk),
+      const int t = terms(c);
+      weigh_c<T, CB, 4>(r, 4 * half, cnt, t == 2 && plus ? w - 1.f : w, (1 << t) - 1, smem + L::oC + ring.at * kBlk, smem + L::oW + (c & 1) * (3 * kBlk),
                         smem + L::oB + ring.at * (CB * kBlk));
       arrive_on(bW + (c & 1));
       ring.next();
@@ -432,7 +447,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   // bFree: a chunk's outputs are complete, and with them everything that read its tiles.  bFreeB: a single tile of b is free
   // earlier.  bIn: one a warp of the state.
   uint64_t *bFull = bars, *bFullC = bars + 3, *bFree = bars + 6, *bFreeB = bars + 9, *bS = bars + 10, *bP = bars + 12, *bX = bars + 14, *bW = bars + 16,
-           *bKv = bars + 18, *bYx = bars + 20, *bKvFree = bars + 21, *bYFree = bars + 22, *bEv = bars + 23, *bIn = bars + 29;
+           *bEv = bars + 18, *bYx = bars + 20, *bKvFree = bars + 21, *bYFree = bars + 22, *bIn = bars + 29;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 33);
   float* sExp = reinterpret_cast<float*>(bars + 36);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 38);   // [2][4]
@@ -451,7 +466,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   auto chunk = [&](int i) { return rank + size * i; };
   // The weighted C comes in events e = 0, 1, ...: a chunk of one term is one, in the tiles in turn; two terms are one in both
   // tiles; a third is another, in the first tile.
-  auto terms = [&](int i) { return STATE ? terms_of<T>(g2, sp.behind(chunk(i))) : 1; };
+  const bool plus = STATE && near_one<T>(g2);      // two terms are those beside C itself
+  auto terms = [&](int i) {
+    const int t = STATE ? terms_of<T>(g2, sp.behind(chunk(i))) : 1;
+    return plus ? min(t, 2) : t;
+  };
 
   // a and b of a chunk land on one barrier, c on its own; `at` is the tile in its ring
   auto load = [&](uint8_t* tiles, uint64_t* full, int which, int blocks, int col, int i) {
@@ -468,7 +487,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   };
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFree + i, 2); }     // bFree: A X and P C
-    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bKv + i, 1); mbar_init(bEv + i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bEv + i, 1); }
     mbar_init(bFreeB, 2); mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bYFree, 128);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     fence_barrier_init();
@@ -549,23 +568,23 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         tc_fence_after();
         const int t = terms(i);
         const uint32_t b_at = base + L::oB + rb.at * (CB * kBlk);
-        if (t == 3) {                              // the first two, and the third by itself
+        // one product; of two terms and C itself two; of three the first two, and the third by itself when its tile is there
+        const int last = t == 3 || (plus && t == 2);
+        for (int pass = 0;; ++pass) {
+          const uint32_t tile = base + (pass && plus ? L::oC + rf.at * kBlk : L::oW + (t == 1 ? (ev & 1) * kBlk : 0));
           if (elect_one()) {
-            product_kv<DK, F>(tm + L::cKv, b_at, base + L::oW, true, false);
-            mma_commit(bEv + (ev & 1));
+            product_kv<DK, F>(tm + L::cKv + (pass && !plus ? 64 : 0), b_at, tile, t > 1 && pass == 0, pass > 0);
+            if (t == 3 || pass == last) mma_commit(bEv + (ev & 1));
           }
           __syncwarp();
-          ++ev;
-          wait(bW + (ev & 1), ev >> 1);
-          tc_fence_after();
+          if (pass == last) break;
+          if (t == 3) {
+            ++ev;
+            wait(bW + (ev & 1), ev >> 1);
+            tc_fence_after();
+          }
         }
-        if (elect_one()) {
-          if (STATE && t == 2) product_kv<DK, F>(tm + L::cKv, b_at, base + L::oW, true, false);
-          else product_kv<DK, F>(tm + L::cKv + (t == 3 ? 64 : 0), b_at, base + L::oW + (t == 3 ? 0 : (ev & 1) * kBlk), false, t == 3);
-          if (STATE) mma_commit(bEv + (ev & 1));
-          mma_commit(bKv + (i & 1));
-          if (L::kB == 1) mma_commit(bFreeB);
-        }
+        if (L::kB == 1 && elect_one()) mma_commit(bFreeB);
         __syncwarp();
         ++ev;
         rf.next();
@@ -767,13 +786,16 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       wait(bIn + w, rank == 0 ? i - 1 : i);
       if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
     };
-    for (int i = 0; i < mine; ++i) {
+    int ev = 0;
+    for (int i = 0; i < mine; ++i, ++ev) {
       const int c = chunk(i), cnt = sp.live(c);
       const DecayStep decay = cnt == kL ? full : DecayStep(ld, cnt);
       mul = both(decay.mul);
       keep = both(decay.keep);
-      const bool two = terms(i) > 1;
-      wait_together<4, 128>(wait, w == 2, bKv + (i & 1), i >> 1);
+      const int t = terms(i);
+      const bool two = t > 1;
+      if (t == 3) ++ev;
+      wait_together<4, 128>(wait, w == 2, bEv + (ev & 1), ev >> 1);
       tc_fence_after();
       if constexpr (DK == 64) {
         // all of a thread's 32 columns in registers: B^T C before the state arrives, then the state behind the chunk, which the
@@ -824,23 +846,26 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           for (int j = 0; j < NC; j += 4) top = max(top, magnitude(*reinterpret_cast<const float4*>(in + 128 * j)));
           down = scale_down(top, i);
         }
+        auto step = [&](auto more) {               // a loop of its own for each number of terms: it is short, and waited for
 #pragma unroll 2
-        for (int j = 0; j < NC; j += 8) {
-          uint32_t h[8], l[8];
-          tmem_ld8(kv + j, h);
-          if (two) {
-            tmem_ld8(kv + 64 + j, l);
-          } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k) l[k] = 0u;
+          for (int j = 0; j < NC; j += 8) {
+            uint32_t h[8], l[8];
+            tmem_ld8(kv + j, h);
+            if constexpr (more.value) tmem_ld8(kv + 64 + j, l);
+            const float4 x0 = *reinterpret_cast<const float4*>(in + 128 * j), x1 = *reinterpret_cast<const float4*>(in + 128 * j + 512);
+            pack(x0, x1, down, j);
+            tmem_wait_ld();
+            auto v = [&](int k) {
+              const F2 first = floats(h[k], h[k + 1]);
+              if constexpr (more.value) return add2(first, floats(l[k], l[k + 1]));
+              else return first;
+            };
+            *reinterpret_cast<float4*>(in + 128 * j) = stepped(x0, v(0), v(2));
+            *reinterpret_cast<float4*>(in + 128 * j + 512) = stepped(x1, v(4), v(6));
           }
-          const float4 x0 = *reinterpret_cast<const float4*>(in + 128 * j), x1 = *reinterpret_cast<const float4*>(in + 128 * j + 512);
-          pack(x0, x1, down, j);
-          tmem_wait_ld();
-          auto v = [&](int k) { return add2(floats(h[k], h[k + 1]), floats(l[k], l[k + 1])); };
-          *reinterpret_cast<float4*>(in + 128 * j) = stepped(x0, v(0), v(2));
-          *reinterpret_cast<float4*>(in + 128 * j + 512) = stepped(x1, v(4), v(6));
-        }
+        };
+        if (two) step(std::true_type{});
+        else step(std::false_type{});
         send(c);
         tc_fence_before();
         arrive_on(bKvFree);
@@ -873,9 +898,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       for (int part = 0; part < parts; ++part, ++ev) {
         // the product with what stood here is done: the event before the last one, or the last where either takes both tiles
         const int back = t > 1 || before > 1 ? 1 : 2;
-        if (leader && ev >= back) wait((STATE ? bEv : bKv) + ((ev - back) & 1), (ev - back) >> 1);
+        if (leader && ev >= back) wait(bEv + ((ev - back) & 1), (ev - back) >> 1);
         asm volatile("bar.sync 3, 128;" ::: "memory");
-        weigh_c<T, CB>(r, 0, cnt, w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
+        weigh_c<T, CB>(r, 0, cnt, plus && t == 2 ? w - 1.f : w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
                        smem + L::oB + rb.at * (CB * kBlk));
         arrive_on(bW + (ev & 1));
         before = t;
