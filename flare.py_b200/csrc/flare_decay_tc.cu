@@ -528,11 +528,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (elect_one()) {
           const uint64_t dA = tile_a(ra.at), dB = smem_desc<128>(base + L::oB + rb.at * (CB * kBlk));
           const uint32_t d = tm + 128 * (i & 1);
+#pragma unroll 1
+          for (int blk = 0; blk < CB; ++blk)
 #pragma unroll
-          for (int kk = 0; kk < DK / 16; ++kk) {
-            const uint32_t off = (kk / 4) * (kBlk >> 4) + 2 * (kk & 3);
-            mma_ss(d, dA + off, dB + off, id_s, kk > 0);
-          }
+            for (int kk = 0; kk < 4; ++kk) mma_ss(d, dA + blk * (kBlk >> 4) + 2 * kk, dB + blk * (kBlk >> 4) + 2 * kk, id_s, blk + kk > 0);
           mma_commit(bS + (i & 1));
           if (L::kB == 1) mma_commit(bFreeB);
         }
@@ -540,22 +539,25 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         ra.next();
         rb.next();
       };
-      if (n > 0) product_s(0);
-      for (int i = 0; i < n && !wait.dead; ++i) {
-        if (L::kB > 1 && i + 1 < n) product_s(i + 1);
+      constexpr int kAhead = L::kB > 1 ? 1 : 0;    // S comes a chunk ahead of P C where there are tiles for it
+      for (int j = 0; j < n + kAhead && !wait.dead; ++j) {
+        if (j < n) product_s(j);
+        const int i = j - kAhead;
+        if (i < 0) continue;
         wait(bP + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dC = smem_desc<128>(base + L::oC + rc.at * kBlk);
           const uint32_t p = tm + 128 * (i & 1);
+#pragma unroll 1
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) mma_ts(tm + L::cY, p + 8 * (kk & 3) + 64 * (kk >> 2), dC + 128 * kk, id_y, kk > 0);
+            for (int kk = 0; kk < 4; ++kk) mma_ts(tm + L::cY, p + 64 * half + 8 * kk, dC + 512 * half + 128 * kk, id_y, half + kk > 0);
           mma_commit(bFree + rc.at);
         }
         __syncwarp();
         rc.next();
-        if (L::kB == 1 && i + 1 < n) product_s(i + 1);
       }
     } else if (warp == L::kWarpI + 1) {
       // ---- B^T C, a chunk ahead where its operands are there, and A X ----------------------------------------------------
@@ -590,28 +592,29 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         rf.next();
         rb.next();
       };
-      if (n > 0) product_bc(0);
-      for (int i = 0; i < n && !wait.dead; ++i) {
+      for (int i = 0, j = 0; i < n && !wait.dead;) {         // B^T C of chunk j, at most one ahead, or A X of chunk i
         // With two tiles of c the next one's weights may be late: A X does not wait for them then (218 -> 197 us at B = 9,
         // H = 8, N = 8192, D = 128; with three tiles it is better to wait, 126 against 135 us at H = 16, D = 64).
-        const bool ahead = i + 1 < n && (L::kB > 1 || is_over(bW + (ev & 1), ev >> 1));
-        if (ahead) product_bc(i + 1);
+        if (j < n && (j == i || (j == i + 1 && (L::kB > 1 || is_over(bW + (ev & 1), ev >> 1))))) {
+          product_bc(j++);
+          continue;
+        }
         wait(bX + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dA = tile_a(ra.at), dX = smem_desc<128>(base + L::oX);
+#pragma unroll 1
+          for (int blk = 0; blk < 2 * CB; ++blk)   // the blocks of 64 features for the first term, then for the second
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int kk = 0; kk < DK / 16; ++kk)
-              mma_ss(tm + L::cYx, dA + (kk / 4) * (kBlk >> 4) + 2 * (kk & 3), dX + t * (L::kXTile >> 4) + 128 * kk, id_y, t + kk > 0);
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(tm + L::cYx, dA + (blk & (CB - 1)) * (kBlk >> 4) + 2 * kk, dX + 512 * blk + 128 * kk, id_y, blk + kk > 0);
           mma_commit(bYx);
           mma_commit(bFree + ra.at);
         }
         __syncwarp();
         ra.next();
-        if (!ahead && i + 1 < n) product_bc(i + 1);
+        ++i;
       }
     } else {
       // ---- loads: tiles are refilled when the chunk's products have completed ---------------------------------------------
