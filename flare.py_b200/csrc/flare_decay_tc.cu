@@ -73,15 +73,15 @@ __device__ __forceinline__ bool is_over(uint64_t* bar, int parity) {
       : "=r"(ok) : "r"(smem_u32(bar)), "r"((uint32_t)parity & 1) : "memory");
   return __all_sync(0xffffffffu, ok != 0);
 }
-// A thread's waits: once one has run out the others return at once, so that the CTA ends; the status word gets its bit.  Warps
-// that meet at a named barrier go through all their chunks all the same.
+// A thread's waits: once one has run out the others return at once, so that the CTA ends, where the status word gets its bit.
+// Warps that meet at a named barrier go through all their chunks all the same.
 struct Waits {
-  int* status;
   bool dead = false;
   __device__ __forceinline__ void operator()(uint64_t* bar, int parity) {
-    if (dead || poll(bar, (uint32_t)parity & 1)) return;
-    dead = true;
-    if (status) atomicOr(status, kErrWaitTimeout);
+    if (!dead) dead = !poll(bar, (uint32_t)parity & 1);
+  }
+  __device__ __forceinline__ void report(int* status) const {
+    if (dead && status) atomicOr(status, kErrWaitTimeout);
   }
 };
 // The wait of a role of several warps: one of them polls, the others sleep at a named barrier.  The polling warps are spread over
@@ -329,7 +329,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Waits wait = {status};
+  Waits wait;
   Ring<NST> ring;
   if (warp == 13) {
     const int nch = __reduce_max_sync(0xffffffffu, sp.nch);
@@ -412,6 +412,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       ring.next();
     }
   }
+  wait.report(status);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc<256>(tmem);
@@ -506,7 +507,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   cluster_sync();                                  // every CTA's barriers stand before a state is sent
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  Waits wait = {status};
+  Waits wait;
 
   if (warp >= L::kWarpI) {
     // counts and addresses through a warp reduction: the compiler then keeps them, and the descriptors, in uniform registers
@@ -987,6 +988,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       arrive_on(bP + (i & 1));
     }
   }
+  wait.report(status);
   tc_fence_before();
   cluster_sync();                                  // no CTA leaves while another may still write into it
   if (warp == 1) tmem_dealloc<512>(tmem);
