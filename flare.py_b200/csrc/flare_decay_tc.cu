@@ -670,24 +670,23 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       ra.next();
       tc_fence_after();
       const F2 fx = both(kHalfRange ? wx * sExp[i & 3] : wx);
-      uint32_t y[2][16], x[2][16];
-      tmem_ld16(y_at, y[0]);
-      tmem_ld16(x_at, x[0]);
-#pragma unroll
+      uint32_t y[16], x[16];
+      tmem_ld16(y_at, y);
+      tmem_ld16(x_at, x);
+#pragma unroll 1
       for (int k = 0; k < 4; ++k) {
-        tmem_wait_ld();
-        if (k < 3) {
-          tmem_ld16(y_at + 16 * (k + 1), y[(k + 1) & 1]);
-          tmem_ld16(x_at + 16 * (k + 1), x[(k + 1) & 1]);
-        }
         uint32_t q[8];
+        tmem_wait_ld();
 #pragma unroll
         for (int m = 0; m < 8; ++m) {
-          F2 in_chunk = floats(y[k & 1][2 * m], y[k & 1][2 * m + 1]);
+          F2 in_chunk = floats(y[2 * m], y[2 * m + 1]);
           if constexpr (kHalfRange) in_chunk = mul2(scale2, in_chunk);
-          q[m] = pack2<T>(fma2(fx, floats(x[k & 1][2 * m], x[k & 1][2 * m + 1]), in_chunk));
+          q[m] = pack2<T>(fma2(fx, floats(x[2 * m], x[2 * m + 1]), in_chunk));
         }
-        if (k == 3) {
+        if (k < 3) {
+          tmem_ld16(y_at + 16 * (k + 1), y);
+          tmem_ld16(x_at + 16 * (k + 1), x);
+        } else {
           tc_fence_before();
           arrive_on(bYFree);
         }
