@@ -427,9 +427,9 @@ template <int DK> struct WalkPlan {
   static constexpr int kW = 2;                     // tiles for the weighted C: two terms at a time, or two chunks of one
   static constexpr bool kStage = DK == 64;         // outputs leave through shared memory and the TMA
   static constexpr int kXTile = DK * 128;          // one term of the packed state: [DK][64]
-  static constexpr int kXBytes = DK * 64 * 4;      // the state in fp32 as it arrives
+  static constexpr int kXPart = DK * 64 + 16;      // a warp's quarter of the state in fp32, as it arrives, and its largest magnitude
   static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + kW * kBlk,
-                       oIn = oX + 2 * kXTile, oOut = oIn + kXBytes, oBars = oOut + (kStage ? kBlk : 0);
+                       oOut = oX + 2 * kXTile, oIn = oOut + (kStage ? kBlk : 0), oBars = oIn + 4 * kXPart;
   static constexpr int kBytes = oBars + 512 + 1024;
   static constexpr int kWarpC = 8, kWarpX = 12, kWarpY = 16, kWarpI = 20, kThreads = 32 * (kWarpI + 3);
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
@@ -499,7 +499,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if (i >= 2) break;
     }
     if (size > 1 && mine > (rank == 0 ? 1 : 0))                           // the first state that comes from another CTA
-      for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, L::kXBytes / 4);
+      for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, L::kXPart);
   }
   if (warp == 1) tmem_alloc<512>(tmem_slot);
   if (L::kStage && tid == 64) prefetch_tmap(&maps.out[blockIdx.z]);
@@ -728,14 +728,35 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
     const int r = tid - 32 * L::kWarpX, w = warp & 3, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
     const uint32_t kv = tmem + ((uint32_t)(w * 32) << 16) + L::cKv + col;
-    uint8_t* in = smem + L::oIn + w * (L::kXBytes / 4) + 16 * lane;
+    uint8_t* in = smem + L::oIn + w * L::kXPart + 16 * lane;
     const long long own = (long long)d * u.Dc + c0 + col;
     const int cols = d < u.Da ? u.Dc - c0 - col : 0;         // of this thread's columns, those that exist
+    auto magnitude = [](const float4& x) {
+      return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
+    };
+    // fp16: the largest magnitude of the state before chunk c.  Of 128 features it is found as the state is made, and travels
+    // with it: a warp's beside its quarter, even and odd chunks apart.  Of 64, whose packing comes last, it is found then.
+    constexpr bool kSent = kHalfRange && DK == 128;
+    auto note = [&](uint32_t top, int c) {
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) *reinterpret_cast<uint32_t*>(in + L::kXPart - 16 + 4 * (c & 1)) = top;
+    };
+    auto noted = [&](int c) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = max(top, *reinterpret_cast<const uint32_t*>(smem + L::oIn + (i + 1) * L::kXPart - 16 + 4 * (c & 1)));
+      return top;
+    };
     if (rank == 0) {
       const float* before = a.n_seg > 1 ? u.seg + ((long long)bh * a.n_seg + seg) * u.Da * u.Dc : u.state_in ? u.state_in + (long long)bh * u.Da * u.Dc : nullptr;
+      uint32_t top = 0;
 #pragma unroll 2
-      for (int j = 0; j < NC; j += 4)
-        *reinterpret_cast<float4*>(in + 128 * j) = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int j = 0; j < NC; j += 4) {
+        const float4 x = before && j < cols ? *reinterpret_cast<const float4*>(before + own + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+        *reinterpret_cast<float4*>(in + 128 * j) = x;
+        if (kSent) top = max(top, magnitude(x));
+      }
+      if (kSent) note(top, 0);
     }
     const DecayStep full(ld, kL);
     // eight columns of the state before the chunk, packed for the product
@@ -763,31 +784,23 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     };
     // the largest magnitude of an fp16 tile to 2^13 ... 2^14: X may lie outside fp16's range
     auto scale_down = [&](uint32_t top, int i) {
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) sMax[4 * (i & 1) + w] = top;
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
-      top = max(max(all.x, all.y), max(all.z, all.w));
       const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
       if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
       return __uint_as_float((uint32_t)(127 - e) << 23);
-    };
-    auto magnitude = [](const float4& x) {
-      return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
     };
     auto send = [&](int c) {                       // what this warp has written, to the CTA of the next chunk
       if (size == 1 || c + 1 == sp.nch) return;
       fence_proxy_async();
       __syncwarp();
       if (lane == 0) {
-        const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * (L::kXBytes / 4));
-        copy_to_cta(remote(at, next), at, L::kXBytes / 4, remote(smem_u32(bIn + w), next));
+        const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * L::kXPart);
+        copy_to_cta(remote(at, next), at, L::kXPart, remote(smem_u32(bIn + w), next));
       }
     };
     auto receive = [&](int i, int c) {
       if (size == 1 || c == 0) return;
-      wait(bIn + w, rank == 0 ? i - 1 : i);
-      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXBytes / 4);
+      for (int k = kSent ? 0 : w; k < (kSent ? 4 : w + 1); ++k) wait(bIn + k, rank == 0 ? i - 1 : i);
+      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXPart);
     };
     int ev = 0;
     for (int i = 0; i < mine; ++i, ++ev) {
@@ -834,7 +847,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           uint32_t top = 0;
 #pragma unroll
           for (int q = 0; q < 8; ++q) top = max(top, magnitude(x[q]));
-          down = scale_down(top, i);
+          top = __reduce_max_sync(0xffffffffu, top);
+          if (lane == 0) sMax[4 * (i & 1) + w] = top;
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));
+          down = scale_down(max(max(all.x, all.y), max(all.z, all.w)), i);
         }
         if (i > 0) wait_together<4, 128>(wait, w == 2, bYx, i - 1);    // the product with the packed state of the chunk before is done
 #pragma unroll
@@ -842,13 +859,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       } else {
         if (i > 0) wait_together<4, 128>(wait, w == 2, bYx, i - 1);
         receive(i, c);
-        float down = 1.f;
-        if constexpr (kHalfRange) {
-          uint32_t top = 0;
-#pragma unroll 2
-          for (int j = 0; j < NC; j += 4) top = max(top, magnitude(*reinterpret_cast<const float4*>(in + 128 * j)));
-          down = scale_down(top, i);
-        }
+        const float down = kSent ? scale_down(noted(c), i) : 1.f;
+        uint32_t top = 0;
         auto step = [&](auto more) {               // a loop of its own for each number of terms: it is short, and waited for
 #pragma unroll 2
           for (int j = 0; j < NC; j += 8) {
@@ -863,12 +875,15 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
               if constexpr (more.value) return add2(first, floats(l[k], l[k + 1]));
               else return first;
             };
-            *reinterpret_cast<float4*>(in + 128 * j) = stepped(x0, v(0), v(2));
-            *reinterpret_cast<float4*>(in + 128 * j + 512) = stepped(x1, v(4), v(6));
+            const float4 y0 = stepped(x0, v(0), v(2)), y1 = stepped(x1, v(4), v(6));
+            *reinterpret_cast<float4*>(in + 128 * j) = y0;
+            *reinterpret_cast<float4*>(in + 128 * j + 512) = y1;
+            if (kSent) top = max(top, max(magnitude(y0), magnitude(y1)));
           }
         };
         if (two) step(std::true_type{});
         else step(std::false_type{});
+        if (kSent) note(top, c + 1);
         send(c);
         tc_fence_before();
         arrive_on(bKvFree);
