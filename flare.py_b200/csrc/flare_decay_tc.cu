@@ -1022,22 +1022,24 @@ int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluste
 }
 
 // How a call is spread: the CTAs of a sequence (a cluster) and the segments of the token axis, whichever the times below say is
-// shortest.  Measured (us, 64 / 128 features): a chunk in a CTA 2.0 / 3.5; a chunk's step of the state from CTA to CTA 0.65 /
-// 1.25, which bounds what a cluster gains on a long sequence (clusters of eight on 32 or more are not worth having); a chunk's
-// sum 0.6 / 0.8; the ends of a launch 7.  E.g. B = 1, H = 8, N = 65536, D = 64: 902 us with one CTA a head, 465, 352 and 271 in
-// clusters of 2, 4 and 8; B = 4, H = 16, N = 8192, D = 64: 128 us, 82 in clusters of 2, 125 in two segments.
+// shortest.  Measured (us, 64 / 128 features): a chunk in a CTA 1.9 / 3.0; a chunk's step of the state from CTA to CTA 0.65 /
+// 1.2, which bounds what a cluster gains on a long sequence; a chunk's sum 0.7 / 1.1; the ends of a launch 7.  Clusters of four
+// and eight do not fill every GPC: 33 and 15 of them fit 148 SMs, and one more costs a second round (97 against 72 us for 36
+// sequences of 8192 tokens).  E.g. D = 64: B = 4, H = 8, N = 8192 55 us in clusters of four, 71 of two, 73 in four segments;
+// H = 16 79 us in clusters of two, 106 of four, 124 in two segments; B = 1, H = 8, N = 65536 109 us in 18 segments, 117 in
+// nine of clusters of two.  Over 28 shapes from 200 to 131077 tokens the choice is within 1 % of the best of all on average.
 struct Spread { int cluster, segments; };
 Spread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
   const long long seqs = (long long)B * H * ((Dc + 63) / 64) * n_units;
   const int chunks = (int)(((long long)N + kL - 1) / kL), sms = num_sms();
   const bool wide = Da > 64;
-  const float chunk = wide ? 3.5f : 2.f, step = wide ? 1.25f : 0.65f, sum = wide ? 0.8f : 0.6f, ends = 7.f;
+  const float chunk = wide ? 3.f : 1.9f, step = wide ? 1.2f : 0.65f, sum = wide ? 1.1f : 0.7f, ends = 7.f;
   auto waves = [&](long long ctas, int room) { return (float)((ctas + room - 1) / room); };
   Spread best = {1, 1};
   float least = 1e30f;
   for (int c = 1; c <= 8; c *= 2) {
     if (c > chunks) break;
-    const int room = c == 8 ? sms * 3 / 4 : sms / c * c;     // clusters of eight do not fill the GPCs
+    const int room = (c == 8 ? sms * 5 / 6 : c == 4 ? sms * 9 / 10 : sms) / c * c;
     const long long full = sms / (seqs * c);                 // segments that fill the GPU once
     for (int k = 0; k < 4; ++k) {
       long long s = k == 0 ? 1 : k == 1 ? full / 2 : k == 2 ? full : 2 * full;
