@@ -13,7 +13,7 @@ taken as they are); Dk, Dv up to 256.  ``log_decay``: [H], a constant of the mod
 decay, -inf leaves a token itself alone.  ``lengths``: int32 (or int64) [B]; tokens at or behind ``lengths[b]`` -- padding,
 which may hold anything -- leave the state alone and have outputs and gradients of zero.  A value that is not finite among the
 live tokens spoils the outputs of the 128-token chunk it stands in, also those before it.  fp16: the products q . k have to
-stay within fp16's range (the scale is applied behind them).
+stay within fp16's range, in the backward dy . v too (the scale is applied behind them).
 """
 from __future__ import annotations
 
@@ -43,7 +43,10 @@ def decay_linear(q, k, v, log_decay, scale: float = 1.0, lengths=None):
 
 
 def decay_linear_prefill(q, k, v, log_decay, scale: float = 1.0, state=None, lengths=None):
-    """(y [B,H,N,Dv], state after the last live token) from ``state`` (None: empty), which is left as it is.  Forward only."""
+    """(y [B,H,N,Dv], state after the last live token) from ``state`` (None: empty), which is left as it is.  Forward only.
+
+    The state is as exact as sums in 32 bits for values of like size along a sequence.  Padding belongs into ``lengths``: behind
+    tokens that were silenced by zeros in k instead, a 16-bit call keeps less of what came before them."""
     q, k, v = _autocast(q, k, v)
     return native.decay_prefill(q, k, v, log_decay, float(scale), state, lengths)
 
