@@ -442,7 +442,7 @@ template <int DK> struct WalkPlan {
 
 template <typename T, int DK, bool STATE>
 __global__ void __launch_bounds__(WalkPlan<DK>::kThreads, 1)
-k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ DecayArgs a, int* status) {
+k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ DecayArgs a, int first, int per_unit, int* status) {
   grid_dep_sync();
   using L = WalkPlan<DK>;
   constexpr int F = Op16<T>::kFmt, CB = L::kCB;
@@ -458,9 +458,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   float* sExp = reinterpret_cast<float*>(bars + 28);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 30);   // [2][4], fp16 of 64 features
 
-  const DecayUnit& u = a.u[blockIdx.z];
-  const int n_cb = (u.Dc + 63) / 64, size = cluster_size(), rank = cluster_rank();
-  const int sequence = blockIdx.x / size, bh = sequence % (a.B * a.H), cb = sequence / (a.B * a.H), seg = blockIdx.y;
+  const int size = cluster_size(), rank = cluster_rank(), job = first + blockIdx.x / size;
+  const int unit = __reduce_max_sync(0xffffffffu, job / per_unit);       // in a uniform register: it indexes the arguments
+  const DecayUnit& u = a.u[unit];
+  const int n_cb = (u.Dc + 63) / 64, sequence = job - unit * per_unit, bh = sequence % (a.B * a.H), cb = sequence / (a.B * a.H), seg = blockIdx.y;
   if (cb >= n_cb) return;                          // the whole cluster alike
   const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -482,14 +483,14 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   auto load = [&](uint8_t* tiles, uint64_t* full, int which, int blocks, int col, int i) {
     for (int k = 0; k < blocks; ++k) tma_load_4d(tiles + k * kBlk, &maps.in[which], full, col + 64 * k, sp.first(chunk(i)), h, b);
   };
-  auto load_a = [&](int i, int at) { load(smem + L::oA + at * (CB * kBlk), bFull + at, maps.ia[blockIdx.z], CB, 0, i); };
+  auto load_a = [&](int i, int at) { load(smem + L::oA + at * (CB * kBlk), bFull + at, maps.ia[unit], CB, 0, i); };
   auto load_b = [&](int i, int at, int at_a) {
     mbar_expect_tx(bFull + at_a, 2 * CB * kBlk);
-    load(smem + L::oB + at * (CB * kBlk), bFull + at_a, maps.ib[blockIdx.z], CB, 0, i);
+    load(smem + L::oB + at * (CB * kBlk), bFull + at_a, maps.ib[unit], CB, 0, i);
   };
   auto load_c = [&](int i, int at) {
     mbar_expect_tx(bFullC + at, kBlk);
-    load(smem + L::oC + at * kBlk, bFullC + at, maps.ic[blockIdx.z], 1, c0, i);
+    load(smem + L::oC + at * kBlk, bFullC + at, maps.ic[unit], 1, c0, i);
   };
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFree + i, 2); }     // bFree: A X and P C
@@ -507,7 +508,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, L::kXPart);
   }
   if (warp == 1) tmem_alloc<512>(tmem_slot);
-  if (L::kStage && tid == 64) prefetch_tmap(&maps.out[blockIdx.z]);
+  if (L::kStage && tid == 64) prefetch_tmap(&maps.out[unit]);
   tc_fence_before();
   cluster_sync();                                  // every CTA's barriers stand before a state is sent
   tc_fence_after();
@@ -633,10 +634,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             if (i + 3 < n) {                       // with so few tiles their way is waited for: it starts in L2
               const int t0 = sp.first(chunk(i + 3));
               for (int k = 0; k < CB; ++k) {
-                tma_prefetch_4d(&maps.in[maps.ib[blockIdx.z]], 64 * k, t0, h, b);
-                tma_prefetch_4d(&maps.in[maps.ia[blockIdx.z]], 64 * k, t0, h, b);
+                tma_prefetch_4d(&maps.in[maps.ib[unit]], 64 * k, t0, h, b);
+                tma_prefetch_4d(&maps.in[maps.ia[unit]], 64 * k, t0, h, b);
               }
-              tma_prefetch_4d(&maps.in[maps.ic[blockIdx.z]], c0, t0, h, b);
+              tma_prefetch_4d(&maps.in[maps.ic[unit]], c0, t0, h, b);
             }
           }
           __syncwarp();
@@ -711,7 +712,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if constexpr (L::kStage) {
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0 && tok0 + 32 * w < a.N) tma_store_4d(&maps.out[blockIdx.z], tile, c0, tok0 + 32 * w, h, b);      // clipped at N and the last column
+        if (lane == 0 && tok0 + 32 * w < a.N) tma_store_4d(&maps.out[unit], tile, c0, tok0 + 32 * w, h, b);      // clipped at N and the last column
       }
     }
     // chunks of the segment that no live token is in: zeros
@@ -1013,7 +1014,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   if (warp == 1) tmem_dealloc<512>(tmem);
 }
 
-int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, const DecayMaps& maps, const DecayArgs& a, int* status) {
+int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, const DecayMaps& maps, const DecayArgs& a, int first,
+                int per_unit, int* status) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid; cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -1022,46 +1024,60 @@ int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluste
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = 2;
-  void* args[] = {const_cast<DecayMaps*>(&maps), const_cast<DecayArgs*>(&a), &status};
+  void* args[] = {const_cast<DecayMaps*>(&maps), const_cast<DecayArgs*>(&a), &first, &per_unit, &status};
   return cudaLaunchKernelExC(&cfg, kernel, args) == cudaSuccess ? FLARE_OK : FLARE_ECUDA;
 }
 
 // How a call is spread: the CTAs of a sequence (a cluster) and the segments of the token axis, whichever the times below say is
 // shortest.  Measured (us, 64 / 128 features): a chunk in a CTA 1.9 / 3.0; a chunk's step of the state from CTA to CTA 0.65 /
-// 1.2, which bounds what a cluster gains on a long sequence; a chunk's sum 0.7 / 1.1; the ends of a launch 7.  Clusters of four
-// and eight do not fill every GPC: 33 and 15 of them fit 148 SMs, and one more costs a second round (97 against 72 us for 36
-// sequences of 8192 tokens).  E.g. D = 64: B = 4, H = 8, N = 8192 55 us in clusters of four, 71 of two, 73 in four segments;
+// 1.2, which bounds what a cluster gains on a long sequence; a chunk's sum 0.7 / 1.1; the ends of a launch 7.  Clusters of
+// three, four and eight do not fill every GPC: 45, 33 and 15 of them fit 148 SMs, and one more costs a second round (97 us in 36
+// clusters of four, 72 in 36 of two, at 8192 tokens).  E.g. D = 64: B = 4, H = 8, N = 8192 55 us in clusters of four, 71 of two, 73 in four segments;
 // H = 16 79 us in clusters of two, 106 of four, 124 in two segments; B = 1, H = 8, N = 65536 109 us in 18 segments, 117 in
 // nine of clusters of two.  Over 28 shapes from 200 to 131077 tokens the choice is within 1 % of the best of all on average.
-struct Spread { int cluster, segments; };
+// Where the last round of a launch would leave most SMs idle, the sequences in it are launched by themselves, in clusters that use
+// more of them: the backward of B = 4, H = 16, N = 8192, D = 64 takes 148 sequences
+// one to a CTA and 44 in clusters of three: 182 us, where 192 clusters of two took 194.
+struct Spread { int cluster, segments, rest, rest_cluster; };
 Spread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
   const long long seqs = (long long)B * H * ((Dc + 63) / 64) * n_units;
   const int chunks = (int)(((long long)N + kL - 1) / kL), sms = num_sms();
   const bool wide = Da > 64;
   const float chunk = wide ? 3.f : 1.9f, step = wide ? 1.2f : 0.65f, sum = wide ? 1.1f : 0.7f, ends = 7.f;
-  auto waves = [&](long long ctas, int room) { return (float)((ctas + room - 1) / room); };
-  Spread best = {1, 1};
+  constexpr int kSizes[] = {1, 2, 3, 4, 8};
+  auto room = [&](int c) { return (c == 8 ? sms * 5 / 6 : c == 4 ? sms * 9 / 10 : c == 3 ? sms * 11 / 12 : sms) / c; };      // clusters that fit
+  auto rounds = [&](long long n, int fit) { return (float)((n + fit - 1) / fit); };
+  auto round = [&](int c, int len) {               // a round of sequences of so many chunks
+    const int own = (len + c - 1) / c;
+    return (c > 1 && len * step > own * chunk ? len * step : own * chunk) + ends;
+  };
+  Spread best = {1, 1, 0, 1};
   float least = 1e30f;
-  for (int c = 1; c <= 8; c *= 2) {
+  auto consider = [&](float t, const Spread& s) {
+    if (t < least) { least = t; best = s; }
+  };
+  for (int c : kSizes) {
     if (c > chunks) break;
-    const int room = (c == 8 ? sms * 5 / 6 : c == 4 ? sms * 9 / 10 : sms) / c * c;
     const long long full = sms / (seqs * c);                 // segments that fill the GPU once
     for (int k = 0; k < 4; ++k) {
       long long s = k == 0 ? 1 : k == 1 ? full / 2 : k == 2 ? full : 2 * full;
       if (s > chunks / (2 * c)) s = chunks / (2 * c);
       if (s > 256) s = 256;
       if (s < 1) s = 1;
-      const int len = (int)((chunks + s - 1) / s), own = (len + c - 1) / c;
-      float t = waves(seqs * c * s, room) * ((c > 1 && len * step > own * chunk ? len * step : own * chunk) + ends);
-      if (s > 1) t += waves(seqs * (s - 1), sms) * (len * sum + ends) + 4.f;
-      if (t < least) { least = t; best = {c, (int)s}; }
+      const int len = (int)((chunks + s - 1) / s);
+      float t = rounds(seqs * s, room(c)) * round(c, len);
+      if (s > 1) t += rounds(seqs * (s - 1), sms) * (len * sum + ends) + 4.f;
+      consider(t, {c, (int)s, 0, 1});
     }
+    const long long whole = seqs / room(c), rest = seqs - whole * room(c);
+    for (int r : kSizes)
+      if (whole > 0 && rest > 0 && r <= chunks) consider(whole * round(c, chunks) + rounds(rest, room(r)) * round(r, chunks) + 3.f, {c, 1, (int)rest, r});
   }
   return best;
 }
 
 template <typename T, int DK>
-int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, int cluster, cudaStream_t st) {
+int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, const Spread& spread, cudaStream_t st) {
   using W = WalkPlan<DK>;
   using S = SumPlan<DK>;
   int* status = tc_status_ptr();
@@ -1075,7 +1091,12 @@ int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, int cluster, c
     launch_dep(k_decay_tc_sums<T, DK>, dim3(seqs, (unsigned)a.n_seg - 1, (unsigned)a.n_units), dim3(S::kThreads), S::kBytes, st, maps, a, status);
     launch_decay_prefix(a, st);
   }
-  return launch_walk(walk, dim3(seqs * cluster, (unsigned)a.n_seg, (unsigned)a.n_units), W::kThreads, W::kBytes, cluster, st, maps, a, status);
+  const unsigned jobs = seqs * (unsigned)a.n_units, rest = (unsigned)spread.rest;
+  int rc = launch_walk(walk, dim3((jobs - rest) * spread.cluster, (unsigned)a.n_seg), W::kThreads, W::kBytes, spread.cluster, st, maps, a, 0, (int)seqs, status);
+  if (rc == FLARE_OK && rest)
+    rc = launch_walk(walk, dim3(rest * spread.rest_cluster, (unsigned)a.n_seg), W::kThreads, W::kBytes, spread.rest_cluster, st, maps, a, (int)(jobs - rest), (int)seqs,
+                     status);
+  return rc;
 }
 
 }  // namespace
@@ -1133,9 +1154,9 @@ int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
     maps.ic[i] = map_of(u.c, u.cs, u.Dc, order[i][2]);
     if (maps.ia[i] < 0 || maps.ib[i] < 0 || maps.ic[i] < 0) return FLARE_EUNSUPPORTED;
   }
-  const int cluster = pick_spread(a.B, a.H, a.N, Da, Dc, a.n_units).cluster;
-  if (dtype == FLARE_BF16) return Da <= 64 ? launch_all<__nv_bfloat16, 64>(maps, a, Dc, cluster, st) : launch_all<__nv_bfloat16, 128>(maps, a, Dc, cluster, st);
-  return Da <= 64 ? launch_all<__half, 64>(maps, a, Dc, cluster, st) : launch_all<__half, 128>(maps, a, Dc, cluster, st);
+  const Spread spread = pick_spread(a.B, a.H, a.N, Da, Dc, a.n_units);
+  if (dtype == FLARE_BF16) return Da <= 64 ? launch_all<__nv_bfloat16, 64>(maps, a, Dc, spread, st) : launch_all<__nv_bfloat16, 128>(maps, a, Dc, spread, st);
+  return Da <= 64 ? launch_all<__half, 64>(maps, a, Dc, spread, st) : launch_all<__half, 128>(maps, a, Dc, spread, st);
 }
 
 }  // namespace flare

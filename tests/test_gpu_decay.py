@@ -147,6 +147,49 @@ def test_long_sequences_in_clusters_and_segments(fb, cuda_dev, shape, dtype):
     assert fb.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(10, 16, 700, 64, 64), (4, 16, 700, 64, 64), (5, 9, 1100, 64, 64), (5, 3, 1100, 64, 64), (2, 13, 1300, 128, 128)])
+def test_sequences_that_do_not_fill_their_last_round(fb, cuda_dev, shape, dtype):
+    """More sequences than SMs, or a few less than a multiple: the ones of the last round are spread over more CTAs."""
+    B, H, N, Dk, Dv = shape
+    q, k, v, ld = make(cuda_dev, *shape, dtype, seed=B * H)
+    lengths = torch.tensor([N - 150 * b for b in range(B - 1)] + [N], device=cuda_dev).clamp(min=0)
+    state = torch.randn(B, H, Dk, Dv, device=cuda_dev)
+    y, end = fb.decay_linear_prefill(q, k, v, ld, 0.1, state=state, lengths=lengths)
+    y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld, 0.1, state, lengths)
+    assert rel(y, y_ref) <= tol_y(dtype) and rel(end, end_ref) <= tol_state(dtype)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    dy = torch.randn_like(v)
+    got = torch.autograd.grad(fb.decay_linear(*leaves, ld, 0.1, lengths), leaves, dy)
+    for b in range(0, B, 3):                         # an entry at a time: the definition is N x N
+        one = [t[b:b + 1].detach().double().requires_grad_(True) for t in (q, k, v)]
+        want = torch.autograd.grad(O.decay_linear_dense(*one, ld, 0.1, lengths[b:b + 1]), one, dy[b:b + 1].double())
+        for g, w in zip(got, want):
+            assert rel(g[b:b + 1], w) <= tol_y(dtype)
+    assert fb.device_status() == 0
+
+
+@pytest.mark.parametrize("N", [300, 2100])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_states_keep_the_bits_of_sums_in_fp32(fb, cuda_dev, dtype, D, N):
+    """Decays on both sides of every border at which the number of 16-bit terms changes.  What the terms leave (bf16): beside
+    B^T C itself 2^-18 of 0.24; where a chunk counts for 2^-3 or less 2^-18 of that, for 2^-13 or less 2^-9 of that: together below
+    2e-6; the sums in fp32 sqrt(N) * 2^-24."""
+    rates = [0.0, 1e-4, 1e-3, 2.1e-3, 2.2e-3, 4e-3, 1e-2, 0.05, 0.3, 3.0]
+    H = len(rates)
+    q, k, v, _ = make(cuda_dev, 1, H, N, D, D, dtype, seed=N + D)
+    ld = -torch.tensor(rates, device=cuda_dev)
+    end = fb.decay_linear_prefill(q, k, v, ld)[1]
+    ref = O.decay_linear_recurrent(q, k, v, ld)[1]
+    half = N // 2 + 3                                # the same in two calls
+    first = fb.decay_linear_prefill(q[:, :, :half], k[:, :, :half], v[:, :, :half], ld)[1]
+    second = fb.decay_linear_prefill(q[:, :, half:], k[:, :, half:], v[:, :, half:], ld, state=first)[1]
+    for h in range(H):
+        assert rel(end[:, h], ref[:, h]) <= 2e-6 + N ** 0.5 * 2.0 ** -24
+        assert rel(second[:, h], ref[:, h]) <= 2e-6 + N ** 0.5 * 2.0 ** -24
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_offsets_that_pass_32_bits(fb, cuda_dev, dtype):
     B, H, N, D = 2, 2, 140, 64
