@@ -217,11 +217,11 @@ __device__ __forceinline__ int terms_of(float g2, int behind) {
 template <typename T>
 __device__ __forceinline__ bool near_one(float g2) { return Op16<T>::kFmt == 1 && fabsf(g2) <= 0.4f / kL; }
 
-// C weighted by the decay to the chunk's end; a thread takes PIECES of the eight 16-byte pieces of a row.  `which` of its terms
-// are written, bit by bit: 1, 2 and 4 for the first, second and third, to w_t and the tiles behind it, but the third alone to w_t.
-// Rows behind the length are cleared, here and in the tiles of b and c themselves.
+// C weighted by the decay to the chunk's end; a thread takes PIECES of the 16-byte pieces of a row, and of those the first `pieces`
+// hold columns.  `which` of its terms are written, bit by bit: 1, 2 and 4 for the first, second and third, to w_t and the tiles
+// behind it, but the third alone to w_t.  Rows behind the length are cleared, here and in the tiles of b and c themselves.
 template <typename T, int CB, int PIECES = 8>
-__device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, int which, uint8_t* src, uint8_t* w_t, uint8_t* b_t) {
+__device__ __forceinline__ void weigh_c(int r, int p0, int pieces, int cnt, float w, int which, uint8_t* src, uint8_t* w_t, uint8_t* b_t) {
   const uint32_t row = 128 * r + 16 * (r & 7);     // 16-byte piece ch of the swizzled row: row ^ 16 ch
   const F2 w2 = both(w);
   if (r >= cnt) {
@@ -240,7 +240,7 @@ __device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, int whi
   } else if (which == 1) {
     auto weighed = [&](uint32_t x) { return pack2<T>(mul2(unpack2<T>(x), w2)); };
 #pragma unroll 4
-    for (int ch = p0; ch < p0 + PIECES; ++ch) {
+    for (int ch = p0; ch < p0 + pieces; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       *reinterpret_cast<uint4*>(w_t + at) = make_uint4(weighed(x.x), weighed(x.y), weighed(x.z), weighed(x.w));
@@ -249,7 +249,7 @@ __device__ __forceinline__ void weigh_c(int r, int p0, int cnt, float w, int whi
     const F2 minus_one = both(-1.f);
     uint8_t* third = w_t + (which == 7 ? 2 * kBlk : 0);
 #pragma unroll 2
-    for (int ch = p0; ch < p0 + PIECES; ++ch) {
+    for (int ch = p0; ch < p0 + pieces; ++ch) {
       const uint32_t at = row ^ (16 * ch);
       const uint4 x = *reinterpret_cast<const uint4*>(src + at);
       uint4 t0, t1;
@@ -411,7 +411,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       const int t = terms(c);
-      weigh_c<T, CB, 4>(r, 4 * half, cnt, t == 2 && plus ? w - 1.f : w, (1 << t) - 1, smem + L::oC + ring.at * kBlk, smem + L::oW + (c & 1) * (3 * kBlk),
+      weigh_c<T, CB, 4>(r, 4 * half, 4, cnt, t == 2 && plus ? w - 1.f : w, (1 << t) - 1, smem + L::oC + ring.at * kBlk, smem + L::oW + (c & 1) * (3 * kBlk),
                         smem + L::oB + ring.at * (CB * kBlk));
       arrive_on(bW + (c & 1));
       ring.next();
@@ -432,7 +432,7 @@ template <int DK> struct WalkPlan {
   static constexpr int kW = 2;                     // tiles for the weighted C: two terms at a time, or two chunks of one
   static constexpr bool kStage = DK == 64;         // outputs leave through shared memory and the TMA
   static constexpr int kXTile = DK * 128;          // one term of the packed state: [DK][64]
-  static constexpr int kXPart = DK * 64 + 16;      // a warp's quarter of the state in fp32, as it arrives, and its largest magnitude
+  static constexpr int kXPart = 16 + DK * 64;      // a warp's quarter of the state in fp32, as it arrives, behind its largest magnitude
   static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + kW * kBlk,
                        oOut = oX + 2 * kXTile, oIn = oOut + (kStage ? kBlk : 0), oBars = oIn + 4 * kXPart;
   static constexpr int kBytes = oBars + 512 + 1024;
@@ -465,6 +465,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   if (cb >= n_cb) return;                          // the whole cluster alike
   const int b = bh / a.H, h = bh % a.H, c0 = 64 * cb;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  // Columns that exist: with 128 features the roles leave the others out (half of the state's step where Dv is 32), and what is in
+  // them is never stored.  With 64 the state's threads take all theirs at once.
+  const int width = DK == 128 ? min(64, u.Dc - c0) : 64;
+  const int part = DK == 128 ? 16 + 128 * width : L::kXPart;           // bytes of the state that a warp sends
   const int live = decay_live(a, b);
   const bool rev = u.rev != 0;
   const Span sp(a, live, seg, rev);
@@ -505,7 +509,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if (i >= 2) break;
     }
     if (size > 1 && mine > (rank == 0 ? 1 : 0))                           // the first state that comes from another CTA
-      for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, L::kXPart);
+      for (int i = 0; i < 4; ++i) mbar_expect_tx(bIn + i, part);
   }
   if (warp == 1) tmem_alloc<512>(tmem_slot);
   if (L::kStage && tid == 64) prefetch_tmap(&maps.out[unit]);
@@ -680,7 +684,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       tmem_ld16(y_at, y);
       tmem_ld16(x_at, x);
 #pragma unroll 1
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; 16 * k < width; ++k) {
         uint32_t q[8];
         tmem_wait_ld();
 #pragma unroll
@@ -689,7 +693,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           if constexpr (kHalfRange) in_chunk = mul2(scale2, in_chunk);
           q[m] = pack2<T>(fma2(fx, floats(x[2 * m], x[2 * m + 1]), in_chunk));
         }
-        if (k < 3) {
+        if (16 * (k + 1) < width) {
           tmem_ld16(y_at + 16 * (k + 1), y);
           tmem_ld16(x_at + 16 * (k + 1), x);
         } else {
@@ -734,7 +738,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     constexpr int NC = DK == 128 ? 64 : 32;        // columns of a thread
     const int r = tid - 32 * L::kWarpX, w = warp & 3, d = r & (DK - 1), col = DK == 128 ? 0 : 32 * (r >> 6);
     const uint32_t kv = tmem + ((uint32_t)(w * 32) << 16) + L::cKv + col;
-    uint8_t* in = smem + L::oIn + w * L::kXPart + 16 * lane;
+    uint8_t* in = smem + L::oIn + w * L::kXPart + 16 + 16 * lane;
     const long long own = (long long)d * u.Dc + c0 + col;
     const int cols = d < u.Da ? u.Dc - c0 - col : 0;         // of this thread's columns, those that exist
     auto magnitude = [](const float4& x) {
@@ -745,12 +749,12 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     constexpr bool kSent = kHalfRange && DK == 128;
     auto note = [&](uint32_t top, int c) {
       top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) *reinterpret_cast<uint32_t*>(in + L::kXPart - 16 + 4 * (c & 1)) = top;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(in - 16 + 4 * (c & 1)) = top;
     };
     auto noted = [&](int c) {
       uint32_t top = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) top = max(top, *reinterpret_cast<const uint32_t*>(smem + L::oIn + (i + 1) * L::kXPart - 16 + 4 * (c & 1)));
+      for (int i = 0; i < 4; ++i) top = max(top, *reinterpret_cast<const uint32_t*>(smem + L::oIn + i * L::kXPart + 4 * (c & 1)));
       return top;
     };
     if (rank == 0) {
@@ -800,13 +804,13 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       __syncwarp();
       if (lane == 0) {
         const uint32_t next = (rank + 1) % size, at = smem_u32(smem + L::oIn + w * L::kXPart);
-        copy_to_cta(remote(at, next), at, L::kXPart, remote(smem_u32(bIn + w), next));
+        copy_to_cta(remote(at, next), at, part, remote(smem_u32(bIn + w), next));
       }
     };
     auto receive = [&](int i, int c) {
       if (size == 1 || c == 0) return;
       for (int k = kSent ? 0 : w; k < (kSent ? 4 : w + 1); ++k) wait(bIn + k, rank == 0 ? i - 1 : i);
-      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, L::kXPart);
+      if (lane == 0 && i + 1 < mine) mbar_expect_tx(bIn + w, part);
     };
     int ev = 0;
     for (int i = 0; i < mine; ++i, ++ev) {
@@ -869,7 +873,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         uint32_t top = 0;
         auto step = [&](auto more) {               // a loop of its own for each number of terms: it is short, and waited for
 #pragma unroll 2
-          for (int j = 0; j < NC; j += 8) {
+          for (int j = 0; j < width; j += 8) {
             uint32_t h[8], l[8];
             tmem_ld8(kv + j, h);
             if constexpr (more.value) tmem_ld8(kv + 64 + j, l);
@@ -924,7 +928,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         const int back = t > 1 || before > 1 ? 1 : 2;
         if (leader && ev >= back) wait(bEv + ((ev - back) & 1), (ev - back) >> 1);
         asm volatile("bar.sync 3, 128;" ::: "memory");
-        weigh_c<T, CB>(r, 0, cnt, plus && t == 2 ? w - 1.f : w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
+        weigh_c<T, CB>(r, 0, width / 8, cnt, plus && t == 2 ? w - 1.f : w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
                        smem + L::oB + rb.at * (CB * kBlk));
         arrive_on(bW + (ev & 1));
         before = t;
