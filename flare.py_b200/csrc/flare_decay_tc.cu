@@ -1040,8 +1040,9 @@ int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluste
 // H = 16 79 us in clusters of two, 106 of four, 124 in two segments; B = 1, H = 8, N = 65536 109 us in 18 segments, 117 in
 // nine of clusters of two.  Over 28 shapes from 200 to 131077 tokens the choice is within 1 % of the best of all on average.
 // Where the last round of a launch would leave most SMs idle, the sequences in it are launched by themselves, in clusters that use
-// more of them: the backward of B = 4, H = 16, N = 8192, D = 64 takes 148 sequences
-// one to a CTA and 44 in clusters of three: 182 us, where 192 clusters of two took 194.
+// more of them: the backward of B = 4, H = 16, N = 8192, D = 64 takes 148 sequences one to a CTA and 44 in clusters of three:
+// 182 us, where 192 clusters of two took 194.  Behind another launch the last of the clusters that fit did not find its place:
+// 45 of three took 208 us.
 struct Spread { int cluster, segments, rest, rest_cluster; };
 Spread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
   const long long seqs = (long long)B * H * ((Dc + 63) / 64) * n_units;
@@ -1075,7 +1076,8 @@ Spread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
     }
     const long long whole = seqs / room(c), rest = seqs - whole * room(c);
     for (int r : kSizes)
-      if (whole > 0 && rest > 0 && r <= chunks) consider(whole * round(c, chunks) + rounds(rest, room(r)) * round(r, chunks) + 3.f, {c, 1, (int)rest, r});
+      if (whole > 0 && rest > 0 && r <= chunks)
+        consider(whole * round(c, chunks) + rounds(rest, room(r) - (r > 2)) * round(r, chunks) + 3.f, {c, 1, (int)rest, r});
   }
   return best;
 }
