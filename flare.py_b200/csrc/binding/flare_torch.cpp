@@ -314,7 +314,7 @@ struct Decay {
     for (int i = 0; i < 4; ++i)
       if (k_.size(i) > INT32_MAX) raise_py(PyExc_ValueError, "a dimension exceeds 32 bits");
     q = decay_rows(q_); k = decay_rows(k_); v = decay_rows(v_);
-    log_decay = ld.to(at::kFloat).contiguous();
+    log_decay = ld.scalar_type() == at::kFloat && ld.is_contiguous() ? ld : ld.to(at::kFloat).contiguous();
     p.B = (int32_t)k.size(0); p.H = (int32_t)k.size(1); p.N = (int32_t)k.size(2); p.Dk = (int32_t)k.size(3); p.Dv = (int32_t)v.size(3);
     p.dtype = dtype_code(k);
     p.scale = (float)scale;
@@ -341,9 +341,9 @@ Tensor decay_run(Decay& d, const float* state_in, float* state_out) {
   Tensor y = like_tokens(d.v);
   set_stride(d.p.y_stride, y);
   const size_t bytes = flare_decay_workspace_bytes(&d.p);
-  const Tensor ws = scratch(bytes, d.k);
+  const Tensor ws = bytes ? scratch(bytes, d.k) : Tensor();
   check_rc(flare_decay_fwd(&d.p, d.q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), fp(d.log_decay), d.len(), y.data_ptr(), state_in,
-                           state_out, fp(ws), bytes, stream_of(d.k)), "flare_decay_fwd");
+                           state_out, bytes ? fp(ws) : nullptr, bytes, stream_of(d.k)), "flare_decay_fwd");
   return y;
 }
 
@@ -365,9 +365,9 @@ Three decay_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   if (d.empty()) return {dq, dk, dv};
   set_stride(d.p.dy_stride, dy); set_stride(d.p.dq_stride, dq); set_stride(d.p.dk_stride, dk); set_stride(d.p.dv_stride, dv);
   const size_t bytes = flare_decay_bwd_workspace_bytes(&d.p);
-  const Tensor ws = scratch(bytes, k);
+  const Tensor ws = bytes ? scratch(bytes, k) : Tensor();
   check_rc(flare_decay_bwd(&d.p, d.q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), dy.data_ptr(), fp(d.log_decay), d.len(),
-                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), fp(ws), bytes, stream_of(k)), "flare_decay_bwd");
+                           dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), bytes ? fp(ws) : nullptr, bytes, stream_of(k)), "flare_decay_bwd");
   return {dq, dk, dv};
 }
 
@@ -379,7 +379,7 @@ Two decay_prefill(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   Tensor before;
   if (state.has_value()) {
     need_cuda(*state);
-    before = state->contiguous();
+    before = state->is_contiguous() ? *state : state->contiguous();
     d.check_state(before);
   }
   if (d.empty()) {

@@ -57,9 +57,12 @@ struct DecayStep {
   __device__ __forceinline__ float operator()(float s) const { return fmaf(mul, s, keep * s); }
 };
 
+// How the tensor-core kernels spread a call: the CTAs of a sequence (a cluster), the segments of the token axis, and the sequences
+// of the last round, if they are launched by themselves.
+struct DecaySpread { int cluster, segments, rest, rest_cluster; };
 bool decay_tc_supported(const DecayArgs& a, int dtype);
-int decay_tc_segments(int B, int H, int N, int Da, int Dc, int n_units);
-int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st);
+DecaySpread decay_tc_spread(int B, int H, int N, int Da, int Dc, int n_units);
+int decay_tc(const DecayArgs& a, int dtype, const DecaySpread& spread, cudaStream_t st);
 // the sums of the segments into the states before them, in place; reads state_in
 void launch_decay_prefix(const DecayArgs& a, cudaStream_t st);
 

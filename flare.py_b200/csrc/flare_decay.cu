@@ -573,32 +573,34 @@ DecayUnit unit(const void* x, const int64_t* xs, const void* y, const int64_t* y
   return u;
 }
 
-// Segments and workspace follow from the sizes alone, for either family, so that the size asked for fits both.
-int seg_max(const FlareDecay* p, int units) {
-  const int D = p->Dk > p->Dv ? p->Dk : p->Dv;
-  int s = pick_segments(p->B, p->H, p->N, units == 1 ? p->Dv : D, units);
-  const int t = decay_tc_segments(p->B, p->H, p->N, units == 1 ? p->Dk : D, units == 1 ? p->Dv : D, units);
-  return s > t ? s : t;
-}
-size_t ws_bytes(const FlareDecay* p, int units) {
-  const int s = seg_max(p, units);
-  return s > 1 ? (size_t)units * p->B * p->H * s * p->Dk * p->Dv * sizeof(float) : 0;
+// How a call is cut follows from its sizes alone, for either family, so that the workspace asked for fits both.
+struct Plan {
+  int simt_segments;
+  DecaySpread tc;
+  size_t bytes;
+};
+Plan plan_of(const FlareDecay* p, int units) {
+  const int D = p->Dk > p->Dv ? p->Dk : p->Dv, Da = units == 1 ? p->Dk : D, Dc = units == 1 ? p->Dv : D;
+  Plan plan = {pick_segments(p->B, p->H, p->N, Dc, units), decay_tc_spread(p->B, p->H, p->N, Da, Dc, units), 0};
+  const int s = plan.simt_segments > plan.tc.segments ? plan.simt_segments : plan.tc.segments;
+  if (s > 1) plan.bytes = (size_t)units * p->B * p->H * s * p->Dk * p->Dv * sizeof(float);
+  return plan;
 }
 
-int run(DecayArgs& a, const FlareDecay* p, float* ws, cudaStream_t st, const char* what) {
+int run(DecayArgs& a, const FlareDecay* p, const Plan& plan, float* ws, cudaStream_t st, const char* what) {
   int Da = 0, Dc = 0;
   for (int i = 0; i < a.n_units; ++i) {
     Da = a.u[i].Da > Da ? a.u[i].Da : Da;
     Dc = a.u[i].Dc > Dc ? a.u[i].Dc : Dc;
   }
   const bool tc = decay_tc_supported(a, p->dtype);
-  int n = tc ? decay_tc_segments(p->B, p->H, p->N, Da, Dc, a.n_units) : pick_segments(p->B, p->H, p->N, Dc, a.n_units);
+  const int n = tc ? plan.tc.segments : plan.simt_segments;
   const int block = tc ? 128 : kSub;
   a.seg_len = (int)((((long long)p->N + n - 1) / n + block - 1) / block) * block;
   a.n_seg = (p->N + a.seg_len - 1) / a.seg_len;
   for (int i = 0; i < a.n_units; ++i) a.u[i].seg = ws + (size_t)i * p->B * p->H * a.n_seg * p->Dk * p->Dv;
   int rc;
-  if (tc) rc = decay_tc(a, p->dtype, st);
+  if (tc) rc = decay_tc(a, p->dtype, plan.tc, st);
   else if (p->dtype == FLARE_F32) rc = run_simt<float>(a, Da, Dc, st);
   else if (p->dtype == FLARE_F16) rc = run_simt<__half>(a, Da, Dc, st);
   else rc = run_simt<__nv_bfloat16>(a, Da, Dc, st);
@@ -621,15 +623,16 @@ using namespace flare;
 
 extern "C" {
 
-size_t flare_decay_workspace_bytes(const FlareDecay* p) { return check_problem("decay", p) == FLARE_OK ? ws_bytes(p, 1) : 0; }
-size_t flare_decay_bwd_workspace_bytes(const FlareDecay* p) { return check_problem("decay_bwd", p) == FLARE_OK ? ws_bytes(p, 3) : 0; }
+size_t flare_decay_workspace_bytes(const FlareDecay* p) { return check_problem("decay", p) == FLARE_OK ? plan_of(p, 1).bytes : 0; }
+size_t flare_decay_bwd_workspace_bytes(const FlareDecay* p) { return check_problem("decay_bwd", p) == FLARE_OK ? plan_of(p, 3).bytes : 0; }
 
 int flare_decay_fwd(const FlareDecay* p, const void* q, const void* k, const void* v, const float* log_decay,
                     const int32_t* lengths, void* y, const float* state_in, float* state_out, float* workspace,
                     size_t workspace_bytes, flare_stream_t stream) {
   if (int rc = check_problem("decay", p)) return rc;
   if (!q || !k || !v || !y || !log_decay) return refuse(FLARE_EINVAL, "decay: null pointer");
-  const size_t need = ws_bytes(p, 1);
+  const Plan plan = plan_of(p, 1);
+  const size_t need = plan.bytes;
   if (need && (!workspace || workspace_bytes < need)) return refuse(FLARE_EWORKSPACE, "decay: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return refuse(FLARE_EALIGN, "decay: workspace must be 16-byte aligned");
   DecayArgs a = base_args(p, log_decay, lengths);
@@ -637,7 +640,7 @@ int flare_decay_fwd(const FlareDecay* p, const void* q, const void* k, const voi
   a.u[0] = unit(q, p->q_stride, k, p->k_stride, v, p->v_stride, y, p->y_stride, p->Dk, p->Dv, 0);
   a.u[0].state_in = state_in;
   a.u[0].state_out = state_out;
-  return run(a, p, workspace, static_cast<cudaStream_t>(stream), "decay");
+  return run(a, p, plan, workspace, static_cast<cudaStream_t>(stream), "decay");
 }
 
 int flare_decay_bwd(const FlareDecay* p, const void* q, const void* k, const void* v, const void* dy, const float* log_decay,
@@ -645,7 +648,8 @@ int flare_decay_bwd(const FlareDecay* p, const void* q, const void* k, const voi
                     flare_stream_t stream) {
   if (int rc = check_problem("decay_bwd", p)) return rc;
   if (!q || !k || !v || !dy || !dq || !dk || !dv || !log_decay) return refuse(FLARE_EINVAL, "decay_bwd: null pointer");
-  const size_t need = ws_bytes(p, 3);
+  const Plan plan = plan_of(p, 3);
+  const size_t need = plan.bytes;
   if (need && (!workspace || workspace_bytes < need)) return refuse(FLARE_EWORKSPACE, "decay_bwd: workspace of %zu bytes, %zu needed", workspace_bytes, need);
   if (reinterpret_cast<uintptr_t>(workspace) % 16) return refuse(FLARE_EALIGN, "decay_bwd: workspace must be 16-byte aligned");
   DecayArgs a = base_args(p, log_decay, lengths);
@@ -653,7 +657,7 @@ int flare_decay_bwd(const FlareDecay* p, const void* q, const void* k, const voi
   a.u[0] = unit(dy, p->dy_stride, v, p->v_stride, k, p->k_stride, dq, p->dq_stride, p->Dv, p->Dk, 0);
   a.u[1] = unit(v, p->v_stride, dy, p->dy_stride, q, p->q_stride, dk, p->dk_stride, p->Dv, p->Dk, 1);
   a.u[2] = unit(k, p->k_stride, q, p->q_stride, dy, p->dy_stride, dv, p->dv_stride, p->Dk, p->Dv, 1);
-  return run(a, p, workspace, static_cast<cudaStream_t>(stream), "decay_bwd");
+  return run(a, p, plan, workspace, static_cast<cudaStream_t>(stream), "decay_bwd");
 }
 
 int flare_decay_decode(const FlareDecay* p, const void* q, const void* k, const void* v, const float* log_decay,

@@ -1043,57 +1043,54 @@ int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluste
 // more of them: the backward of B = 4, H = 16, N = 8192, D = 64 takes 148 sequences one to a CTA and 44 in clusters of three:
 // 182 us, where 192 clusters of two took 194.  Behind another launch the last of the clusters that fit did not find its place:
 // 45 of three took 208 us.
-struct Spread { int cluster, segments, rest, rest_cluster; };
-Spread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
-  const long long seqs = (long long)B * H * ((Dc + 63) / 64) * n_units;
-  const int chunks = (int)(((long long)N + kL - 1) / kL), sms = num_sms();
+DecaySpread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
+  const int seqs = B * H * ((Dc + 63) / 64) * n_units;                 // 2^24 * 4 * 3 at most
+  const int chunks = (N + kL - 1) / kL, sms = num_sms();
   const bool wide = Da > 64;
   const float chunk = wide ? 3.f : 1.9f, step = wide ? 1.2f : 0.65f, sum = wide ? 1.1f : 0.7f, ends = 7.f;
   constexpr int kSizes[] = {1, 2, 3, 4, 8};
   auto room = [&](int c) { return (c == 8 ? sms * 5 / 6 : c == 4 ? sms * 9 / 10 : c == 3 ? sms * 11 / 12 : sms) / c; };      // clusters that fit
-  auto rounds = [&](long long n, int fit) { return (float)((n + fit - 1) / fit); };
+  auto rounds = [&](int n, int fit) { return (float)((n + fit - 1) / fit); };
   auto round = [&](int c, int len) {               // a round of sequences of so many chunks
     const int own = (len + c - 1) / c;
     return (c > 1 && len * step > own * chunk ? len * step : own * chunk) + ends;
   };
-  Spread best = {1, 1, 0, 1};
+  DecaySpread best = {1, 1, 0, 1};
   float least = 1e30f;
-  auto consider = [&](float t, const Spread& s) {
+  auto consider = [&](float t, const DecaySpread& s) {
     if (t < least) { least = t; best = s; }
   };
   for (int c : kSizes) {
     if (c > chunks) break;
-    const long long full = sms / (seqs * c);                 // segments that fill the GPU once
-    for (int k = 0; k < 4; ++k) {
-      long long s = k == 0 ? 1 : k == 1 ? full / 2 : k == 2 ? full : 2 * full;
-      if (s > chunks / (2 * c)) s = chunks / (2 * c);
+    const int fit = room(c), most = chunks / (2 * c), full = seqs <= sms ? sms / (seqs * c) : 0;       // full: segments that fill the GPU once
+    consider(rounds(seqs, fit) * round(c, chunks), {c, 1, 0, 1});
+    for (int k = 0; k < 3; ++k) {
+      int s = k == 0 ? full / 2 : k == 1 ? full : 2 * full;
+      s = s < most ? s : most;
+      if (s < 2) continue;
       if (s > 256) s = 256;
-      if (s < 1) s = 1;
-      const int len = (int)((chunks + s - 1) / s);
-      float t = rounds(seqs * s, room(c)) * round(c, len);
-      if (s > 1) t += rounds(seqs * (s - 1), sms) * (len * sum + ends) + 4.f;
-      consider(t, {c, (int)s, 0, 1});
+      const int len = (chunks + s - 1) / s;
+      consider(rounds(seqs * s, fit) * round(c, len) + rounds(seqs * (s - 1), sms) * (len * sum + ends) + 4.f, {c, s, 0, 1});
     }
-    const long long whole = seqs / room(c), rest = seqs - whole * room(c);
-    for (int r : kSizes)
-      if (whole > 0 && rest > 0 && r <= chunks)
-        consider(whole * round(c, chunks) + rounds(rest, room(r) - (r > 2)) * round(r, chunks) + 3.f, {c, 1, (int)rest, r});
+    const int whole = seqs / fit, rest = seqs - whole * fit;
+    if (whole > 0 && rest > 0)
+      for (int r : kSizes)
+        if (r <= chunks) consider(whole * round(c, chunks) + rounds(rest, room(r) - (r > 2)) * round(r, chunks) + 3.f, {c, 1, rest, r});
   }
   return best;
 }
 
 template <typename T, int DK>
-int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, const Spread& spread, cudaStream_t st) {
+int launch_all(const DecayMaps& maps, const DecayArgs& a, int Dc, const DecaySpread& spread, cudaStream_t st) {
   using W = WalkPlan<DK>;
   using S = SumPlan<DK>;
   int* status = tc_status_ptr();
   const void* walk = a.u[0].state_out ? reinterpret_cast<const void*>(&k_decay_tc_walk<T, DK, true>)
                                       : reinterpret_cast<const void*>(&k_decay_tc_walk<T, DK, false>);
-  if (tc_set_dyn_smem(walk, W::kBytes) != FLARE_OK ||
-      tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_tc_sums<T, DK>), S::kBytes) != FLARE_OK)
-    return FLARE_ECUDA;
+  if (tc_set_dyn_smem(walk, W::kBytes) != FLARE_OK) return FLARE_ECUDA;
   const unsigned seqs = (unsigned)(a.B * a.H * ((Dc + 63) / 64));
   if (a.n_seg > 1) {                               // the last segment walked needs no sum
+    if (tc_set_dyn_smem(reinterpret_cast<const void*>(&k_decay_tc_sums<T, DK>), S::kBytes) != FLARE_OK) return FLARE_ECUDA;
     launch_dep(k_decay_tc_sums<T, DK>, dim3(seqs, (unsigned)a.n_seg - 1, (unsigned)a.n_units), dim3(S::kThreads), S::kBytes, st, maps, a, status);
     launch_decay_prefix(a, st);
   }
@@ -1124,11 +1121,9 @@ bool decay_tc_supported(const DecayArgs& a, int dtype) {
   return true;
 }
 
-int decay_tc_segments(int B, int H, int N, int Da, int Dc, int n_units) {
-  return pick_spread(B, H, N, Da, Dc, n_units).segments;
-}
+DecaySpread decay_tc_spread(int B, int H, int N, int Da, int Dc, int n_units) { return pick_spread(B, H, N, Da, Dc, n_units); }
 
-int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
+int decay_tc(const DecayArgs& a, int dtype, const DecaySpread& spread, cudaStream_t st) {
   DecayMaps maps;
   const void* seen[4] = {};
   int n = 0, Da = 0, Dc = 0;
@@ -1160,7 +1155,6 @@ int decay_tc(const DecayArgs& a, int dtype, cudaStream_t st) {
     maps.ic[i] = map_of(u.c, u.cs, u.Dc, order[i][2]);
     if (maps.ia[i] < 0 || maps.ib[i] < 0 || maps.ic[i] < 0) return FLARE_EUNSUPPORTED;
   }
-  const Spread spread = pick_spread(a.B, a.H, a.N, Da, Dc, a.n_units);
   if (dtype == FLARE_BF16) return Da <= 64 ? launch_all<__nv_bfloat16, 64>(maps, a, Dc, spread, st) : launch_all<__nv_bfloat16, 128>(maps, a, Dc, spread, st);
   return Da <= 64 ? launch_all<__half, 64>(maps, a, Dc, spread, st) : launch_all<__half, 128>(maps, a, Dc, spread, st);
 }
