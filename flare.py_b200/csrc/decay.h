@@ -58,7 +58,7 @@ struct DecayStep {
 };
 
 // How the tensor-core kernels spread a call: the CTAs of a sequence (a cluster), the segments of the token axis, and the sequences
-// of the last round, if they are launched by themselves.
+// of the last wave, if they are launched by themselves.
 struct DecaySpread { int cluster, segments, rest, rest_cluster; };
 bool decay_tc_supported(const DecayArgs& a, int dtype);
 DecaySpread decay_tc_spread(int B, int H, int N, int Da, int Dc, int n_units);

@@ -1035,11 +1035,12 @@ int launch_walk(const void* kernel, dim3 grid, int threads, int smem, int cluste
 // How a call is spread: the CTAs of a sequence (a cluster) and the segments of the token axis, whichever the times below say is
 // shortest.  Measured (us, 64 / 128 features): a chunk in a CTA 1.9 / 3.0; a chunk's step of the state from CTA to CTA 0.65 /
 // 1.2, which bounds what a cluster gains on a long sequence; a chunk's sum 0.7 / 1.1; the ends of a launch 7.  Clusters of
-// three, four and eight do not fill every GPC: 45, 33 and 15 of them fit 148 SMs, and one more costs a second round (97 us in 36
-// clusters of four, 72 in 36 of two, at 8192 tokens).  E.g. D = 64: B = 4, H = 8, N = 8192 55 us in clusters of four, 71 of two, 73 in four segments;
-// H = 16 79 us in clusters of two, 106 of four, 124 in two segments; B = 1, H = 8, N = 65536 109 us in 18 segments, 117 in
-// nine of clusters of two.  Over 28 shapes from 200 to 131077 tokens the choice is within 1 % of the best of all on average.
-// Where the last round of a launch would leave most SMs idle, the sequences in it are launched by themselves, in clusters that use
+// three, four and eight do not fill every GPC: 45, 33 and 15 of them fit 148 SMs, and one more costs a second wave (97 us in 36
+// clusters of four, 72 in 36 of two, at 8192 tokens).  E.g. D = 64, N = 8192: B = 4, H = 8 55 us in clusters of four, 71 of two,
+// 73 in four segments; H = 16 79 us in clusters of two, 106 of four, 124 in two segments; B = 1, H = 8, N = 65536 109 us in 18
+// segments, 117 in nine of clusters of two.  Over 28 shapes from 200 to 131077 tokens the choice is within 1 % of the best of all
+// on average.
+// Where the last wave of a launch would leave most SMs idle, the sequences in it are launched by themselves, in clusters that use
 // more of them: the backward of B = 4, H = 16, N = 8192, D = 64 takes 148 sequences one to a CTA and 44 in clusters of three:
 // 182 us, where 192 clusters of two took 194.  Behind another launch the last of the clusters that fit did not find its place:
 // 45 of three took 208 us.
@@ -1050,8 +1051,8 @@ DecaySpread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
   const float chunk = wide ? 3.f : 1.9f, step = wide ? 1.2f : 0.65f, sum = wide ? 1.1f : 0.7f, ends = 7.f;
   constexpr int kSizes[] = {1, 2, 3, 4, 8};
   auto room = [&](int c) { return (c == 8 ? sms * 5 / 6 : c == 4 ? sms * 9 / 10 : c == 3 ? sms * 11 / 12 : sms) / c; };      // clusters that fit
-  auto rounds = [&](int n, int fit) { return (float)((n + fit - 1) / fit); };
-  auto round = [&](int c, int len) {               // a round of sequences of so many chunks
+  auto waves = [&](int n, int fit) { return (float)((n + fit - 1) / fit); };
+  auto wave = [&](int c, int len) {               // a wave of sequences of so many chunks
     const int own = (len + c - 1) / c;
     return (c > 1 && len * step > own * chunk ? len * step : own * chunk) + ends;
   };
@@ -1061,21 +1062,24 @@ DecaySpread pick_spread(int B, int H, int N, int Da, int Dc, int n_units) {
     if (t < least) { least = t; best = s; }
   };
   for (int c : kSizes) {
-    if (c > chunks) break;
-    const int fit = room(c), most = chunks / (2 * c), full = seqs <= sms ? sms / (seqs * c) : 0;       // full: segments that fill the GPU once
-    consider(rounds(seqs, fit) * round(c, chunks), {c, 1, 0, 1});
+    const int fit = room(c);
+    if (c > chunks || fit < 1) break;
+    const int most = chunks / (2 * c), full = seqs <= sms ? sms / (seqs * c) : 0;       // full: segments that fill the GPU once
+    consider(waves(seqs, fit) * wave(c, chunks), {c, 1, 0, 1});
     for (int k = 0; k < 3; ++k) {
       int s = k == 0 ? full / 2 : k == 1 ? full : 2 * full;
       s = s < most ? s : most;
       if (s < 2) continue;
       if (s > 256) s = 256;
       const int len = (chunks + s - 1) / s;
-      consider(rounds(seqs * s, fit) * round(c, len) + rounds(seqs * (s - 1), sms) * (len * sum + ends) + 4.f, {c, s, 0, 1});
+      consider(waves(seqs * s, fit) * wave(c, len) + waves(seqs * (s - 1), sms) * (len * sum + ends) + 4.f, {c, s, 0, 1});
     }
     const int whole = seqs / fit, rest = seqs - whole * fit;
     if (whole > 0 && rest > 0)
-      for (int r : kSizes)
-        if (r <= chunks) consider(whole * round(c, chunks) + rounds(rest, room(r) - (r > 2)) * round(r, chunks) + 3.f, {c, 1, rest, r});
+      for (int r : kSizes) {
+        const int places = room(r) - (r > 2);
+        if (r <= chunks && places > 0) consider(whole * wave(c, chunks) + waves(rest, places) * wave(r, chunks) + 3.f, {c, 1, rest, r});
+      }
   }
   return best;
 }

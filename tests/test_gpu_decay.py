@@ -153,8 +153,8 @@ def test_long_sequences_in_clusters_and_segments(fb, cuda_dev, shape, dtype):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(10, 16, 700, 64, 64), (4, 16, 700, 64, 64), (5, 9, 1100, 64, 64), (5, 3, 1100, 64, 64), (2, 13, 1300, 128, 128)])
-def test_sequences_that_do_not_fill_their_last_round(fb, cuda_dev, shape, dtype):
-    """More sequences than SMs, or a few less than a multiple: the ones of the last round are spread over more CTAs."""
+def test_sequences_that_do_not_fill_their_last_wave(fb, cuda_dev, shape, dtype):
+    """More sequences than SMs, or a few less than a multiple: the ones of the last wave are spread over more CTAs."""
     B, H, N, Dk, Dv = shape
     q, k, v, ld = make(cuda_dev, *shape, dtype, seed=B * H)
     lengths = torch.tensor([N - 150 * b for b in range(B - 1)] + [N], device=cuda_dev).clamp(min=0)
