@@ -555,6 +555,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         if (j < n) product_s(j);
         const int i = j - kAhead;
         if (i < 0) continue;
+        wait(bFullC + rc.at, rc.phase);            // the weighing warps' wait for c orders only what comes behind their event
         wait(bP + (i & 1), i >> 1);
         if (i > 0) wait(bYFree, i - 1);
         tc_fence_after();
