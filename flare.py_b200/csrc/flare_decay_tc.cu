@@ -457,6 +457,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 27);
   float* sExp = reinterpret_cast<float*>(bars + 28);         // 2^e of the packed state, by chunk modulo 4
   uint32_t* sMax = reinterpret_cast<uint32_t*>(bars + 30);   // [2][4], fp16 of 64 features
+  // Rows behind the length are cleared, in the one chunk of a segment that has them.  S waits for that on a barrier of its own: on
+  // bW, whose other phases it does not follow, a phase could go by unseen (the wait would then run out) or be taken for the last.
+  uint64_t* bClear = bars + 34;
 
   const int size = cluster_size(), rank = cluster_rank(), job = first + blockIdx.x / size;
   const int unit = __reduce_max_sync(0xffffffffu, job / per_unit);       // in a uniform register: it indexes the arguments
@@ -499,7 +502,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   if (tid == 0) {
     for (int i = 0; i < 3; ++i) { mbar_init(bFull + i, 1); mbar_init(bFullC + i, 1); mbar_init(bFree + i, 2); }     // bFree: A X and P C
     for (int i = 0; i < 2; ++i) { mbar_init(bS + i, 1); mbar_init(bP + i, 256); mbar_init(bX + i, 128); mbar_init(bW + i, 128); mbar_init(bEv + i, 1); }
-    mbar_init(bFreeB, 2); mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bYFree, 128);
+    mbar_init(bFreeB, 2); mbar_init(bClear, 128); mbar_init(bYx, 1); mbar_init(bKvFree, 128); mbar_init(bYFree, 128);
     for (int i = 0; i < 4; ++i) mbar_init(bIn + i, 1);
     fence_barrier_init();
     for (int i = 0; i < mine; ++i) {
@@ -530,11 +533,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     Ring<L::kC> rc;
     if (warp == L::kWarpI) {
       // ---- S = A B^T and P C -------------------------------------------------------------------------------------------
-      int ev = 0;
       auto product_s = [&](int i) {
         wait(bFull + ra.at, ra.phase);
-        if (sp.live(chunk(i)) < kL) wait(bW + (ev & 1), ev >> 1);      // rows behind the length are cleared first
-        ev += terms(i) == 3 ? 2 : 1;
+        if (sp.live(chunk(i)) < kL) wait(bClear, 0);
         tc_fence_after();
         if (elect_one()) {
           const uint64_t dA = tile_a(ra.at), dB = smem_desc<128>(base + L::oB + rb.at * (CB * kBlk));
@@ -931,6 +932,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         asm volatile("bar.sync 3, 128;" ::: "memory");
         weigh_c<T, CB>(r, 0, width / 8, cnt, plus && t == 2 ? w - 1.f : w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
                        smem + L::oB + rb.at * (CB * kBlk));
+        if (cnt < kL && part == 0) arrive_on(bClear);
         arrive_on(bW + (ev & 1));
         before = t;
       }

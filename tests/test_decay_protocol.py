@@ -112,8 +112,9 @@ class Pipe:
 class Cta:
     """One CTA of a walk.  chunks: those it takes; terms[c], cnt[c]: the terms and the live tokens of chunk c of the sequence."""
 
-    def __init__(self, sim, wide, rank, size, terms, cnt, plus=False, wait_c=True):
-        self.sim, self.rank, self.size, self.terms, self.cnt, self.plus, self.wait_c = sim, rank, size, terms, cnt, plus, wait_c
+    def __init__(self, sim, wide, rank, size, terms, cnt, plus=False, wait_c=True, own_clear=True):
+        self.sim, self.rank, self.size, self.terms, self.cnt, self.plus, self.wait_c, self.own_clear = \
+            sim, rank, size, terms, cnt, plus, wait_c, own_clear
         self.wide, self.total = wide, len(terms)
         self.chunks = list(range(rank, self.total, size))
         self.kA, self.kB, self.kC = (2, 1, 2) if wide else (3, 3, 3)
@@ -121,7 +122,7 @@ class Cta:
         self.full = [B(f"bFull{i}", 1) for i in range(self.kA)]
         self.fullC = [B(f"bFullC{i}", 1) for i in range(self.kC)]
         self.free = [B(f"bFree{i}", 2) for i in range(self.kA)]
-        self.freeB, self.yx = B("bFreeB", 2), B("bYx", 1)
+        self.freeB, self.clear, self.yx = B("bFreeB", 2), B("bClear", 1), B("bYx", 1)
         self.S, self.P, self.X = ([B(f"{n}{i}", 1) for i in range(2)] for n in ("bS", "bP", "bX"))
         self.W, self.Ev = ([B(f"{n}{i}", 1) for i in range(2)] for n in ("bW", "bEv"))
         self.kvFree, self.yFree, self.inn = B("bKvFree", 1), B("bYFree", 1), B("bIn", 1)
@@ -199,10 +200,13 @@ class Cta:
     # -- products --------------------------------------------------------------------------------------------------------
     def r_spc(self):
         pipe, n = Pipe(self.sim), len(self.chunks)
-        ahead = 0 if self.wide else 1
+        ahead, ev = 0 if self.wide else 1, 0
         for j in range(n + ahead):
             if j < n:
                 yield self.full[j % self.kA], j // self.kA
+                if self.cnt[self.chunks[j]] < KL:
+                    yield (self.clear, 0) if self.own_clear else (self.W[ev & 1], ev >> 1)
+                ev += 2 if self.t(j) == 3 else 1
 
                 def read(j=j):
                     self.see("S reads a", self.a[j % self.kA], self.raw(j))
@@ -308,6 +312,8 @@ class Cta:
                     self.b[i % self.kB] = self.c[i % self.kC] = (i, "cleared")
                 for x in ((ev & 1,) if t == 1 else (0,) if part else (0, 1)):
                     self.w[x] = ev
+                if short and part == 0:
+                    self.clear.arrive()
                 self.W[ev & 1].arrive()
                 before = t
                 ev += 1
@@ -399,6 +405,24 @@ def test_whole_chunks(terms, wide, size):
     for seed in SEEDS:
         walk(seed, wide, size, terms)
         walk(seed, wide, size, [min(t, 2) for t in terms], plus=True)
+
+
+@pytest.mark.parametrize("size", [1, 2, 3, 4])
+@pytest.mark.parametrize("wide", [False, True], ids=["64", "128"])
+@pytest.mark.parametrize("terms", TERMS, ids=str)
+def test_a_chunk_that_ends_early(terms, wide, size):
+    """The sequence's last chunk, or its mirror image's first; the mirror image returns no state, so its chunks take one term."""
+    for seed in SEEDS:
+        walk(seed, wide, size, terms, last=50)
+        walk(seed, wide, size, [min(t, 2) for t in terms], last=1, plus=True)
+        walk(seed, wide, size, [1] * len(terms), last=72, rev=True)
+
+
+@pytest.mark.parametrize("terms,rev,how", [([1] * 7, True, "went by unseen"), ([3, 3], False, "a wait for phase 1 passed while 0")])
+def test_the_model_notices_phases_that_are_not_followed(terms, rev, how):
+    with pytest.raises(Fault, match=how):
+        for seed in range(4000):
+            walk(seed, False, 1, terms, last=72, rev=rev, own_clear=False)
 
 
 @pytest.mark.parametrize("wide", [False, True], ids=["64", "128"])
