@@ -746,11 +746,26 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     auto magnitude = [](const float4& x) {
       return max(max(__float_as_uint(x.x) & 0x7fffffffu, __float_as_uint(x.y) & 0x7fffffffu), max(__float_as_uint(x.z) & 0x7fffffffu, __float_as_uint(x.w) & 0x7fffffffu));
     };
+    // Values that are not finite have no say in it: one of them, in a column of its own, would scale the others' down to nothing.
+    constexpr uint32_t kInf = 0x7f800000u;
+    auto finite_magnitude = [](const float4& x) {
+      auto of = [](float v) {
+        const uint32_t m = __float_as_uint(v) & 0x7fffffffu;
+        return m < kInf ? m : 0u;
+      };
+      return max(max(of(x.x), of(x.y)), max(of(x.z), of(x.w)));
+    };
     // fp16: the largest magnitude of the state before chunk c.  Of 128 features it is found as the state is made, and travels
     // with it: a warp's beside its quarter, even and odd chunks apart.  Of 64, whose packing comes last, it is found then.
     constexpr bool kSent = kHalfRange && DK == 128;
     auto note = [&](uint32_t top, int c) {
       top = __reduce_max_sync(0xffffffffu, top);
+      if (top >= kInf) {
+        top = 0;
+#pragma unroll 1
+        for (int j = 0; j < width; j += 4) top = max(top, finite_magnitude(*reinterpret_cast<const float4*>(in + 128 * j)));
+        top = __reduce_max_sync(0xffffffffu, top);
+      }
       if (lane == 0) *reinterpret_cast<uint32_t*>(in - 16 + 4 * (c & 1)) = top;
     };
     auto noted = [&](int c) {
@@ -860,6 +875,12 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
           for (int q = 0; q < 8; ++q) top = max(top, magnitude(x[q]));
           top = __reduce_max_sync(0xffffffffu, top);
+          if (top >= kInf) {
+            top = 0;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) top = max(top, finite_magnitude(x[q]));
+            top = __reduce_max_sync(0xffffffffu, top);
+          }
           if (lane == 0) sMax[4 * (i & 1) + w] = top;
           asm volatile("bar.sync 1, 128;" ::: "memory");
           const uint4 all = *reinterpret_cast<const uint4*>(sMax + 4 * (i & 1));

@@ -1,0 +1,70 @@
+"""Decayed linear attention in 16 bits over the range of its operands: small and large values, and single ones that are not finite.
+
+Tolerances are those of test_gpu_decay.py, relative to what is compared, plus what a result of fp16 rounds by below its normal range:
+half of 2^-24 an element."""
+import pytest
+import torch
+
+from oracle import flare_oracle as O
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def fb(cuda_dev):
+    import flare_b200
+    return flare_b200
+
+
+def off(a, b):
+    return (a.detach().double() - b.detach().double()).norm().item()
+
+
+def bound(ref, dtype):
+    """Two roundings of 16 bits and the fp32 sums, relative; half a step of the smallest fp16 numbers, absolute."""
+    eps = torch.finfo(dtype).eps
+    return (eps + 8e-6) * ref.norm().item() + (ref.numel() ** 0.5 * 2.0 ** -25 if dtype == torch.float16 else 0.0)
+
+
+def make(dev, B, H, N, Dk, Dv, dtype, sizes, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [(s * torch.randn(B, H, N, D, generator=g, device=dev)).to(dtype) for s, D in zip(sizes, (Dk, Dk, Dv, Dv))]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_a_value_that_is_not_finite_spoils_its_own_column_alone(fb, cuda_dev, dtype, D, bad):
+    """v enters column by column: the others of the outputs and of the state are what they are without it."""
+    N, at, col = 900, 300, 5
+    q, k, v, _ = make(cuda_dev, 1, 2, N, D, 64, dtype, (1.0, 1.0, 1.0, 1.0), seed=13)
+    ld = torch.tensor([-0.002, -0.1], device=cuda_dev)
+    state = torch.randn(1, 2, D, 64, device=cuda_dev)
+    keep = [c for c in range(64) if c != col]
+    y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld, 0.125, state)
+    v[0, :, at, col] = bad
+    y, end = fb.decay_linear_prefill(q, k, v, ld, 0.125, state=state)
+    assert not end[..., col].isfinite().any() and not y[:, :, at:, col].isfinite().any()
+    for h in range(2):
+        assert off(y[:, h][..., keep], y_ref[:, h][..., keep]) <= bound(y_ref[:, h][..., keep], dtype)
+        assert off(end[:, h][..., keep], end_ref[:, h][..., keep]) <= 1e-5 * end_ref[:, h][..., keep].norm().item()
+    # the same in the state that a call starts from
+    y_ref, end_ref = O.decay_linear_recurrent(q[:, :, :at], k[:, :, :at], v[:, :, :at], ld, 0.125, state)
+    state[0, :, 7, col] = bad
+    y, end = fb.decay_linear_prefill(q[:, :, :at], k[:, :, :at], v[:, :, :at], ld, 0.125, state=state)
+    assert not end[:, :, 7, col].isfinite().any()
+    for h in range(2):
+        assert off(y[:, h][..., keep], y_ref[:, h][..., keep]) <= bound(y_ref[:, h][..., keep], dtype)
+        assert off(end[:, h][..., keep], end_ref[:, h][..., keep]) <= 1e-5 * end_ref[:, h][..., keep].norm().item()
+
+
+def test_a_key_that_is_not_finite_leaves_the_tokens_before_it(fb, cuda_dev):
+    """k enters through q . k: P is zero for the tokens before, whatever stands there."""
+    for dtype in (torch.bfloat16, torch.float16):
+        q, k, v, _ = make(cuda_dev, 1, 1, 400, 64, 64, dtype, (1.0, 1.0, 1.0, 1.0), seed=17)
+        ld = torch.tensor([-0.05], device=cuda_dev)
+        ref = O.decay_linear_dense(q.double(), k.double(), v.double(), ld, 0.125)
+        k[0, 0, 200, 3] = float("nan")
+        y = fb.decay_linear(q, k, v, ld, 0.125)
+        assert off(y[:, :, :200], ref[:, :, :200]) <= bound(ref[:, :, :200], dtype)
+        assert not y[:, :, 200:].isfinite().any()
