@@ -217,6 +217,32 @@ __device__ __forceinline__ int terms_of(float g2, int behind) {
 template <typename T>
 __device__ __forceinline__ bool near_one(float g2) { return Op16<T>::kFmt == 1 && fabsf(g2) <= 0.4f / kL; }
 
+// fp16: what is rounded to it is first taken, by a power of two, to where its largest magnitude is 2^13 to 2^14.  The type ends at
+// 2^-24 below and at 65504 above: unscaled, values of size 1e-3 would keep 5e-5 of a state and of size 1e-5 3e-3 of a gradient.
+__device__ __forceinline__ int exponent_of(uint32_t top) { return max(-100, min(100, (int)(top >> 23) - 127 - 13)); }
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+// The largest magnitude among the pieces of a row, weighted, as its bits.  Values that are not finite have no say in it: they may
+// stand in a column of their own.
+__device__ __forceinline__ uint32_t top_of_row(int r, int p0, int pieces, float w, const uint8_t* src) {
+  const uint32_t row = 128 * r + 16 * (r & 7);
+  uint32_t m = 0;
+#pragma unroll 4
+  for (int ch = p0; ch < p0 + pieces; ++ch) {
+    const uint4 x = *reinterpret_cast<const uint4*>(src + (row ^ (16 * ch)));
+    m = __vmaxu2(m, __vmaxu2(__vmaxu2(x.x & 0x7fff7fffu, x.y & 0x7fff7fffu), __vmaxu2(x.z & 0x7fff7fffu, x.w & 0x7fff7fffu)));
+  }
+  constexpr uint32_t kInf = 0x7c00u;
+  if (max(m & 0xffffu, m >> 16) >= kInf) {
+    m = 0;
+#pragma unroll 1
+    for (int i = 8 * p0; i < 8 * (p0 + pieces); ++i) {
+      const uint32_t x = *reinterpret_cast<const uint16_t*>(src + (row ^ (16 * (i >> 3))) + 2 * (i & 7)) & 0x7fffu;
+      m = max(m, x < kInf ? x : 0u);
+    }
+  }
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max(m & 0xffffu, m >> 16))) * w);
+}
+
 // C weighted by the decay to the chunk's end; a thread takes PIECES of the 16-byte pieces of a row, and of those the first `pieces`
 // hold columns.  `which` of its terms are written, bit by bit: 1, 2 and 4 for the first, second and third, to w_t and the tiles
 // behind it, but the third alone to w_t.  Rows behind the length are cleared, here and in the tiles of b and c themselves.
@@ -304,6 +330,9 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBars);
   uint64_t *bFull = bars, *bFree = bars + 3, *bW = bars + 6, *bKv = bars + 8, *bKvFree = bars + 10;      // bW, bKv, bKvFree: two buffers each
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint32_t* sTop = reinterpret_cast<uint32_t*>(bars + 14);   // [8], fp16: the weighing warps' largest magnitudes
+  float* sUnit = reinterpret_cast<float*>(bars + 18);        // and what the weighted C of a chunk was divided by, by chunk modulo 4
+  constexpr bool kHalfRange = F == 0;
   const DecayUnit& u = a.u[blockIdx.z];
   const int n_cb = (u.Dc + 63) / 64;
   const int bh = blockIdx.x % (a.B * a.H), cb = blockIdx.x / (a.B * a.H), seg = u.rev ? blockIdx.y + 1 : blockIdx.y;
@@ -378,6 +407,7 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       const bool more = terms(c) > 1;
       wait_together<2, 128>(wait, warp == 8, bKv + (c & 1), c >> 1);
       tc_fence_after();
+      const float unit = kHalfRange ? sUnit[c & 3] : 1.f;
 #pragma unroll
       for (int j = 0; j < NC; j += 16) {
         uint32_t v[16], lo[16];
@@ -390,7 +420,10 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         }
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i) X[j + i] = decay(X[j + i]) + (__uint_as_float(v[i]) + __uint_as_float(lo[i]));
+        for (int i = 0; i < 16; ++i) {
+          const float x = __uint_as_float(v[i]) + __uint_as_float(lo[i]);
+          X[j + i] = decay(X[j + i]) + (kHalfRange ? x * unit : x);
+        }
       }
       tc_fence_before();
       arrive_on(bKvFree + (c & 1));
@@ -404,12 +437,23 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     const int r = tid & 127, half = tid >> 7;      // row, half of its pieces
     for (int c = 0; c < sp.nch; ++c) {
       const int cnt = sp.live(c);
-      const float w = exp2f(g2 * (float)(sp.rev ? r : max(0, cnt - 1 - r)));
-      if (warp == 1) {
-        wait(bFull + ring.at, ring.phase);
-        if (c > 1) wait(bKv + (c & 1), (c - 2) >> 1);        // the product with what stood here is done
+      float w = exp2f(g2 * (float)(sp.rev ? r : max(0, cnt - 1 - r)));
+      if (warp == 1) wait(bFull + ring.at, ring.phase);
+      if constexpr (kHalfRange) {
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const uint32_t top = __reduce_max_sync(0xffffffffu, r < cnt ? top_of_row(r, 4 * half, 4, w, smem + L::oC + ring.at * kBlk) : 0u);
+        if ((tid & 31) == 0) sTop[warp] = top;
       }
+      if (warp == 1 && c > 1) wait(bKv + (c & 1), (c - 2) >> 1);       // the product with what stood here is done
       asm volatile("bar.sync 1, 256;" ::: "memory");
+      if constexpr (kHalfRange) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = max(top, sTop[i]);
+        const int e = exponent_of(top);
+        if (tid == 0) sUnit[c & 3] = power_of_two(e);        // the sum of chunk c - 4 has read what stood here: its product is behind
+        w *= power_of_two(-e);
+      }
       const int t = terms(c);
       weigh_c<T, CB, 4>(r, 4 * half, 4, cnt, t == 2 && plus ? w - 1.f : w, (1 << t) - 1, smem + L::oC + ring.at * kBlk, smem + L::oW + (c & 1) * (3 * kBlk),
                         smem + L::oB + ring.at * (CB * kBlk));
@@ -460,6 +504,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   // Rows behind the length are cleared, in the one chunk of a segment that has them.  S waits for that on a barrier of its own: on
   // bW, whose other phases it does not follow, a phase could go by unseen (the wait would then run out) or be taken for the last.
   uint64_t* bClear = bars + 34;
+  uint32_t* sTop = reinterpret_cast<uint32_t*>(bars + 36);   // [4], fp16: the weighing warps' largest magnitudes
+  float* sUnit = reinterpret_cast<float*>(bars + 38);        // and what the weighted C was divided by, by chunk modulo 4
 
   const int size = cluster_size(), rank = cluster_rank(), job = first + blockIdx.x / size;
   const int unit = __reduce_max_sync(0xffffffffu, job / per_unit);       // in a uniform register: it indexes the arguments
@@ -811,9 +857,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     };
     // the largest magnitude of an fp16 tile to 2^13 ... 2^14: X may lie outside fp16's range
     auto scale_down = [&](uint32_t top, int i) {
-      const int e = max(-100, min(100, (int)(top >> 23) - 127 - 13));
-      if (r == 0) sExp[i & 3] = __uint_as_float((uint32_t)(127 + e) << 23);
-      return __uint_as_float((uint32_t)(127 - e) << 23);
+      const int e = exponent_of(top);
+      if (r == 0) sExp[i & 3] = power_of_two(e);
+      return power_of_two(-e);
     };
     auto send = [&](int c) {                       // what this warp has written, to the CTA of the next chunk
       if (size == 1 || c + 1 == sp.nch) return;
@@ -840,6 +886,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if (t == 3) ++ev;
       wait_together<4, 128>(wait, w == 2, bEv + (ev & 1), ev >> 1);
       tc_fence_after();
+      const float unit = kHalfRange ? sUnit[i & 3] : 1.f;
       if constexpr (DK == 64) {
         // all of a thread's 32 columns in registers: B^T C before the state arrives, then the state behind the chunk, which the
         // next CTA waits for, and last the packing for this chunk's product
@@ -862,6 +909,11 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         }
         tc_fence_before();
         arrive_on(bKvFree);
+        if constexpr (kHalfRange) {
+          const F2 unit2 = both(unit);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = mul2(v[k], unit2);
+        }
         receive(i, c);
         float4 x[8];
 #pragma unroll
@@ -904,9 +956,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             pack(x0, x1, down, j);
             tmem_wait_ld();
             auto v = [&](int k) {
-              const F2 first = floats(h[k], h[k + 1]);
-              if constexpr (more.value) return add2(first, floats(l[k], l[k + 1]));
-              else return first;
+              F2 x = floats(h[k], h[k + 1]);
+              if constexpr (more.value) x = add2(x, floats(l[k], l[k + 1]));
+              if constexpr (kHalfRange) x = mul2(x, both(unit));
+              return x;
             };
             const float4 y0 = stepped(x0, v(0), v(2)), y1 = stepped(x1, v(4), v(6));
             *reinterpret_cast<float4*>(in + 128 * j) = y0;
@@ -939,18 +992,29 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     int ev = 0, before = 1;                        // events so far, terms of the last
     for (int i = 0; i < mine; ++i) {
       const int cnt = sp.live(chunk(i));
-      const float w = rev || cnt == kL ? w_full : exp2f(g2 * (float)max(0, cnt - 1 - r));
+      float w = rev || cnt == kL ? w_full : exp2f(g2 * (float)max(0, cnt - 1 - r));
       const int t = terms(i), parts = t == 3 ? 2 : 1;
       const bool leader = warp == L::kWarpC + 2;
       if (leader) {
         wait(bFullC + ra.at, ra.phase);
         if (cnt < kL) wait(bFull + ra.at, ra.phase);
       }
+      if constexpr (kHalfRange) {                  // while the product with what stands in w_t may still run
+        asm volatile("bar.sync 3, 128;" ::: "memory");
+        const uint32_t top = __reduce_max_sync(0xffffffffu, r < cnt ? top_of_row(r, 0, width / 8, w, smem + L::oC + ra.at * kBlk) : 0u);
+        if (lane == 0) sTop[warp & 3] = top;
+      }
       for (int part = 0; part < parts; ++part, ++ev) {
         // the product with what stood here is done: the event before the last one, or the last where either takes both tiles
         const int back = t > 1 || before > 1 ? 1 : 2;
         if (leader && ev >= back) wait(bEv + ((ev - back) & 1), (ev - back) >> 1);
         asm volatile("bar.sync 3, 128;" ::: "memory");
+        if constexpr (kHalfRange) {                // fp16 has one part
+          const uint4 tops = *reinterpret_cast<const uint4*>(sTop);
+          const int e = exponent_of(max(max(tops.x, tops.y), max(tops.z, tops.w)));
+          if (r == 0) sUnit[i & 3] = power_of_two(e);        // chunk i - 4 has been read here: B^T C of i - 2, behind that, is done
+          w *= power_of_two(-e);
+        }
         weigh_c<T, CB>(r, 0, width / 8, cnt, plus && t == 2 ? w - 1.f : w, part ? 4 : t == 1 ? 1 : 3, smem + L::oC + ra.at * kBlk, smem + L::oW + (t == 1 ? (ev & 1) * kBlk : 0),
                        smem + L::oB + rb.at * (CB * kBlk));
         if (cnt < kL && part == 0) arrive_on(bClear);

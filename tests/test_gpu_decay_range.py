@@ -31,6 +31,37 @@ def make(dev, B, H, N, Dk, Dv, dtype, sizes, seed):
     return [(s * torch.randn(B, H, N, D, generator=g, device=dev)).to(dtype) for s, D in zip(sizes, (Dk, Dk, Dv, Dv))]
 
 
+@pytest.mark.parametrize("size", [0.1, 0.01, 1e-3, 1e-4, 1e-5, 100.0])
+@pytest.mark.parametrize("N", [300, 2100])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_states_keep_their_bits_for_values_of_any_size(fb, cuda_dev, dtype, D, N, size):
+    """The bound of values of size 1: what the 16-bit terms leave is 2e-6 of the state, the sums in fp32 sqrt(N) * 2^-24."""
+    rates = [0.0, 1e-3, 4e-3, 1e-2, 0.05, 0.3, 3.0]
+    H = len(rates)
+    q, k, v, _ = make(cuda_dev, 1, H, N, D, D, dtype, (1.0, 1.0, size, 1.0), seed=N + D)
+    ld = -torch.tensor(rates, device=cuda_dev)
+    end = fb.decay_linear_prefill(q, k, v, ld)[1]
+    ref = O.decay_linear_recurrent(q, k, v, ld)[1]
+    for h in range(H):
+        assert off(end[:, h], ref[:, h]) <= (2e-6 + N ** 0.5 * 2.0 ** -24) * ref[:, h].norm().item(), rates[h]
+
+
+@pytest.mark.parametrize("shape", [(1, 1, 9000, 64, 64), (2, 1, 5000, 128, 64)])
+def test_small_values_in_clusters_and_segments(fb, cuda_dev, shape):
+    dtype = torch.float16
+    B, H, N, Dk, Dv = shape
+    q, k, v, _ = make(cuda_dev, *shape, dtype, (1e-3, 1e-2, 1e-3, 1.0), seed=7)
+    ld = torch.tensor([-1e-3], device=cuda_dev)
+    lengths = torch.tensor([N - 1000] + [N] * (B - 1), device=cuda_dev)
+    state = torch.randn(B, H, Dk, Dv, device=cuda_dev) * 1e-4
+    scale = 1e5
+    y, end = fb.decay_linear_prefill(q, k, v, ld, scale, state=state, lengths=lengths)
+    y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld, scale, state, lengths)
+    assert off(y, y_ref) <= bound(y_ref, dtype)
+    assert off(end, end_ref) <= (2e-6 + N ** 0.5 * 2.0 ** -24) * end_ref.norm().item()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
