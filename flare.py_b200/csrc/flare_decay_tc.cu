@@ -478,8 +478,8 @@ template <int DK> struct WalkPlan {
   static constexpr int kXTile = DK * 128;          // one term of the packed state: [DK][64]
   static constexpr int kXPart = 16 + DK * 64;      // a warp's quarter of the state in fp32, as it arrives, behind its largest magnitude
   static constexpr int oA = 0, oB = oA + kA * kCB * kBlk, oC = oB + kB * kCB * kBlk, oW = oC + kC * kBlk, oX = oW + kW * kBlk,
-                       oOut = oX + 2 * kXTile, oIn = oOut + (kStage ? kBlk : 0), oBars = oIn + 4 * kXPart;
-  static constexpr int kBytes = oBars + 512 + 1024;
+                       oOut = oX + 2 * kXTile, oIn = oOut + (kStage ? kBlk : 0), oBars = oIn + 4 * kXPart, oRows = oBars + 512;
+  static constexpr int kBytes = oRows + 6 * 128 + 1024;
   static constexpr int kWarpC = 8, kWarpX = 12, kWarpY = 16, kWarpI = 20, kThreads = 32 * (kWarpI + 3);
   static constexpr int cY = 256, cYx = 320, cKv = 384;       // tensor memory: S of even and odd chunks at 0 and 128
 };
@@ -506,6 +506,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
   uint64_t* bClear = bars + 34;
   uint32_t* sTop = reinterpret_cast<uint32_t*>(bars + 36);   // [4], fp16: the weighing warps' largest magnitudes
   float* sUnit = reinterpret_cast<float*>(bars + 38);        // and what the weighted C was divided by, by chunk modulo 4
+  uint8_t* sRow = smem + L::oRows;                           // [2][128], fp16: the exponent of the largest P of a row's halves
+  int8_t* sPow = reinterpret_cast<int8_t*>(sRow + 256);      // [4][128]: P of a row was divided by 2^this, by chunk modulo 4
 
   const int size = cluster_size(), rank = cluster_rank(), job = first + blockIdx.x / size;
   const int unit = __reduce_max_sync(0xffffffffu, job / per_unit);       // in a uniform register: it indexes the arguments
@@ -712,7 +714,6 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     const int w = warp & 3, r = 32 * w + lane;     // token
     const uint32_t y_at = tmem + ((uint32_t)(32 * w) << 16) + L::cY, x_at = y_at + (L::cYx - L::cY);
     const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
-    const F2 scale2 = both(a.scale);
     T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0;
     const int cols = u.Dc - c0;                    // of the 64 columns, those that exist
     uint8_t* tile = smem + L::oOut + w * 4096;     // the warp's [32 rows][64], swizzled: piece k of a row at row ^ 16 k
@@ -727,7 +728,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       wait_together<5, 128>(wait, w == 0, bFree + ra.at, ra.phase);
       ra.next();
       tc_fence_after();
-      const F2 fx = both(kHalfRange ? wx * sExp[i & 3] : wx);
+      const F2 fx = both(kHalfRange ? wx * sExp[i & 3] : wx), scale2 = both(kHalfRange ? a.scale * power_of_two(sPow[128 * (i & 3) + r]) : 1.f);
       uint32_t y[16], x[16];
       tmem_ld16(y_at, y);
       tmem_ld16(x_at, x);
@@ -1028,6 +1029,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     // ---- weights of P --------------------------------------------------------------------------------------------------
     const int r0 = 32 * (warp & 3), r = r0 + lane, hb = warp >> 2;    // token, half of the columns
     const uint32_t lane_base = tmem + ((uint32_t)r0 << 16);
+    // fp16: a row of P is scaled by a power of two of its own before it is rounded, so that products q . k of any size keep their
+    // bits, those beyond 65504 too.  The weighted row goes back to tensor memory until its largest is known.
     const float scale_p = kHalfRange ? 1.f : a.scale;
     // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
     // diagonal the latter exceeds 1, up to lambda^-15, and the former makes up for it: products as small as 2^-66 stay normal
@@ -1042,12 +1045,14 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       const uint32_t s = lane_base + 128 * (i & 1) + 64 * hb;
       wait_together<2, 256>(wait, warp == 3, bS + (i & 1), i >> 1);
       tc_fence_after();
+      uint32_t top = 0;
 #pragma unroll 1
       for (int k = 0; k < 4; ++k) {
         const int j0 = 64 * hb + 16 * k;           // the block's first column; the warp's rows are r0 ... r0 + 31
         const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = rev ? j0 >= r0 + 31 : j0 + 15 <= r0;
         uint32_t p[8];
         if (none) {
+          if constexpr (kHalfRange) continue;
 #pragma unroll
           for (int m = 0; m < 8; ++m) p[m] = 0u;
         } else {
@@ -1058,7 +1063,16 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
           tmem_wait_ld();
           if (all) {
 #pragma unroll
-            for (int m = 0; m < 8; ++m) p[m] = pack2<T>(mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), row));
+            for (int m = 0; m < 8; ++m) {
+              const F2 x = mul2(mul2(floats(v[2 * m], v[2 * m + 1]), wcol[m]), row);
+              if constexpr (kHalfRange) {
+                const float2 f = x.get();
+                v[2 * m] = __float_as_uint(f.x);
+                v[2 * m + 1] = __float_as_uint(f.y);
+              } else {
+                p[m] = pack2<T>(x);
+              }
+            }
           } else if (mild) {
             const int t = r - j0;                  // columns up to t, or from t on
 #pragma unroll
@@ -1074,8 +1088,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
               for (int m = 0; m < 16; ++m) v[m] = m <= t ? v[m] : 0u;
             }
+            if constexpr (!kHalfRange)
 #pragma unroll
-            for (int m = 0; m < 8; ++m) p[m] = Op16<T>::pack(__uint_as_float(v[2 * m]), __uint_as_float(v[2 * m + 1]));
+              for (int m = 0; m < 8; ++m) p[m] = Op16<T>::pack(__uint_as_float(v[2 * m]), __uint_as_float(v[2 * m + 1]));
           } else {
 #pragma unroll 1
             for (int m = 0; m < 8; ++m) {
@@ -1089,11 +1104,47 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
               const uint32_t t = Op16<T>::pack(x0, x1);
 #pragma unroll
               for (int q = 0; q < 8; ++q)
-                if (q == m) p[q] = t;
+                if (q == m) {
+                  if constexpr (kHalfRange) {
+                    v[2 * q] = __float_as_uint(x0);
+                    v[2 * q + 1] = __float_as_uint(x1);
+                  } else {
+                    p[q] = t;
+                  }
+                }
             }
           }
+          if constexpr (kHalfRange) {
+#pragma unroll
+            for (int m = 0; m < 16; ++m) top = max(top, v[m] & 0x7fffffffu);
+            tmem_st16(s + 16 * k, v);
+          }
         }
-        tmem_st8(s + 8 * k, p);                    // over columns that are read already
+        if constexpr (!kHalfRange) tmem_st8(s + 8 * k, p);   // over columns that are read already
+      }
+      if constexpr (kHalfRange) {
+        sRow[128 * hb + r] = (uint8_t)(top >> 23);
+        tmem_wait_st();
+        asm volatile("bar.sync %0, 64;" ::"r"(6 + (warp & 3)) : "memory");         // the two warps of these rows
+        const int e = exponent_of(max(top >> 23, (uint32_t)sRow[128 * (hb ^ 1) + r]) << 23);
+        if (hb == 0) sPow[128 * (i & 3) + r] = (int8_t)e;
+        const F2 up = both(power_of_two(-e));
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+          const int j0 = 64 * hb + 16 * k;
+          uint32_t p[8];
+          if (rev ? j0 + 15 < r0 : j0 > r0 + 31) {
+#pragma unroll
+            for (int m = 0; m < 8; ++m) p[m] = 0u;
+          } else {
+            uint32_t v[16];
+            tmem_ld16(s + 16 * k, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int m = 0; m < 8; ++m) p[m] = pack2<T>(mul2(floats(v[2 * m], v[2 * m + 1]), up));
+          }
+          tmem_st8(s + 8 * k, p);
+        }
       }
       tmem_wait_st();
       tc_fence_before();

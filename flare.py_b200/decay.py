@@ -12,8 +12,8 @@ q, k: [B,H,N,Dk], v: [B,H,N,Dv] in one of fp32, fp16, bf16, any strides (the 'b 
 taken as they are); Dk, Dv up to 256.  ``log_decay``: [H], a constant of the model (no gradient), usually at most 0: 0 is no
 decay, -inf leaves a token itself alone.  ``lengths``: int32 (or int64) [B]; tokens at or behind ``lengths[b]`` -- padding,
 which may hold anything -- leave the state alone and have outputs and gradients of zero.  A value that is not finite among the
-live tokens spoils the outputs of the 128-token chunk it stands in, also those before it.  fp16: the products q . k have to
-stay within fp16's range, in the backward dy . v too (the scale is applied behind them).
+live tokens spoils the outputs of the 128-token chunk it stands in, also those before it.  Products, weighted values and states of
+fp16 operands carry powers of two of their own, so that small and large ones keep their bits; results are fp16's.
 """
 from __future__ import annotations
 

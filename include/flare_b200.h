@@ -304,8 +304,8 @@ int flare_causal_linear(int B, int H, int N, int Dk, int Dv, int dtype, const vo
  *     dv_n = scale sum_{t>=n} lambda^(t-n) (k_n . q_t) dy_t.
  *   flare_decay_decode: the N tokens (usually N = 1) one after the other on `state`, updated in place.
  * 16-bit inputs with Dk up to 128 (in the backward Dv too), both multiples of 8, and 16-byte aligned rows, strides and
- * states run on the tensor cores, the rest on fp32 kernels.  fp16 products q.k (in the backward dy.v too) must stay within
- * fp16's range there.  Workspaces: the two functions' bytes, 0 when a problem needs none. */
+ * states run on the tensor cores, the rest on fp32 kernels.  Workspaces: the two functions' bytes, 0 when a problem
+ * needs none. */
 typedef struct FlareDecay {
   int32_t B, H, N, Dk, Dv;
   int32_t dtype;                 /* of q, k, v, y, dy, dq, dk, dv */

@@ -128,6 +128,7 @@ class Cta:
         self.kvFree, self.yFree, self.inn = B("bKvFree", 1), B("bYFree", 1), B("bIn", 1)
         self.a, self.b, self.c = [None] * self.kA, [None] * self.kB, [None] * self.kC
         self.w, self.s = [None] * 2, [None] * 2
+        self.unit, self.pow = [None] * 4, [None] * 4       # fp16: powers of two of the weighted c and of P
         self.kv = self.y = self.yx_v = self.packed = self.state = None
         self.pend = {}
         self.out = []
@@ -312,6 +313,7 @@ class Cta:
                     self.b[i % self.kB] = self.c[i % self.kC] = (i, "cleared")
                 for x in ((ev & 1,) if t == 1 else (0,) if part else (0, 1)):
                     self.w[x] = ev
+                self.unit[i & 3] = i
                 if short and part == 0:
                     self.clear.arrive()
                 self.W[ev & 1].arrive()
@@ -324,7 +326,7 @@ class Cta:
             self.see("weights read S", self.s[i & 1], ("S", i))
             yield None
             self.see("weights read S", self.s[i & 1], ("S", i))
-            self.s[i & 1] = ("P", i)
+            self.s[i & 1], self.pow[i & 3] = ("P", i), i
             self.P[i & 1].arrive()
 
     def r_state(self):
@@ -334,6 +336,7 @@ class Cta:
                 ev += 1
             yield self.Ev[ev & 1], ev >> 1
             self.see("the state reads B^T C", self.kv, i)
+            self.see("the state reads its unit", self.unit[i & 3], i)
             yield None
             self.see("the state reads B^T C", self.kv, i)
             if not self.wide:
@@ -369,6 +372,7 @@ class Cta:
             yield self.free[i % self.kA], i // self.kA
             self.see("outputs read P C", self.y, i)
             self.see("outputs read A X", self.yx_v, i)
+            self.see("outputs read P's power", self.pow[i & 3], i)
             yield None
             self.see("outputs read P C", self.y, i)
             self.see("outputs read A X", self.yx_v, i)

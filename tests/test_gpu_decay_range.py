@@ -47,6 +47,31 @@ def test_states_keep_their_bits_for_values_of_any_size(fb, cuda_dev, dtype, D, N
         assert off(end[:, h], ref[:, h]) <= (2e-6 + N ** 0.5 * 2.0 ** -24) * ref[:, h].norm().item(), rates[h]
 
 
+# sizes of q, k, v, dy: the products q . k and dy . v far below and far above what a 16-bit number of fp16 holds well
+SIZES = [(1.0, 1.0, 1.0, 1.0), (1e-2, 1e-2, 1.0, 1e-2), (1e-3, 1e-3, 1.0, 1e-2), (1e-4, 1e-3, 1.0, 1e-3), (1.0, 1.0, 1e-3, 1e-3), (1.0, 1.0, 1e-4, 1e-4),
+         (1.0, 1.0, 1e-5, 1e-2), (60.0, 60.0, 1.0, 1.0), (1.0, 1.0, 100.0, 100.0), (300.0, 1e-3, 200.0, 1e-3)]
+
+
+@pytest.mark.parametrize("sizes", SIZES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 3, 700, 64, 64), (1, 3, 650, 128, 32), (2, 3, 300, 64, 128)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_outputs_and_gradients_for_operands_of_any_size(fb, cuda_dev, dtype, shape, sizes):
+    q, k, v, dy = make(cuda_dev, *shape, dtype, sizes, seed=shape[2])
+    scale = 1.0 / (8.0 * sizes[0] * sizes[1] * sizes[2])
+    ld = torch.tensor([-0.005, -0.2, -2.0], device=cuda_dev)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    y = fb.decay_linear(*leaves, ld, scale)
+    got = (y, *torch.autograd.grad(y, leaves, dy))
+    ref = [t.detach().double().requires_grad_(True) for t in (q, k, v)]
+    y_ref = O.decay_linear_dense(*ref, ld, scale)
+    want = (y_ref, *torch.autograd.grad(y_ref, ref, dy.double()))
+    top = torch.finfo(dtype).max
+    for x, w in zip(got, want):
+        assert w.abs().max() < top                   # the cases are chosen so that no result leaves its type
+        for h in range(shape[1]):
+            assert off(x[:, h], w[:, h]) <= bound(w[:, h], dtype)
+
+
 @pytest.mark.parametrize("shape", [(1, 1, 9000, 64, 64), (2, 1, 5000, 128, 64)])
 def test_small_values_in_clusters_and_segments(fb, cuda_dev, shape):
     dtype = torch.float16
@@ -60,6 +85,21 @@ def test_small_values_in_clusters_and_segments(fb, cuda_dev, shape):
     y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld, scale, state, lengths)
     assert off(y, y_ref) <= bound(y_ref, dtype)
     assert off(end, end_ref) <= (2e-6 + N ** 0.5 * 2.0 ** -24) * end_ref.norm().item()
+
+
+def test_rows_of_very_different_sizes(fb, cuda_dev):
+    """Every token's outputs are as exact as that token's own size asks for."""
+    q, k, v, _ = make(cuda_dev, 1, 2, 400, 64, 64, torch.float16, (1.0, 0.05, 1.0, 1.0), seed=3)
+    spread = torch.rand(400, 1, generator=torch.Generator(device=cuda_dev).manual_seed(4), device=cuda_dev)
+    q = q * (10.0 ** -(4 * spread)).half()
+    ld = torch.tensor([-0.01, -0.5], device=cuda_dev)
+    scale = 100.0
+    y = fb.decay_linear(q, k, v, ld, scale)
+    ref = O.decay_linear_dense(q.double(), k.double(), v.double(), ld, scale)
+    for h in range(2):
+        for n in range(400):
+            # eight half steps for a single row of 64 outputs, whose sums may cancel
+            assert off(y[0, h, n], ref[0, h, n]) <= 8 * torch.finfo(torch.float16).eps / 2 * ref[0, h, n].norm().item() + 8 * 2.0 ** -25, (h, n)
 
 
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
