@@ -633,8 +633,16 @@ Two scatter_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& z, doub
 // ------------------------------------------------------------------------------------------------
 // autograd of the decayed linear attention and of the rotation
 // ------------------------------------------------------------------------------------------------
+// Forward-mode differentiation: tangents travel beside the operands and are no part of requires_grad.  A result that left them
+// out would read as a derivative of zero.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (has_tangent(*t)) raise_py(PyExc_NotImplementedError, std::string(what) + " has no forward-mode derivative");
+}
 void no_gradient_of(const char* what, const Tensor& t) {
-  if (torch::autograd::compute_requires_grad(t)) raise_py(PyExc_NotImplementedError, std::string(what) + " is not differentiated; pass it detached");
+  if (torch::autograd::compute_requires_grad(t) || has_tangent(t))
+    raise_py(PyExc_NotImplementedError, std::string(what) + " is not differentiated; pass it detached");
 }
 
 class DecayFn : public torch::autograd::Function<DecayFn> {
@@ -658,6 +666,7 @@ class DecayFn : public torch::autograd::Function<DecayFn> {
 };
 Tensor decay_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale, const optional<Tensor>& lengths) {
   no_gradient_of("log_decay", log_decay);
+  no_tangents("flare_b200::decay_fwd", {&q, &k, &v});
   if (!torch::autograd::compute_requires_grad(q, k, v)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return Op_decay_fwd::get().call(q, k, v, log_decay, scale, lengths);
@@ -666,6 +675,7 @@ Tensor decay_fwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, con
 }
 Three decay_bwd_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& dy, const Tensor& log_decay, double scale,
                          const optional<Tensor>& lengths) {
+  no_tangents("flare_b200::decay_bwd", {&q, &k, &v, &dy, &log_decay});
   Three r;
   {
     at::AutoDispatchBelowADInplaceOrView below;
@@ -728,9 +738,15 @@ class RotaryPairFn : public torch::autograd::Function<RotaryPairFn> {
     return out;
   }
 };
+// A rotation is linear: the tangent of its result is the rotated tangent.
 Tensor rotary_autograd(const Tensor& x, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset, bool interleaved, double scale,
                        bool back) {
   no_gradient_of("freqs", freqs);
+  if (has_tangent(x)) {
+    const Tensor y = Op_rotary::get().call(x._fw_primal(0), freqs, positions, offset, interleaved, scale, back);
+    y._set_fw_grad(Op_rotary::get().call(x._fw_grad(0), freqs, positions, offset, interleaved, scale, back), 0, false);
+    return y;
+  }
   if (!torch::autograd::compute_requires_grad(x)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return Op_rotary::get().call(x, freqs, positions, offset, interleaved, scale, back);
@@ -740,6 +756,16 @@ Tensor rotary_autograd(const Tensor& x, const Tensor& freqs, const optional<Tens
 Two rotary_pair_autograd(const Tensor& q, const Tensor& k, const Tensor& freqs, const optional<Tensor>& positions, int64_t offset,
                          bool interleaved, double scale, bool back) {
   no_gradient_of("freqs", freqs);
+  if (has_tangent(q) || has_tangent(k)) {
+    auto primal = [](const Tensor& t) { return has_tangent(t) ? t._fw_primal(0) : t; };
+    Two r = Op_rotary_pair::get().call(primal(q), primal(k), freqs, positions, offset, interleaved, scale, back);
+    auto tangent = [&](const Tensor& x, const Tensor& y) {
+      if (has_tangent(x)) y._set_fw_grad(Op_rotary::get().call(x._fw_grad(0), freqs, positions, offset, interleaved, scale, back), 0, false);
+    };
+    tangent(q, std::get<0>(r));
+    tangent(k, std::get<1>(r));
+    return r;
+  }
   if (!torch::autograd::compute_requires_grad(q, k)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return Op_rotary_pair::get().call(q, k, freqs, positions, offset, interleaved, scale, back);
@@ -1050,6 +1076,8 @@ FLARE_PY(decay_prefill, 7, {
   const double scale = double_arg(a[4]);
   const optional<Tensor> state = optional_arg(a[5]), lengths = optional_arg(a[6]);
   Two r;
+  no_tangents("decay_linear_prefill", {&q, &k, &v, &ld});
+  if (state) no_tangents("decay_linear_prefill", {&*state});
   { pybind11::gil_scoped_release nogil; at::AutoDispatchBelowADInplaceOrView below; r = decay_prefill(q, k, v, ld, scale, state, lengths); }
   return pair(std::get<0>(r), std::get<1>(r));
 })
@@ -1058,6 +1086,7 @@ FLARE_PY(decay_decode, 7, {
   const double scale = double_arg(a[5]);
   const optional<Tensor> lengths = optional_arg(a[6]);
   Tensor y;
+  no_tangents("decay_linear_decode", {&q, &k, &v, &ld, &state});
   { pybind11::gil_scoped_release nogil; at::AutoDispatchBelowADInplaceOrView below; y = decay_decode(q, k, v, ld, state, scale, lengths); }
   return THPVariable_Wrap(std::move(y));
 })

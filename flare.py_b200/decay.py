@@ -33,7 +33,7 @@ def decay_linear_state_init(B: int, H: int, Dk: int, Dv: int, device) -> torch.T
 def decay_linear(q, k, v, log_decay, scale: float = 1.0, lengths=None):
     """y [B,H,N,Dv] of a whole sequence from an empty state; differentiable in q, k and v.
 
-    Nothing of the forward but its operands is kept for the backward.  Works under torch.autocast (q, k, v are cast to the
+    A second derivative and forward mode raise.  Nothing of the forward but its operands is kept for the backward.  Works under torch.autocast (q, k, v are cast to the
     autocast dtype) and inside torch.compile (registered operators ``flare_b200::decay_fwd`` / ``decay_bwd``)."""
     q, k, v = _autocast(q, k, v)
     if torch.compiler.is_compiling():

@@ -59,8 +59,9 @@ def rotary_frequencies(dim: int, base: float = 10_000.0, scaling: Optional[str] 
 
 
 def rotary(x, freqs, positions=None, offset: int = 0, interleaved: bool = False, scale: float = 1.0):
-    """x [B,H,N,D] (fp32, fp16 or bf16, any strides) with its first 2 * len(freqs) features turned; differentiable, any number
-    of times.  freqs: fp64 on x's device.  Token n stands at ``positions[n]`` (int32 or int64; [N], [1,N] or [B,N]) or, without
+    """x [B,H,N,D] (fp32, fp16 or bf16, any strides) with its first 2 * len(freqs) features turned; differentiable by
+    torch.autograd, any number of times, and in forward mode (torch.func's reverse-mode transforms take no native autograd function
+    and raise).  freqs: fp64 on x's device.  Token n stands at ``positions[n]`` (int32 or int64; [N], [1,N] or [B,N]) or, without
     positions, at n; ``offset`` is added to either."""
     if torch.compiler.is_compiling():
         _need_cuda(x)
