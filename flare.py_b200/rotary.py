@@ -35,7 +35,7 @@ def rotary_frequencies(dim: int, base: float = 10_000.0, scaling: Optional[str] 
         raise ValueError(f"dim must be an even number of features, got {dim}")
     if not (base > 0 and factor > 0):
         raise ValueError(f"base and factor must be positive, got {base} and {factor}")
-    exponent = torch.arange(0, dim, 2, dtype=torch.float64) / dim
+    exponent = torch.arange(0, dim, 2, dtype=torch.float64, device="cpu") / dim
     freqs = base ** -exponent
     if scaling is None:
         if factor != 1.0:
@@ -87,12 +87,12 @@ class Rotary(nn.Module):
         super().__init__()
         freqs, self.scale = rotary_frequencies(dim, base, scaling, factor, original_length, turns)
         self.interleaved = bool(interleaved)
-        self._freqs64 = freqs
-        self.register_buffer("freqs", freqs.clone(), persistent=False)
+        self._freqs64 = freqs                                  # on the CPU, wherever the module is built
+        self.register_buffer("freqs", freqs.clone().to(torch.empty(0).device), persistent=False)
 
     def _apply(self, fn, recurse=True):
         super()._apply(fn, recurse)
-        self.freqs = self._freqs64.to(self.freqs.device)       # a cast of the module must not round them
+        self.freqs = self._freqs64.to(self.freqs.device)       # a cast must not round them, nor to_empty leave them unset
         return self
 
     def forward(self, x, positions=None, offset: int = 0):
