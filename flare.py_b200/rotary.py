@@ -91,8 +91,11 @@ class Rotary(nn.Module):
         self.register_buffer("freqs", freqs.clone().to(torch.empty(0).device), persistent=False)
 
     def _apply(self, fn, recurse=True):
+        before = self.freqs
         super()._apply(fn, recurse)
-        self.freqs = self._freqs64.to(self.freqs.device)       # a cast must not round them, nor to_empty leave them unset
+        # A cast must not round them, nor to_empty leave them unset; where nothing moves, the buffer stays: captured graphs read it.
+        stays = self.freqs.device == before.device and before.device.type != "meta"
+        self.freqs = before if stays else self._freqs64.to(self.freqs.device, copy=True)
         return self
 
     def forward(self, x, positions=None, offset: int = 0):

@@ -35,3 +35,39 @@ def test_the_default_device_is_the_buffers_not_the_functions():
         assert fb.rotary_frequencies(16, scaling="by_parts", factor=2.0, original_length=64)[0].device.type == "cpu"
     finally:
         torch.set_default_device(None)
+
+
+def test_a_move_that_is_none_leaves_the_buffer_where_it_is():
+    """A captured graph reads the frequencies at their address: casting a model, or moving it to where it is, must not change it."""
+    rope = fb.Rotary(16)
+    at = rope.freqs.data_ptr()
+    net = torch.nn.Sequential(rope)
+    for move in (lambda: net.half(), lambda: net.float(), lambda: net.to("cpu"), lambda: net.to(torch.bfloat16), lambda: net.double(),
+                 lambda: net.cpu(), lambda: net.to_empty(device="cpu")):
+        move()
+        right(rope)
+        assert rope.freqs.data_ptr() == at
+    net.share_memory()
+    assert rope.freqs.is_shared()
+    right(rope)
+    # and what a user does to the buffer of one module stays with it
+    other = fb.Rotary(16).to("meta").to_empty(device="cpu")
+    other.freqs.zero_()
+    right(other.to("meta").to_empty(device="cpu"))
+
+
+@pytest.mark.gpu
+def test_a_captured_graph_outlives_a_move_to_the_same_device(cuda_dev):
+    rope = fb.Rotary(16).to(cuda_dev)
+    x = torch.randn(1, 2, 9, 16, device=cuda_dev)
+    rope(x)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = rope(x)
+    at = rope.freqs.data_ptr()
+    rope.to(cuda_dev).half().float()
+    assert rope.freqs.data_ptr() == at
+    fill = [torch.full((8,), 7.0, dtype=torch.float64, device=cuda_dev) for _ in range(64)]   # whatever was freed is used again
+    graph.replay()
+    assert torch.equal(y, rope(x)) and len(fill) == 64
