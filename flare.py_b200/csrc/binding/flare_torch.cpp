@@ -69,16 +69,17 @@ void same_dtype(const char* msg, std::initializer_list<const Tensor*> ts) {
 
 // Whether the kernels can address t in place: unit stride on the last dimension, 16-byte aligned rows, no broadcast
 // (stride 0) dimension -- a TMA tensor map cannot describe one.
-bool addressable(const Tensor& t) {
+bool addressable_strides(const Tensor& t) {
   const auto st = t.strides();
   const auto sz = t.sizes();
   const int64_t e = t.element_size(), nd = t.dim();
   if (nd == 0) raise_py(PyExc_IndexError, "expected a tensor of four dimensions, got a scalar");
-  if (st[nd - 1] != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  if (st[nd - 1] != 1) return false;
   for (int64_t i = 0; i + 1 < nd; ++i)
     if ((st[i] * e) % 16 || (st[i] == 0 && sz[i] != 1)) return false;
   return true;
 }
+bool addressable(const Tensor& t) { return addressable_strides(t) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 Tensor tok(const Tensor& t) { return addressable(t) ? t : t.contiguous(); }
 
 // q as [H,M,D] (latents shared by the batch) or [B,H,M,D]; an expand()-ed batch is folded back.
@@ -297,11 +298,20 @@ Tensor decay_rows(const Tensor& t) {
   return t;
 }
 
+// The result beside an operand that decay_rows made of t.  Its strides follow from t's alone, never from t's address: the shapes that
+// the compiler works with (register_fake in decay.py) know no address.
+Tensor beside(const Tensor& t, const Tensor& rows) {
+  const bool moved = t.element_size() == 2 && t.size(-1) % 8 == 0 && t.stride(-1) == 1 && addressable_strides(t);
+  return like_tokens(moved ? t : rows);
+}
+
 // The operands of a call: checked, laid out, and the C description of them.
 struct Decay {
   Tensor q, k, v, log_decay, lengths;
+  const Tensor &q_given, &k_given, &v_given;
   FlareDecay p{};
-  Decay(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& ld, double scale, const optional<Tensor>& len) {
+  Decay(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& ld, double scale, const optional<Tensor>& len)
+      : q_given(q_), k_given(k_), v_given(v_) {
     for (const Tensor* t : {&q_, &k_, &v_, &ld}) need_cuda(*t);
     for (const Tensor* t : {&q_, &k_, &v_})
       if (t->dim() != 4) raise_py(PyExc_ValueError, "q, k, v must be [B,H,N,D]");
@@ -327,6 +337,9 @@ struct Decay {
       lengths = (len->scalar_type() == at::kInt ? *len : len->clamp(0, p.N).to(at::kInt)).contiguous();
     }
   }
+  Tensor like_q() const { return beside(q_given, q); }
+  Tensor like_k() const { return beside(k_given, k); }
+  Tensor like_v() const { return beside(v_given, v); }
   const int32_t* len() const { return lengths.defined() ? static_cast<const int32_t*>(lengths.data_ptr()) : nullptr; }
   bool empty() const { return p.B == 0 || p.H == 0 || p.N == 0; }
   void check_state(const Tensor& s) const {
@@ -338,7 +351,7 @@ struct Decay {
 };
 
 Tensor decay_run(Decay& d, const float* state_in, float* state_out) {
-  Tensor y = like_tokens(d.v);
+  Tensor y = d.like_v();
   set_stride(d.p.y_stride, y);
   const size_t bytes = flare_decay_workspace_bytes(&d.p);
   const Tensor ws = bytes ? scratch(bytes, d.k) : Tensor();
@@ -350,7 +363,7 @@ Tensor decay_run(Decay& d, const float* state_in, float* state_out) {
 Tensor decay_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, double scale, const optional<Tensor>& lengths) {
   c10::cuda::CUDAGuard guard(k.device());
   Decay d(q, k, v, log_decay, scale, lengths);
-  if (d.empty()) return like_tokens(d.v);
+  if (d.empty()) return d.like_v();
   return decay_run(d, nullptr, nullptr);
 }
 
@@ -361,7 +374,7 @@ Three decay_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   if (dy_.sizes() != v.sizes() || dy_.scalar_type() != v.scalar_type() || dy_.device() != v.device())
     raise_py(PyExc_ValueError, "dy must have the shape, dtype and device of v");
   const Tensor dy = decay_rows(dy_);
-  Tensor dq = like_tokens(d.q), dk = like_tokens(d.k), dv = like_tokens(d.v);
+  Tensor dq = d.like_q(), dk = d.like_k(), dv = d.like_v();
   if (d.empty()) return {dq, dk, dv};
   set_stride(d.p.dy_stride, dy); set_stride(d.p.dq_stride, dq); set_stride(d.p.dk_stride, dk); set_stride(d.p.dv_stride, dv);
   const size_t bytes = flare_decay_bwd_workspace_bytes(&d.p);
@@ -383,7 +396,7 @@ Two decay_prefill(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
     d.check_state(before);
   }
   if (d.empty()) {
-    return {like_tokens(d.v), before.defined() ? before.clone() : at::zeros({d.p.B, d.p.H, d.p.Dk, d.p.Dv}, d.k.options().dtype(at::kFloat))};
+    return {d.like_v(), before.defined() ? before.clone() : at::zeros({d.p.B, d.p.H, d.p.Dk, d.p.Dv}, d.k.options().dtype(at::kFloat))};
   }
   Tensor after = f32({d.p.B, d.p.H, d.p.Dk, d.p.Dv}, d.k);
   Tensor y = decay_run(d, before.defined() ? fp(before) : nullptr, fp(after));
@@ -396,7 +409,7 @@ Tensor decay_decode(const Tensor& q, const Tensor& k, const Tensor& v, const Ten
   c10::cuda::CUDAGuard guard(k.device());
   Decay d(q, k, v, log_decay, scale, lengths);
   d.check_state(state);
-  Tensor y = like_tokens(d.v);
+  Tensor y = d.like_v();
   if (d.empty()) return y;
   set_stride(d.p.y_stride, y);
   check_rc(flare_decay_decode(&d.p, d.q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), fp(d.log_decay), d.len(), y.data_ptr(), fp(state),

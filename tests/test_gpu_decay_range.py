@@ -139,3 +139,36 @@ def test_a_key_that_is_not_finite_leaves_the_tokens_before_it(fb, cuda_dev):
         y = fb.decay_linear(q, k, v, ld, 0.125)
         assert off(y[:, :, :200], ref[:, :, :200]) <= bound(ref[:, :, :200], dtype)
         assert not y[:, :, 200:].isfinite().any()
+
+
+def test_the_strides_of_results_do_not_depend_on_an_address(fb, cuda_dev):
+    """What the compiler assumes of a result (strides from strides) holds for operands off any 16-byte boundary."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    B, H, N, D = 2, 3, 140, 64
+    ops = torch.ops.flare_b200
+    ld = torch.tensor([-0.01, -0.2, -1.0], device=cuda_dev)
+    store = torch.randn(B * N * H * D * 2 + 16, device=cuda_dev).bfloat16()
+    layouts = {"heads inside": (N * H * D, D, H * D, 1), "dense": (H * N * D, N * D, D, 1), "packed": (2 * N * H * D, D, 2 * H * D, 1),
+               "shared": (N * H * D, 0, H * D, 1), "odd rows": (H * N * (D + 1), N * (D + 1), D + 1, 1), "transposed": (H * N * D, N * D, 1, N)}
+    for name, strides in layouts.items():
+        for offset in (0, 1, 4, 8):
+            x = store.as_strided((B, H, N, D), strides, offset)
+            got = (ops.decay_fwd(x, x, x, ld, 0.1, None), *ops.decay_bwd(x, x, x, x, ld, 0.1, None))
+            with FakeTensorMode() as mode:
+                f, g = mode.from_tensor(x), mode.from_tensor(ld)
+                want = (ops.decay_fwd(f, f, f, g, 0.1, None), *ops.decay_bwd(f, f, f, f, g, 0.1, None))
+            for a, b in zip(got, want):
+                assert a.stride() == b.stride() and a.shape == b.shape and a.dtype == b.dtype, (name, offset)
+            ref = O.decay_linear_dense(x.double(), x.double(), x.double(), ld, 0.1)
+            assert off(got[0], ref) <= bound(ref, x.dtype), (name, offset)
+    x = store.as_strided((B, H, N, D), layouts["heads inside"], 1).requires_grad_(True)
+    fn = torch.compile(lambda t: fb.decay_linear(t, t, t, ld, 0.1).transpose(1, 2).reshape(B, N, H * D) * 2, fullgraph=True)
+    y, want = fn(x), fb.decay_linear(x, x, x, ld, 0.1).transpose(1, 2).reshape(B, N, H * D) * 2
+    assert torch.equal(y, want)
+    # x is q, k and v at once: the three gradients, the same to the bit either way, are added up in bf16 one after the other in
+    # eager mode, in the compiler's order and width otherwise.  Either sum rounds twice at most, by 2^-8 of a partial sum that the sum
+    # of magnitudes bounds: 4 * 2^-8 of that between them.
+    parts = ops.decay_bwd(x.detach(), x.detach(), x.detach(), torch.full_like(x, 2.0), ld, 0.1, None)
+    size = sum(p.double().abs() for p in parts)
+    got, eager = (torch.autograd.grad(t.sum(), x)[0].double() for t in (y, want))
+    assert ((got - eager).abs() <= 4 * 2.0 ** -8 * size).all()
