@@ -713,7 +713,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     // ---- outputs -------------------------------------------------------------------------------------------------------
     const int w = warp & 3, r = 32 * w + lane;     // token
     const uint32_t y_at = tmem + ((uint32_t)(32 * w) << 16) + L::cY, x_at = y_at + (L::cYx - L::cY);
-    const float wx = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
+    const float wx_full = a.scale * exp2f(g2 * (float)(rev ? kL - r : r + 1));
     T* out = static_cast<T*>(u.out) + b * u.os[0] + h * u.os[1] + c0;
     const int cols = u.Dc - c0;                    // of the 64 columns, those that exist
     uint8_t* tile = smem + L::oOut + w * 4096;     // the warp's [32 rows][64], swizzled: piece k of a row at row ^ 16 k
@@ -728,6 +728,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       wait_together<5, 128>(wait, w == 0, bFree + ra.at, ra.phase);
       ra.next();
       tc_fence_after();
+      // of a mirrored chunk that ends early: by the tokens there are, so that growth (log_decay above 0) stays in range
+      const float wx = rev && cnt < kL ? a.scale * exp2f(g2 * (float)max(0, cnt - r)) : wx_full;
       const F2 fx = both(kHalfRange ? wx * sExp[i & 3] : wx), scale2 = both(kHalfRange ? a.scale * power_of_two(sPow[128 * (i & 3) + r]) : 1.f);
       uint32_t y[16], x[16];
       tmem_ld16(y_at, y);
@@ -1035,8 +1037,9 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
     // The weight lambda^(i-j) of a block of 16 columns is a factor of the column times one of the row and the block.  On the
     // diagonal the latter exceeds 1, up to lambda^-15, and the former makes up for it: products as small as 2^-66 stay normal
     // numbers on the way for every decay above 2^-4 a token; stronger ones take an exponential for each value there.
-    // Columns behind the length are zero in S already: its rows of b were cleared.
-    const bool mild = g2 >= -4.f;
+    // Columns behind the length are zero in S already: its rows of b were cleared.  The mirrored walk, whose weights grow towards
+    // them where log_decay is above 0, leaves them out all the same: a weight beyond the range of 32 bits would make them NaN.
+    const bool mild = fabsf(g2) <= 4.f;
     F2 wcol[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k)
@@ -1046,10 +1049,12 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       wait_together<2, 256>(wait, warp == 3, bS + (i & 1), i >> 1);
       tc_fence_after();
       uint32_t top = 0;
+      const int cnt = rev ? sp.live(chunk(i)) : kL;
+      auto none_of = [&](int j0) { return rev ? j0 + 15 < r0 || j0 >= cnt : j0 > r0 + 31; };
 #pragma unroll 1
       for (int k = 0; k < 4; ++k) {
         const int j0 = 64 * hb + 16 * k;           // the block's first column; the warp's rows are r0 ... r0 + 31
-        const bool none = rev ? j0 + 15 < r0 : j0 > r0 + 31, all = rev ? j0 >= r0 + 31 : j0 + 15 <= r0;
+        const bool none = none_of(j0), all = rev ? j0 >= r0 + 31 && j0 + 15 < cnt : j0 + 15 <= r0;
         uint32_t p[8];
         if (none) {
           if constexpr (kHalfRange) continue;
@@ -1083,7 +1088,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
             }
             if (rev) {
 #pragma unroll
-              for (int m = 0; m < 16; ++m) v[m] = m >= t ? v[m] : 0u;
+              for (int m = 0; m < 16; ++m) v[m] = m >= t && m < cnt - j0 ? v[m] : 0u;
             } else {
 #pragma unroll
               for (int m = 0; m < 16; ++m) v[m] = m <= t ? v[m] : 0u;
@@ -1099,8 +1104,8 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
 #pragma unroll
               for (int q = 0; q < 8; ++q)
                 if (q == m) { s0 = v[2 * q]; s1 = v[2 * q + 1]; }
-              const float x0 = d0 >= 0 ? __uint_as_float(s0) * (scale_p * exp2f(g2 * (float)d0)) : 0.f;
-              const float x1 = d1 >= 0 ? __uint_as_float(s1) * (scale_p * exp2f(g2 * (float)d1)) : 0.f;
+              const float x0 = d0 >= 0 && j0 + 2 * m < cnt ? __uint_as_float(s0) * (scale_p * exp2f(g2 * (float)d0)) : 0.f;
+              const float x1 = d1 >= 0 && j0 + 2 * m + 1 < cnt ? __uint_as_float(s1) * (scale_p * exp2f(g2 * (float)d1)) : 0.f;
               const uint32_t t = Op16<T>::pack(x0, x1);
 #pragma unroll
               for (int q = 0; q < 8; ++q)
@@ -1133,7 +1138,7 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
         for (int k = 0; k < 4; ++k) {
           const int j0 = 64 * hb + 16 * k;
           uint32_t p[8];
-          if (rev ? j0 + 15 < r0 : j0 > r0 + 31) {
+          if (none_of(j0)) {
 #pragma unroll
             for (int m = 0; m < 8; ++m) p[m] = 0u;
           } else {

@@ -172,3 +172,31 @@ def test_the_strides_of_results_do_not_depend_on_an_address(fb, cuda_dev):
     size = sum(p.double().abs() for p in parts)
     got, eager = (torch.autograd.grad(t.sum(), x)[0].double() for t in (y, want))
     assert ((got - eager).abs() <= 4 * 2.0 ** -8 * size).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N,rates", [(7, (0.02, 1.4, 7.0)), (2, (0.5, 6.0, 20.0)), (37, (0.1, 0.8, 1.5)), (130, (0.02, 0.3, 0.5)), (300, (0.01, 0.05, 0.2))])
+def test_growth(fb, cuda_dev, dtype, D, N, rates):
+    """log_decay above 0: weights of tokens that do not exist may overflow, those of tokens that do must not suffer from it."""
+    H = len(rates)
+    q, k, v, dy = make(cuda_dev, 2, H, N + 5, D, D, dtype, (1.0, 1.0, 1.0, 1.0), seed=N)
+    lengths = torch.tensor([N, N - 1], device=cuda_dev)
+    live = (torch.arange(N + 5, device=cuda_dev) < lengths[:, None])[:, None, :, None]
+    for h, rate in enumerate(rates):                 # a head at a time: the scale keeps its results in the type's range
+        ld = torch.tensor([rate], device=cuda_dev)
+        scale = float(torch.exp(-ld * (N - 1))) / 64
+        one = [t[:, h:h + 1].clone().requires_grad_(True) for t in (q, k, v)]
+        y = fb.decay_linear(*one, ld, scale, lengths)
+        got = (y, *torch.autograd.grad(y, one, dy[:, h:h + 1]))
+        ref = [torch.where(live, t.detach().double(), 0.0).requires_grad_(True) for t in one]
+        y_ref = O.decay_linear_dense(*ref, ld, scale, lengths)
+        want = (y_ref, *torch.autograd.grad(y_ref, ref, torch.where(live, dy[:, h:h + 1].double(), 0.0)))
+        # the exponent rate * n * log2(e) is rounded at 2^-24 of itself, twice
+        slack = rate * N * 2.0 ** -23
+        for x, w in zip(got, want):
+            small = w.numel() ** 0.5 * 2.0 ** -25 if dtype == torch.float16 else 0.0
+            assert off(x, w) <= ((0 if dtype == torch.float32 else torch.finfo(dtype).eps) + 8e-6 + slack) * w.norm().item() + small, rate
+        end = fb.decay_linear_prefill(*[t.detach() for t in one], ld, scale, lengths=lengths)[1]
+        end_ref = O.decay_linear_recurrent(*[t.detach() for t in one], ld, scale, lengths=lengths)[1]
+        assert off(end, end_ref) <= (1e-5 + slack) * end_ref.norm().item(), rate
