@@ -200,3 +200,25 @@ def test_growth(fb, cuda_dev, dtype, D, N, rates):
         end = fb.decay_linear_prefill(*[t.detach() for t in one], ld, scale, lengths=lengths)[1]
         end_ref = O.decay_linear_recurrent(*[t.detach() for t in one], ld, scale, lengths=lengths)[1]
         assert off(end, end_ref) <= (1e-5 + slack) * end_ref.norm().item(), rate
+
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 2, 0, 64, 64), (0, 2, 5, 64, 64), (2, 0, 5, 64, 64)])
+def test_empty_calls_answer_in_full(fb, cuda_dev, shape, dtype):
+    B, H, N, Dk, Dv = shape
+    q, k, v, dy = make(cuda_dev, *shape, dtype, (1.0, 1.0, 1.0, 1.0), seed=1)
+    ld = torch.full((H,), -0.1, device=cuda_dev)
+    state = torch.randn(B, H, Dk, Dv, device=cuda_dev)
+    before = state.clone()
+    y, end = fb.decay_linear_prefill(q, k, v, ld, state=state)
+    assert y.shape == v.shape and y.dtype == dtype
+    assert end.shape == state.shape and torch.equal(end, before) and torch.equal(state, before)
+    if state.numel():
+        assert end.data_ptr() != state.data_ptr()
+    y, end = fb.decay_linear_prefill(q, k, v, ld)
+    assert y.shape == v.shape and end.shape == state.shape and not end.any()
+    assert fb.decay_linear_decode(q, k, v, ld, state).shape == v.shape and torch.equal(state, before)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    for g, t in zip(torch.autograd.grad(fb.decay_linear(*leaves, ld), leaves, dy), leaves):
+        assert g.shape == t.shape and g.dtype == dtype
