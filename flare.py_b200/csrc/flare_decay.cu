@@ -4,8 +4,8 @@
 // flare_decay_tc.cu do not take), the scan over segments, and the single-token form.
 //
 // The token axis is cut into segments, a CTA each (two CTAs fit an SM).  With one segment a CTA walks its whole sequence; with
-// several, pass 1 adds up every segment (sum of lambda^(end-1-n) b_n c_n^T), k_decay_prefix turns the sums into the states
-// before the segments, and pass 2 walks all segments side by side.  A walk takes 64 tokens at a time:
+// several, pass 1 adds up every segment (sum of lambda^(end-1-n) b_n c_n^T; the last one walked too, which nothing reads),
+// k_decay_prefix turns the sums into the states before the segments, and pass 2 walks all segments side by side.  A walk takes 64 tokens at a time:
 //     out = (lambda^(i-j) (a_i . b_j))_{j <= i} C  +  lambda^(i+1) A S,      S <- lambda^64 S + (lambda^(63-j) B)^T C
 // The mirror image (n >= t) of the gradients is the same walk over rows taken from the end.
 #include <cstdarg>
@@ -500,7 +500,9 @@ int run_decode(const DecodeArgs& a0, cudaStream_t st) {
 int pick_segments(int B, int H, int N, int Dc, int n_units) {
   const int cb = (Dc + 63) / 64;
   const long long ctas = (long long)B * H * cb * n_units;
-  long long s = 2LL * num_sms() / ctas;                      // the two CTAs that an SM holds
+  // Two CTAs an SM and blocks of 64 columns are what up to 124 features have.  Of 125 to 128 one CTA fits (117 kB of shared memory), of
+  // more the blocks are 32 columns wide and above 164 one CTA fits again: those grids take two to four waves.
+  long long s = 2LL * num_sms() / ctas;
   const long long max_s = ((long long)N + kSub - 1) / kSub;
   if (s > max_s) s = max_s;
   if (s > 256) s = 256;

@@ -6,7 +6,8 @@
 // one or two tensors (q and k) one after the other.  Angles made once a block, in shared memory, were slower (81 against 55 us
 // for q and k at B = 4, H = 16, N = 8192, D = 64 bf16: two more dependent accesses a head), and so were the loads of four heads
 // ahead of their use (82 us: at 111 registers too few threads fit).
-// What bounds it is HBM: every element is read and written once, 16 bytes an access; 4.9 TB/s at that size, 74 % of a copy's.
+// Every element is read and written once, 16 bytes an access; 4.9 TB/s at that size, 74 % of a copy's.  What bounds it is the loads'
+// latency: a thread has one head's access in flight, as an output may be its input and loads do not pass stores.
 #include <cstdarg>
 #include <cstdio>
 #include "common.cuh"
