@@ -445,8 +445,10 @@ k_decay_tc_sums(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       if (warp == 1) wait(bFull + ring.at, ring.phase);
       if constexpr (kHalfRange) {
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        const uint32_t top = __reduce_max_sync(0xffffffffu, r < cnt ? top_of_row(r, 4 * half, 4, w, smem + L::oC + ring.at * kBlk) : 0u);
+        const uint32_t own = r < cnt ? top_of_row(r, 4 * half, 4, w, smem + L::oC + ring.at * kBlk) : 0u;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, own);
         if ((tid & 31) == 0) sTop[warp] = top;
+        if (own == 0) w = 0.f;                     // zeros weigh nothing: under growth w times the power of two might overflow
       }
       if (warp == 1 && c > 1) wait(bKv + (c & 1), (c - 2) >> 1);       // the product with what stood here is done
       asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -1008,8 +1010,10 @@ k_decay_tc_walk(const __grid_constant__ DecayMaps maps, const __grid_constant__ 
       }
       if constexpr (kHalfRange) {                  // while the product with what stands in w_t may still run
         asm volatile("bar.sync 3, 128;" ::: "memory");
-        const uint32_t top = __reduce_max_sync(0xffffffffu, r < cnt ? top_of_row(r, 0, width / 8, w, smem + L::oC + ra.at * kBlk) : 0u);
+        const uint32_t own = r < cnt ? top_of_row(r, 0, width / 8, w, smem + L::oC + ra.at * kBlk) : 0u;
+        const uint32_t top = __reduce_max_sync(0xffffffffu, own);
         if (lane == 0) sTop[warp & 3] = top;
+        if (own == 0) w = 0.f;                     // zeros weigh nothing: under growth w times the power of two might overflow
       }
       for (int part = 0; part < parts; ++part, ++ev) {
         // the product with what stood here is done: the event before the last one, or the last where either takes both tiles

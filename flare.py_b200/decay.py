@@ -13,7 +13,8 @@ taken as they are); Dk, Dv up to 256.  ``log_decay``: [H], a constant of the mod
 decay, -inf leaves a token itself alone.  ``lengths``: int32 (or int64) [B]; tokens at or behind ``lengths[b]`` -- padding,
 which may hold anything -- leave the state alone and have outputs and gradients of zero.  A value that is not finite among the
 live tokens spoils the outputs of the 128-token chunk it stands in, also those before it.  Products, weighted values and states of
-fp16 operands carry powers of two of their own, so that small and large ones keep their bits; results are fp16's.
+fp16 operands carry powers of two of their own, so that small and large ones keep their bits; results are fp16's.  Weighted
+products of one token that are 2^37 times smaller than its largest do not (under strong growth, where what is large meets zeros in v).
 """
 from __future__ import annotations
 

@@ -222,3 +222,31 @@ def test_empty_calls_answer_in_full(fb, cuda_dev, shape, dtype):
     leaves = [t.requires_grad_(True) for t in (q, k, v)]
     for g, t in zip(torch.autograd.grad(fb.decay_linear(*leaves, ld), leaves, dy), leaves):
         assert g.shape == t.shape and g.dtype == dtype
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,N", [(64, 128), (64, 100), (128, 128), (128, 250)])
+def test_growth_over_tokens_of_zero(fb, cuda_dev, dtype, D, N):
+    """Zeros weigh nothing, however large the weight of their place is; v (or dy) is zero but for the last (the first) token, or all."""
+    q, k, v, dy = make(cuda_dev, 1, 2, N, D, D, dtype, (1.0, 1.0, 1e-5, 1e-5), seed=N)
+    ld = torch.tensor([0.5, 0.6], device=cuda_dev) * 128 / max(N, 128)
+    v[:, :, :-1] = 0
+    dy[:, :, 1:] = 0
+    def limit(a, b, c, w):
+        """fp16: a token's products are rounded as numbers of which the largest is 2^13 or more, by half of 2^-24 at least: by 2^-38
+        of the largest.  Times the values they meet."""
+        if dtype != torch.float16:
+            return bound(w, dtype)
+        n = torch.arange(N, device=cuda_dev)
+        weight = torch.exp(ld.double()[:, None, None] * (n[:, None] - n)).tril()
+        largest = (a.double() @ b.double().transpose(-1, -2) * weight).abs().amax(-1, keepdim=True)
+        return bound(w, dtype) + 1e4 * 2.0 ** -38 * (largest * c.double().abs().cumsum(2)).norm().item()
+
+    y, end = fb.decay_linear_prefill(q, k, v, ld, 1e4)
+    y_ref, end_ref = O.decay_linear_recurrent(q, k, v, ld, 1e4)
+    assert off(y, y_ref) <= limit(q, k, v, y_ref) and off(end, end_ref) <= 1e-5 * end_ref.norm().item()
+    got = torch.ops.flare_b200.decay_bwd(q, k, torch.randn_like(v), dy, ld, 1e4, None)[2]
+    back = O.decay_linear_recurrent(k.flip(2), q.flip(2), dy.flip(2), ld, 1e4)[0].flip(2)
+    assert off(got, back) <= limit(k.flip(2), q.flip(2), dy.flip(2), back)
+    y, end = fb.decay_linear_prefill(q, k, torch.zeros_like(v), ld, 1e4)
+    assert not y.any() and not end.any()
