@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(256) k_decay_prefix(const __grid_constant__ De
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int seg = u.rev ? a.n_seg - 1 - s0 - j : s0 + j;
-      x[j] = s0 + j < a.n_seg ? s[(long long)seg * per] : 0.f;
+      x[j] = s0 + j + 1 < a.n_seg ? s[(long long)seg * per] : 0.f;     // the last one walked has no sum, or one that nobody needs
     }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {

@@ -250,3 +250,33 @@ def test_growth_over_tokens_of_zero(fb, cuda_dev, dtype, D, N):
     assert off(got, back) <= limit(k.flip(2), q.flip(2), dy.flip(2), back)
     y, end = fb.decay_linear_prefill(q, k, torch.zeros_like(v), ld, 1e4)
     assert not y.any() and not end.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_results_do_not_depend_on_what_a_workspace_held(fb, cuda_dev, dtype):
+    """The C entries with workspaces full of NaN: a sequence in segments, forward with a state and backward."""
+    import ctypes as C
+    from flare_b200 import _cabi
+    B, H, N, Dk, Dv = 1, 2, 9000, 64, 32
+    q, k, v, dy = make(cuda_dev, B, H, N, Dk, Dv, dtype, (1.0, 1.0, 1.0, 1.0), seed=2)
+    ld, state = torch.tensor([-0.001, -0.1], device=cuda_dev), torch.randn(B, H, Dk, Dv, device=cuda_dev)
+    lengths = torch.tensor([N - 77], device=cuda_dev, dtype=torch.int32)
+    y, end, dq, dk, dv = torch.empty_like(v), torch.empty_like(state), torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    p = _cabi.FlareDecay(B=B, H=H, N=N, Dk=Dk, Dv=Dv, dtype=_cabi.DTYPE_CODE[dtype], scale=0.125)
+    for name, t in dict(q=q, k=k, v=v, y=y, dy=dy, dq=dq, dk=dk, dv=dv).items():
+        getattr(p, f"{name}_stride")[:] = t.stride()[:3]
+    stream = torch.cuda.current_stream().cuda_stream
+    at = lambda t: t.data_ptr()
+    for bytes_of, call in ((_cabi.lib.flare_decay_workspace_bytes, lambda ws, n: _cabi.lib.flare_decay_fwd(
+            C.byref(p), at(q), at(k), at(v), at(ld), at(lengths), at(y), at(state), at(end), ws, n, stream)),
+            (_cabi.lib.flare_decay_bwd_workspace_bytes, lambda ws, n: _cabi.lib.flare_decay_bwd(
+                C.byref(p), at(q), at(k), at(v), at(dy), at(ld), at(lengths), at(dq), at(dk), at(dv), ws, n, stream))):
+        n = bytes_of(C.byref(p))
+        assert n > 0                                 # the sequence is cut
+        ws = torch.full((n // 4,), float("nan"), device=cuda_dev)
+        assert call(ws.data_ptr(), n) == 0
+        torch.cuda.synchronize()
+    want_y, want_end = fb.decay_linear_prefill(q, k, v, ld, 0.125, state=state, lengths=lengths)
+    assert torch.equal(y, want_y) and torch.equal(end, want_end)
+    for got, want in zip((dq, dk, dv), torch.ops.flare_b200.decay_bwd(q, k, v, dy, ld, 0.125, lengths)):
+        assert torch.equal(got, want)
