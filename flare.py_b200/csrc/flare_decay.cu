@@ -5,7 +5,8 @@
 //
 // The token axis is cut into segments, a CTA each (two CTAs fit an SM).  With one segment a CTA walks its whole sequence; with
 // several, pass 1 adds up every segment (sum of lambda^(end-1-n) b_n c_n^T; the last one walked too, which nothing reads),
-// k_decay_prefix turns the sums into the states before the segments, and pass 2 walks all segments side by side.  A walk takes 64 tokens at a time:
+// k_decay_prefix turns the sums into the states before the segments, and pass 2 walks all segments side by side.  A walk takes 64
+// tokens at a time:
 //     out = (lambda^(i-j) (a_i . b_j))_{j <= i} C  +  lambda^(i+1) A S,      S <- lambda^64 S + (lambda^(63-j) B)^T C
 // The mirror image (n >= t) of the gradients is the same walk over rows taken from the end.
 #include <cstdarg>
